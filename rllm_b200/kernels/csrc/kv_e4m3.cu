@@ -1,0 +1,179 @@
+// Writing a cache that is kept in 8 bits, and reading it back (see kv_e4m3.cuh for what a row becomes).
+#include "kv_e4m3.cuh"
+
+// ---------------------------------------------------------------------------
+// write: rotation of q, rotation and quantisation of k, quantisation of v
+// ---------------------------------------------------------------------------
+// One block a token, one warp a row (a query, key or value head of the token); a lane holds the dims lane, lane + 32, ...
+// in registers, so a row is read once.  The angles are made once for all heads.  Any head size up to 256 and any rotary_dim.
+template <typename T>
+__global__ void __launch_bounds__(256)
+kv_e4m3_write_kernel(const T* qkv, T* q_out, long long q_stride, const int* __restrict__ positions,
+                     const int* __restrict__ token_seq, const double* __restrict__ inv_freq, int rotary_dim,
+                     const int* __restrict__ block_table, int max_blocks, int num_seqs, unsigned char* __restrict__ kcache,
+                     unsigned char* __restrict__ vcache, unsigned char* __restrict__ kscale,
+                     unsigned char* __restrict__ vscale, int nq, int nkv, int d, int page_size, int num_pages,
+                     int* __restrict__ err) {
+  extern __shared__ float cs[];  // cos[rd/2], sin[rd/2]
+  pdl_wait_on(qkv, positions, token_seq, block_table, q_out);
+  pdl_launch();
+  const int t = blockIdx.x;
+  const int pos = positions[t];
+  const int half = rotary_dim >> 1;
+  for (int i = threadIdx.x; i < half; i += blockDim.x) {
+    if (sizeof(T) == 4) {            // the true 32-bit path: float64 cosine and sine, rounded once
+      double s, c;
+      sincos((double)pos * inv_freq[i], &s, &c);
+      cs[i] = (float)c;
+      cs[half + i] = (float)s;
+    } else {
+      rope_cos_sin(pos, inv_freq[i], &cs[i], &cs[half + i]);
+    }
+  }
+  __syncthreads();
+  const int seq = token_seq[t];
+  long long slot = -1;               // row of kv head 0; a head further: page_size rows on
+  if (pos >= 0 && pos / page_size < max_blocks && seq >= 0 && seq < num_seqs) {
+    const int page = block_table[(size_t)seq * max_blocks + pos / page_size];
+    if (page >= 0 && page < num_pages) slot = (long long)page * nkv * page_size + pos % page_size;
+  }
+  if (slot < 0 && threadIdx.x == 0) atomicOr(err, 2);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const T* row = qkv + (size_t)t * (nq + 2 * nkv) * d;
+  const int heads = slot < 0 ? nq : nq + 2 * nkv;
+  for (int h = warp; h < heads; h += blockDim.x >> 5) {
+    const T* src = row + (size_t)h * d;
+    const bool turned = h < nq + nkv;
+    float x[8];
+    float top = 0.f;
+    bool odd = false;                // an infinity or a NaN
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int i = lane + 32 * k;
+      if (i < d) {
+        float v = to_f32(src[i]);
+        if (turned && i < rotary_dim) {
+          if (i < half) v = v * cs[i] - to_f32(src[i + half]) * cs[half + i];
+          else          v = v * cs[i - half] + to_f32(src[i - half]) * cs[i];
+        }
+        x[k] = v;
+        top = fmaxf(top, fabsf(v));
+        odd = odd || !(fabsf(v) <= 3.402823466e38f);
+      }
+    }
+    if (h < nq) {
+      __syncwarp();                  // q_out may be the row itself: all of it has been read
+      T* dst = q_out + (size_t)t * q_stride + (size_t)h * d;
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (lane + 32 * k < d) dst[lane + 32 * k] = from_f32<T>(x[k]);
+      continue;
+    }
+    top = warp_max(top);
+    odd = __any_sync(0xffffffffu, odd);
+    const int byte = odd ? KV8_NAN_SCALE : kv8_scale_byte(top);
+    const float inv = odd ? 0.f : kv8_inverse(byte);
+    const long long r = slot + (long long)(turned ? h - nq : h - nq - nkv) * page_size;
+    unsigned char* dst = (turned ? kcache : vcache) + r * d;
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (lane + 32 * k < d) dst[lane + 32 * k] = odd ? (unsigned char)0 : (unsigned char)(kv8_pack2(x[k] * inv, 0.f) & 0xffu);
+    if (lane == 0) (turned ? kscale : vscale)[r] = (unsigned char)byte;
+  }
+}
+
+RLLM_EXPORT int rllm_kv_e4m3_write(const void* qkv, int dtype, void* q_out, long long q_stride, const int* positions,
+                                   const int* token_seq, const double* inv_freq, int rotary_dim, const int* block_table,
+                                   int max_blocks, int num_seqs, void* kcache, void* vcache, void* kscale, void* vscale,
+                                   int T, int nq, int nkv, int d, int page_size, int num_pages, int* err,
+                                   cudaStream_t stream) {
+  if (T <= 0) return 0;
+  if (!qkv || !q_out || !positions || !token_seq || !block_table || !kcache || !vcache || !kscale || !vscale || !err ||
+      nq <= 0 || nkv <= 0 || d <= 0 || rotary_dim < 0 || rotary_dim > d || (rotary_dim & 1) || (rotary_dim && !inv_freq) ||
+      page_size <= 0 || num_pages <= 0 || max_blocks <= 0 || num_seqs <= 0 || q_stride < (long long)nq * d)
+    return RLLM_E_BADARG;
+  if (d % 16 || d > 256) return RLLM_E_UNSUPPORTED;
+  const size_t smem = (size_t)rotary_dim * sizeof(float);
+  RLLM_DISPATCH_DTYPE(dtype, T_,
+    rllm_launch_pdl(kv_e4m3_write_kernel<T_>, dim3(T), dim3(256), smem, stream, (const T_*)qkv, (T_*)q_out, q_stride, positions,
+                    token_seq, inv_freq, rotary_dim, block_table, max_blocks, num_seqs, (unsigned char*)kcache,
+                    (unsigned char*)vcache, (unsigned char*)kscale, (unsigned char*)vscale, nq, nkv, d, page_size, num_pages, err));
+  RLLM_LAUNCH_CHECK();
+  return 0;
+}
+
+// ---------------------------------------------------------------------------
+// read: out_k[t], out_v[t] = the rows of (token_seq[t], positions[t])
+// ---------------------------------------------------------------------------
+// A thread reads 16 numbers (16 bytes) of a row and writes them as 16 values.
+template <typename T>
+__global__ void __launch_bounds__(256)
+kv_e4m3_read_kernel(const int* __restrict__ positions, const int* __restrict__ token_seq, const int* __restrict__ block_table,
+                    int max_blocks, int num_seqs, const unsigned char* __restrict__ kcache,
+                    const unsigned char* __restrict__ vcache, const unsigned char* __restrict__ kscale,
+                    const unsigned char* __restrict__ vscale, T* __restrict__ out_k, T* __restrict__ out_v, int T_tokens,
+                    int nkv, int d, int page_size, int num_pages, int* __restrict__ err) {
+  pdl_wait_on(positions, token_seq, block_table, kcache, vcache, kscale, vscale);
+  pdl_launch();
+  const int pieces = nkv * (d >> 4);                   // of a token's keys; as many of its values
+  const long long all = (long long)T_tokens * 2 * pieces;
+  for (long long at = (long long)blockIdx.x * blockDim.x + threadIdx.x; at < all; at += (long long)gridDim.x * blockDim.x) {
+    const int t = (int)(at / (2 * pieces));
+    int c = (int)(at - (long long)t * 2 * pieces);
+    const bool value = c >= pieces;
+    if (value) c -= pieces;
+    const int h = c / (d >> 4), i = (c - h * (d >> 4)) << 4;
+    const int pos = positions[t], seq = token_seq[t];
+    long long r = -1;
+    if (pos >= 0 && pos / page_size < max_blocks && seq >= 0 && seq < num_seqs) {
+      const int page = block_table[(size_t)seq * max_blocks + pos / page_size];
+      if (page >= 0 && page < num_pages) r = ((long long)page * nkv + h) * page_size + pos % page_size;
+    }
+    float x[16];
+    if (r < 0) {
+      if (c == 0) atomicOr(err, 4);
+#pragma unroll
+      for (int k = 0; k < 16; ++k) x[k] = 0.f;
+    } else {
+      const uint4 raw = *(const uint4*)((value ? vcache : kcache) + r * d + i);
+      const float power = kv8_power((value ? vscale : kscale)[r]);
+      kv8_floats(raw.x, x); kv8_floats(raw.y, x + 4); kv8_floats(raw.z, x + 8); kv8_floats(raw.w, x + 12);
+#pragma unroll
+      for (int k = 0; k < 16; ++k) x[k] *= power;
+    }
+    T* dst = (value ? out_v : out_k) + (size_t)t * nkv * d + (size_t)h * d + i;
+    float lo[8], hi[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) { lo[k] = x[k]; hi[k] = x[k + 8]; }
+    if constexpr (sizeof(T) == 4) {
+      *(float4*)dst = make_float4(lo[0], lo[1], lo[2], lo[3]);
+      *(float4*)(dst + 4) = make_float4(lo[4], lo[5], lo[6], lo[7]);
+      *(float4*)(dst + 8) = make_float4(hi[0], hi[1], hi[2], hi[3]);
+      *(float4*)(dst + 12) = make_float4(hi[4], hi[5], hi[6], hi[7]);
+    } else {
+      store8(dst, lo);
+      store8(dst + 8, hi);
+    }
+  }
+}
+
+RLLM_EXPORT int rllm_kv_e4m3_read(const int* positions, const int* token_seq, const int* block_table, int max_blocks,
+                                  int num_seqs, const void* kcache, const void* vcache, const void* kscale,
+                                  const void* vscale, void* out_k, void* out_v, int dtype, int T, int nkv, int d,
+                                  int page_size, int num_pages, int* err, cudaStream_t stream) {
+  if (T <= 0) return 0;
+  if (!positions || !token_seq || !block_table || !kcache || !vcache || !kscale || !vscale || !out_k || !out_v || !err ||
+      nkv <= 0 || d <= 0 || page_size <= 0 || num_pages <= 0 || max_blocks <= 0 || num_seqs <= 0)
+    return RLLM_E_BADARG;
+  if (d % 16 || d > 256) return RLLM_E_UNSUPPORTED;
+  if (((uintptr_t)kcache | (uintptr_t)vcache | (uintptr_t)out_k | (uintptr_t)out_v) & 15) return RLLM_E_UNSUPPORTED;
+  const long long threads = (long long)T * 2 * nkv * (d >> 4), blocks = (threads + 255) / 256;
+  const unsigned grid = (unsigned)(blocks < (1 << 20) ? blocks : (1 << 20));
+  RLLM_DISPATCH_DTYPE(dtype, T_,
+    rllm_launch_pdl(kv_e4m3_read_kernel<T_>, dim3(grid), dim3(256), (size_t)0, stream, positions, token_seq, block_table,
+                    max_blocks, num_seqs, (const unsigned char*)kcache, (const unsigned char*)vcache,
+                    (const unsigned char*)kscale, (const unsigned char*)vscale, (T_*)out_k, (T_*)out_v, T, nkv, d, page_size,
+                    num_pages, err));
+  RLLM_LAUNCH_CHECK();
+  return 0;
+}

@@ -60,6 +60,9 @@ def _check(code: int, what: str) -> None:
 # The entry points by name: the library that holds each, its arguments (see native/csrc/launch.cc: p tensor or None, i int,
 # l long long, f float; the stream, which comes last everywhere, is added) and what a refusal calls it.
 _TABLE = {
+    "rllm_kv_e4m3_write": ("kv_e4m3", "piplpppipiippppiiiiiip", "rope_kv_write_e4m3"),
+    "rllm_kv_e4m3_read": ("kv_e4m3", "pppiippppppiiiiiip", "kv_read_e4m3"),
+    "rllm_attention_e4m3_simt": ("attention_e4m3", "pipppppipippiiiiiiiiifp", "attention_e4m3"),
     "rllm_softcap": ("elementwise", "plf", "softcap_rows"),
     "rllm_shared_key_attention_mma": ("shared_key_attention", "pppppippiiiiiiiiiiifiipp", "shared_key_attention_mma"),
     "rllm_shared_key_attention_tcgen05": ("shared_key_attention", "pippppippiiiiiiiiiiiifp", "shared_key_attention_tcgen05"),
@@ -2046,3 +2049,124 @@ def softcap_rows(x: torch.Tensor, cap: float) -> torch.Tensor:
     _contig(x, "x")
     _entries.rllm_softcap(x, x.numel(), cap)
     return x
+
+
+# ---------------------------------------------------------------------------
+# a cache kept in 8 bits: pages of float8_e4m3fn [pages, nkv, page_size, d] and a power of two a row, float8_e8m0fnu
+# [pages, nkv, page_size], for keys and for values (csrc/kv_e4m3.cuh says what a row becomes)
+# ---------------------------------------------------------------------------
+E4M3, E8M0 = torch.float8_e4m3fn, torch.float8_e8m0fnu
+
+
+def _e4m3_cache(kcache: torch.Tensor, vcache: torch.Tensor, kscale: torch.Tensor, vscale: torch.Tensor,
+                block_table: torch.Tensor, nkv: int, d: int) -> None:
+    """What every operator over such a cache asks of it."""
+    if kcache.dtype is not E4M3 or vcache.dtype is not E4M3 or kscale.dtype is not E8M0 or vscale.dtype is not E8M0:
+        raise KernelError("an 8-bit cache has float8_e4m3fn pages and float8_e8m0fnu scales")
+    if kcache.dim() != 4 or kcache.shape != vcache.shape or kcache.shape[1] != nkv or kcache.shape[3] != d or \
+            kscale.shape != kcache.shape[:3] or vscale.shape != kcache.shape[:3]:
+        raise KernelError("an 8-bit cache: pages [pages, nkv, page_size, d] and scales [pages, nkv, page_size], keys' and values' alike")
+    if block_table.dim() != 2 or block_table.dtype is not torch.int32:
+        raise KernelError("block_table must be int32 [sequences, blocks]")
+    for t, name in ((kcache, "kcache"), (vcache, "vcache"), (kscale, "kscale"), (vscale, "vscale"), (block_table, "block_table")):
+        _contig(t, name)
+
+
+def _on_current_device(*tensors: torch.Tensor) -> None:
+    """Launches go to the current device's stream: tensors of another one are refused."""
+    for t in tensors:
+        if not t.is_cuda:
+            raise KernelError("the engine's kernels run on CUDA tensors only; there is no CPU path")
+    here = torch._C._cuda_getDevice()
+    for t in tensors:
+        if t.get_device() != here:
+            raise KernelError(f"a tensor on {t.device} while cuda:{here} is the current device")
+
+
+def _ints(t: torch.Tensor, name: str, n: Optional[int] = None) -> None:
+    if t.dtype is not torch.int32 or t.dim() != 1 or not t.is_contiguous() or (n is not None and t.numel() != n):
+        raise KernelError(f"{name} must be a contiguous int32 vector" + ("" if n is None else f" of {n}"))
+
+
+def rope_kv_write_e4m3(qkv: torch.Tensor, positions: torch.Tensor, token_seq: torch.Tensor,
+                       inv_freq: Optional[torch.Tensor], rotary_dim: int, block_table: torch.Tensor, kcache: torch.Tensor,
+                       vcache: torch.Tensor, kscale: torch.Tensor, vscale: torch.Tensor, nq: int, nkv: int, d: int,
+                       err: torch.Tensor, q_out: Optional[torch.Tensor] = None) -> None:
+    """``rope_kv_write`` into a cache kept in 8 bits: rotates q (into ``q_out`` [T, nq d], whose rows may lie apart, or in
+    place) and k, quantises every token's rotated k and its v, a row of d numbers each, and stores them into the token's page.
+
+    The rotation and the row's scale are float32; a number is rounded once, to e4m3.  A (sequence, position) pair may stand
+    in the step once.  A token whose page is not held sets bit 2 of ``err`` and is not written (its q is rotated)."""
+    T = qkv.shape[0]
+    dt = dtype_code(qkv.dtype)
+    if qkv.dim() != 2 or qkv.shape[1] != (nq + 2 * nkv) * d:
+        raise KernelError("rope_kv_write_e4m3: qkv must be [T, (nq + 2 nkv) d]")
+    _contig(qkv, "qkv")
+    _e4m3_cache(kcache, vcache, kscale, vscale, block_table, nkv, d)
+    _ints(positions, "positions", T); _ints(token_seq, "token_seq", T)
+    if rotary_dim and (inv_freq is None or inv_freq.dtype is not torch.float64 or inv_freq.numel() != rotary_dim // 2):
+        raise KernelError("rope_kv_write_e4m3: inv_freq must be float64 [rotary_dim / 2]")
+    if q_out is None:
+        q_out = qkv
+    elif q_out.dtype is not qkv.dtype or q_out.shape != (T, nq * d) or q_out.stride(1) != 1:
+        raise KernelError("rope_kv_write_e4m3: q_out must be [T, nq d] of qkv's type")
+    _on_current_device(qkv, kcache, block_table, q_out)
+    _entries.rllm_kv_e4m3_write(qkv, dt, q_out, q_out.stride(0), positions, token_seq, inv_freq if rotary_dim else None,
+                                rotary_dim, block_table, block_table.shape[1], block_table.shape[0], kcache, vcache, kscale,
+                                vscale, T, nq, nkv, d, kcache.shape[2], kcache.shape[0], err)
+
+
+def kv_read_e4m3(positions: torch.Tensor, token_seq: torch.Tensor, block_table: torch.Tensor, kcache: torch.Tensor,
+                 vcache: torch.Tensor, kscale: torch.Tensor, vscale: torch.Tensor, out_k: torch.Tensor, out_v: torch.Tensor,
+                 err: torch.Tensor) -> None:
+    """Keys and values of given tokens out of a cache kept in 8 bits: out_k, out_v [T, nkv d] (bfloat16 or float32) = the
+    rows of sequence ``token_seq[t]``'s token at ``positions[t]``.  Exact in float32, and in bfloat16 down to its smallest
+    numbers; NaN where a row's scale is.  A token whose page is not held sets bit 4 of ``err`` and reads as zeros."""
+    T = positions.numel()
+    if kcache.dim() != 4:
+        raise KernelError("kv_read_e4m3: kcache must be [pages, nkv, page_size, d]")
+    nkv, d = kcache.shape[1], kcache.shape[3]
+    _e4m3_cache(kcache, vcache, kscale, vscale, block_table, nkv, d)
+    _ints(positions, "positions"); _ints(token_seq, "token_seq", T)
+    for t, name in ((out_k, "out_k"), (out_v, "out_v")):
+        if t.shape != (T, nkv * d) or t.dtype is not out_k.dtype:
+            raise KernelError("kv_read_e4m3: out_k and out_v must be [T, nkv d] of one type")
+        _contig(t, name)
+    dt = dtype_code(out_k.dtype)
+    _on_current_device(kcache, block_table, out_k)
+    _entries.rllm_kv_e4m3_read(positions, token_seq, block_table, block_table.shape[1], block_table.shape[0], kcache, vcache,
+                               kscale, vscale, out_k, out_v, dt, T, nkv, d, kcache.shape[2],
+                               kcache.shape[0], err)
+
+
+def attention_e4m3(q: torch.Tensor, out: torch.Tensor, kcache: torch.Tensor, vcache: torch.Tensor, kscale: torch.Tensor,
+                   vscale: torch.Tensor, block_table: torch.Tensor, q_start: torch.Tensor, seq_lens: torch.Tensor,
+                   num_decode: int, max_q_len: int, max_seq_len: int, nq: int, nkv: int, window: int, scale: float,
+                   err: torch.Tensor) -> None:
+    """Causal attention of a step's tokens over a cache kept in 8 bits, their own keys and values (written before) among it.
+
+    q [T, >= nq d], rotated; a row's first nq d numbers are read (rows may lie apart).  Row i of ``out`` [T, nq d] gets token
+    i's result.  Sequence s owns the tokens q_start[s] .. q_start[s + 1] - 1, the last ones of its seq_lens[s] in the cache;
+    the first ``num_decode`` sequences bring one token each.  ``max_q_len`` and ``max_seq_len`` bound every sequence's tokens
+    in this step and in the cache.  Rows behind the last sequence's stay as they are.  A page that is not held sets bit 4 of
+    ``err``, and its keys are left out."""
+    dt = dtype_code(q.dtype)
+    S = seq_lens.numel()
+    if q.dim() != 2 or q.stride(1) != 1 or out.dim() != 2 or out.dtype is not q.dtype or out.shape[1] != nq * (kcache.shape[-1]) or \
+            q.shape[1] < out.shape[1] or q.shape[0] < out.shape[0]:
+        raise KernelError("attention_e4m3: q must be [T, >= nq d] and out [T, nq d] of one type")
+    d = kcache.shape[-1]
+    _contig(out, "out")
+    _e4m3_cache(kcache, vcache, kscale, vscale, block_table, nkv, d)
+    _ints(q_start, "q_start", S + 1); _ints(seq_lens, "seq_lens")
+    if not 0 <= num_decode <= S or block_table.shape[0] < S or max_q_len < 0 or max_seq_len < 0:
+        raise KernelError("attention_e4m3: bad counts of sequences or bounds of lengths")
+    if max_seq_len > block_table.shape[1] * kcache.shape[2]:
+        raise KernelError("attention_e4m3: max_seq_len passes what block_table's rows can hold")
+    _on_current_device(q, kcache, block_table, out)
+    T = out.shape[0]
+    if T == 0 or S == 0:
+        return
+    cache = (kcache, vcache, kscale, vscale, dt, block_table, block_table.shape[1], q_start, seq_lens)
+    heads = (nq, nkv, d, kcache.shape[2], kcache.shape[0], window, scale, err)
+    _entries.rllm_attention_e4m3_simt(q, q.stride(0), out, *cache, 0, S, T, *heads)
