@@ -12,6 +12,7 @@
 //                 (token, head of the group) pair) a cluster of CTAs; see below.
 //   simt kernel   CUDA cores, one warp a (token, head): head sizes and pages that the rows kernel does not take.
 #include "kv_e4m3.cuh"
+#include <cooperative_groups.h>
 #include <math.h>
 
 // The sequence of the launch's token i (flat token number): the s in [seq_begin, seq_end) with q_start[s] <= i < q_start[s + 1]
@@ -121,6 +122,456 @@ static int e4_check(const void* q, const void* out, const void* kcache, const vo
     return RLLM_E_BADARG;
   if (d % 16 || d > 256 || (((uintptr_t)kcache | (uintptr_t)vcache) & 15)) return RLLM_E_UNSUPPORTED;
   return 0;
+}
+
+// ---------------------------------------------------------------------------
+// tensor cores, few rows a sequence and kv head
+// ---------------------------------------------------------------------------
+// Keys are the rows of the first product and head dims those of the second, so that query rows are the columns (8 a tile):
+//   S^T [16 keys x 8 rows] = K [16 x d] Q^T,   O^T [d x 8 rows] += V^T [d x 16 keys] P^T
+// (queries as rows would come in sixteens: twice the products, accumulators and exponentials for a group of 8 or fewer).
+// Operands of 8 bits become halves in registers, exactly, by one instruction a pair, and come from global memory straight
+// into the lanes that need them: the order of head dims in the first product and in the second one's rows is free, so a lane
+// takes contiguous bytes.
+//   K: lane (gid, tig) needs keys gid and gid + 8, four dims a step of 16: bytes 64 c + 16 tig .. + 15 of the row, c = 0 ..
+//      d / 64 - 1, are its dims of four steps; the queries are laid out by the same rule.
+//   V: it needs keys 2 tig, 2 tig + 1 and those plus 8, and d / 8 dims: bytes gid d / 8 .. of four rows; the bytes of two
+//      keys are interleaved (prmt) into pairs along the keys.
+//   P^T: the accumulators of S^T hold (key gid, rows 2 tig, 2 tig + 1); movmatrix turns them into (keys 2 tig, 2 tig + 1, row gid).
+// Factors: a key's power of two and its row's factor multiply the score; a value's power multiplies the weight, relative to
+// 2^E, E a running reference of the warp as the maximum is of a row: both move only when passed by 2^4, so that a tile costs
+// one vote, and P 2^(ev - E) 2^7 stays at or below 2^15, within a half (the 2^7 puts the halves' smallest step, 2^-24, at
+// 2^-31 of a weight of 1).  The denominator sums the weights themselves.
+// Queries are put into halves after a division by a power of two of the row's own (bfloat16: exact down to 2^-27 of the
+// row's largest; float32: two halves, 22 bits, and P likewise, with which the path is as good as float32 products).
+// What bounds it is memory: 16 keys of 128 dims are 4 KB a warp and 170 instructions, and warps load a tile ahead.
+//
+// A cluster of C CTAs of 4 warps shares one (sequence, kv head, tile of rows): key tiles go round over the warps of the
+// cluster, partial results are merged in shared memory, first the CTA's, then, each CTA a slice, the cluster's (distributed
+// shared memory): no workspace, no counters, and a captured graph needs nothing of its own.
+#define E4_WARPS 4
+#define E4_SLACK 4                   // log2 of how far a score may pass the row's reference, and a value's power the warp's
+#define E4_SHIFT 7                   // log2 of the weights' factor: 2 E4_SLACK + E4_SHIFT = 15
+__device__ __forceinline__ void e4_mma(float* c, const unsigned* a, unsigned b0, unsigned b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ unsigned e4_turn(unsigned x) {        // an 8 x 8 matrix of halves across the warp, transposed
+  unsigned y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+__device__ __forceinline__ float e4_ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));           // ex2(-inf) = +0
+  return y;
+}
+__device__ __forceinline__ unsigned e4_pack(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *(const unsigned*)&h;
+}
+__device__ __forceinline__ float2 e4_unpack(unsigned h) { return __half22float2(*(const __half2*)&h); }
+
+// a lane's part of a tile of 16 keys
+template <int D> struct E4Tile {
+  uint4 k[2][D / 64];
+  unsigned v[4][D / 32];
+  int kb[2], vb[2];                  // scale bytes of keys gid and gid + 8
+  bool held;
+};
+
+template <int D, int NB, int PF, typename T>
+__global__ void __launch_bounds__(32 * E4_WARPS)
+attention_e4m3_rows_kernel(const T* q, int q_stride, T* __restrict__ out, const unsigned char* __restrict__ kcache,
+                           const unsigned char* __restrict__ vcache, const unsigned char* __restrict__ kscale,
+                           const unsigned char* __restrict__ vscale, const int* __restrict__ block_table, int max_blocks,
+                           const int* __restrict__ q_start, const int* __restrict__ seq_lens, int seq_begin, int nq, int nkv,
+                           int page_size, int num_pages, int window, float scale_log2, int* __restrict__ err) {
+  constexpr int R = 8 * NB, TERMS = sizeof(T) == 4 ? 2 : 1, KC = D / 64, VW = D / 32;
+  extern __shared__ __align__(16) float e4_smem[];
+  pdl_wait_on(q, kcache, vcache, kscale, vscale);
+  pdl_launch();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, gid = lane >> 2, tig = lane & 3;
+  const int C = gridDim.x, rank = blockIdx.x;      // the cluster is the grid's x
+  const int kvh = blockIdx.y % nkv, s = seq_begin + blockIdx.z;
+  const int g = nq / nkv;
+  const int qs = q_start[s], qlen = q_start[s + 1] - qs, len = seq_lens[s];
+  const int rows = qlen * g, r0 = blockIdx.y / nkv * R;
+  if (r0 >= rows) return;                          // the whole cluster
+  const int pos0 = len - qlen;
+  const int t_first = r0 / g, t_last = (min(r0 + R, rows) - 1) / g;
+  const int hi_first = pos0 + t_first + 1, kend = min(pos0 + t_last + 1, max_blocks * page_size);
+  const int kmin = window > 0 ? max(0, hi_first - window) : 0;
+  const int lo_last = window > 0 ? max(0, pos0 + t_last + 1 - window) : 0;
+  const int t_hi = (kend + 15) >> 4, stride = C * E4_WARPS;
+  const int* bt = block_table + (size_t)s * max_blocks;
+
+  // the tile's queries, as float32 rows of D + 4
+  float* sQ = e4_smem;
+  for (int i = threadIdx.x; i < R * D; i += 32 * E4_WARPS) {
+    const int r = i / D, c = i - r * D, row = r0 + r;
+    float x = 0.f;
+    if (row < rows) x = to_f32(q[(size_t)(qs + row / g) * q_stride + (size_t)(kvh * g + row % g) * D + c]);
+    sQ[r * (D + 4) + c] = x;
+  }
+  __syncthreads();
+  unsigned qf[NB][D / 16][2 * TERMS];
+  float rfc[NB][2];
+  int hi[NB][2];
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb) {
+    const float* qr = sQ + (nb * 8 + gid) * (D + 4) + tig * 16;
+    float top = 0.f;
+#pragma unroll
+    for (int c = 0; c < KC; ++c)
+#pragma unroll
+      for (int i = 0; i < 16; i += 4) {
+        const float4 x = *(const float4*)(qr + c * 64 + i);
+        top = fmaxf(fmaxf(top, fmaxf(fabsf(x.x), fabsf(x.y))), fmaxf(fabsf(x.z), fabsf(x.w)));
+      }
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    const int e = min(max((int)(__float_as_uint(top) >> 23) - 127, -100), 127);     // top < 2^(e + 1)
+    const float down = __uint_as_float((unsigned)(127 + 13 - e) << 23), up = __uint_as_float((unsigned)max(127 - 13 + e, 1) << 23) * scale_log2;
+#pragma unroll
+    for (int kk = 0; kk < D / 16; ++kk) {
+      const float4 x = *(const float4*)(qr + (kk >> 2) * 64 + (kk & 3) * 4);
+      const float y[4] = {x.x * down, x.y * down, x.z * down, x.w * down};
+      qf[nb][kk][0] = e4_pack(y[0], y[1]);
+      qf[nb][kk][1] = e4_pack(y[2], y[3]);
+      if (TERMS == 2) {
+        const float2 a = e4_unpack(qf[nb][kk][0]), b = e4_unpack(qf[nb][kk][1]);
+        qf[nb][kk][2 * TERMS - 2] = e4_pack(y[0] - a.x, y[1] - a.y);
+        qf[nb][kk][2 * TERMS - 1] = e4_pack(y[2] - b.x, y[3] - b.y);
+      }
+    }
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      rfc[nb][c] = __shfl_sync(0xffffffffu, up, (2 * tig + c) * 4);
+      hi[nb][c] = pos0 + min(r0 + nb * 8 + 2 * tig + c, rows - 1) / g + 1;
+    }
+  }
+
+  float o[NB][D / 16][4], m[NB][2], l[NB][2];
+  int E = -1000;
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb) {
+    m[nb][0] = m[nb][1] = -INFINITY;
+    l[nb][0] = l[nb][1] = 0.f;
+#pragma unroll
+    for (int j = 0; j < D / 16; ++j) o[nb][j][0] = o[nb][j][1] = o[nb][j][2] = o[nb][j][3] = 0.f;
+  }
+
+  auto load = [&](E4Tile<D>& x, int t) {
+    x.held = false;
+    if (t >= t_hi) return;
+    const int j0 = t << 4, pi = j0 / page_size;
+    const int page = bt[pi];
+    x.held = page >= 0 && page < num_pages;
+    if (!x.held && lane == 0) atomicOr(err, 4);
+    const long long row = x.held ? ((long long)page * nkv + kvh) * page_size + (j0 - pi * page_size) : 0;
+    const unsigned char *kp = kcache + row * D, *vp = vcache + row * D;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int r = gid + 8 * i;
+      const bool ok = x.held && j0 + r >= kmin && j0 + r < kend;
+#pragma unroll
+      for (int c = 0; c < KC; ++c) x.k[i][c] = ok ? *(const uint4*)(kp + r * D + c * 64 + tig * 16) : make_uint4(0u, 0u, 0u, 0u);
+      x.kb[i] = ok ? kscale[row + r] : 0;
+      x.vb[i] = ok ? vscale[row + r] : 0;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = 2 * tig + (i & 1) + 8 * (i >> 1);
+      const bool ok = x.held && j0 + r >= kmin && j0 + r < kend;
+      const unsigned char* p = vp + r * D + gid * (D / 8);
+      if constexpr (D == 64) {
+        const uint2 y = ok ? *(const uint2*)p : make_uint2(0u, 0u);
+        x.v[i][0] = y.x; x.v[i][1] = y.y;
+      } else {
+#pragma unroll
+        for (int c = 0; c < VW; c += 4) {
+          const uint4 y = ok ? *(const uint4*)(p + c * 4) : make_uint4(0u, 0u, 0u, 0u);
+          x.v[i][c] = y.x; x.v[i][c + 1] = y.y; x.v[i][c + 2] = y.z; x.v[i][c + 3] = y.w;
+        }
+      }
+    }
+  };
+
+  auto compute = [&](const E4Tile<D>& x, int t) {
+    const int j0 = t << 4;
+    float sc[NB][4];
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) sc[nb][0] = sc[nb][1] = sc[nb][2] = sc[nb][3] = 0.f;
+#pragma unroll
+    for (int kk = 0; kk < D / 16; ++kk) {
+      const uint4 ka = x.k[0][kk >> 2], kb = x.k[1][kk >> 2];
+      const unsigned wa = (kk & 3) == 0 ? ka.x : (kk & 3) == 1 ? ka.y : (kk & 3) == 2 ? ka.z : ka.w;
+      const unsigned wb = (kk & 3) == 0 ? kb.x : (kk & 3) == 1 ? kb.y : (kk & 3) == 2 ? kb.z : kb.w;
+      const unsigned a[4] = {kv8_halves_lo(wa), kv8_halves_lo(wb), kv8_halves_hi(wa), kv8_halves_hi(wb)};
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+        e4_mma(sc[nb], a, qf[nb][kk][0], qf[nb][kk][1]);
+        if (TERMS == 2) e4_mma(sc[nb], a, qf[nb][kk][2 * TERMS - 2], qf[nb][kk][2 * TERMS - 1]);
+      }
+    }
+    const bool clear = x.held && j0 >= lo_last && j0 >= kmin && j0 + 16 <= hi_first && j0 + 16 <= kend;
+    const float kf[2] = {kv8_power(x.kb[0]), kv8_power(x.kb[1])};
+    unsigned seen = 0xffffffffu;                       // bit nb * 4 + e
+    if (!clear) {
+      seen = 0u;
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int j = j0 + gid + 8 * (e >> 1), h = min(hi[nb][e & 1], kend);
+          if (x.held && j < h && (window == 0 || j >= hi[nb][e & 1] - window)) seen |= 1u << (nb * 4 + e);
+        }
+    }
+    const int v0 = x.vb[0] == KV8_NAN_SCALE ? 0 : x.vb[0], v1 = x.vb[1] == KV8_NAN_SCALE ? 0 : x.vb[1];
+    bool need = max(v0, v1) > E + E4_SLACK;
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float v = sc[nb][e] * rfc[nb][e & 1] * kf[e >> 1];
+        if (!(seen >> (nb * 4 + e) & 1u)) v = -INFINITY;
+        sc[nb][e] = v;
+        need = need || v > m[nb][e & 1] + (float)E4_SLACK;
+      }
+    if (__any_sync(0xffffffffu, need)) {
+      const int vmax = __reduce_max_sync(0xffffffffu, max(v0, v1));
+      float fe = 1.0f;
+      if (vmax > E + E4_SLACK) {
+        fe = E - vmax < -126 ? 0.f : __uint_as_float((unsigned)(127 + E - vmax) << 23);
+        E = vmax;
+      }
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+        float corr[2];
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          float mx = fmaxf(sc[nb][c], sc[nb][c + 2]);
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+          const bool moves = mx > m[nb][c] + (float)E4_SLACK;
+          corr[c] = moves ? e4_ex2(m[nb][c] - mx) : 1.0f;
+          if (moves) m[nb][c] = mx;
+          l[nb][c] *= corr[c];
+          corr[c] *= fe;
+        }
+#pragma unroll
+        for (int j = 0; j < D / 16; ++j) { o[nb][j][0] *= corr[0]; o[nb][j][1] *= corr[1]; o[nb][j][2] *= corr[0]; o[nb][j][3] *= corr[1]; }
+      }
+    }
+    // 2^(ev - E + E4_SHIFT) of the lane's two keys
+    float vf[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      vf[i] = x.vb[i] == KV8_NAN_SCALE ? __uint_as_float(0x7FC00000u)
+                                       : (x.vb[i] - E + E4_SHIFT < -126 ? 0.f : __uint_as_float((unsigned)(127 + E4_SHIFT + x.vb[i] - E) << 23));
+    unsigned pb[NB][2 * TERMS];
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+      float w[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float mm = m[nb][e & 1] == -INFINITY ? 0.f : m[nb][e & 1];
+        const float p = e4_ex2(sc[nb][e] - mm);
+        l[nb][e & 1] += p;
+        w[e] = (seen >> (nb * 4 + e) & 1u) ? p * vf[e >> 1] : 0.f;
+      }
+      const unsigned h0 = e4_pack(w[0], w[1]), h1 = e4_pack(w[2], w[3]);
+      pb[nb][0] = e4_turn(h0);
+      pb[nb][1] = e4_turn(h1);
+      if (TERMS == 2) {
+        const float2 a = e4_unpack(h0), b = e4_unpack(h1);
+        pb[nb][2 * TERMS - 2] = e4_turn(e4_pack(w[0] - a.x, w[1] - a.y));
+        pb[nb][2 * TERMS - 1] = e4_turn(e4_pack(w[2] - b.x, w[3] - b.y));
+      }
+    }
+#pragma unroll
+    for (int c = 0; c < VW; ++c) {
+      // bytes 4 c .. 4 c + 3 of keys 2 tig and 2 tig + 1, and of the two 8 keys on, as pairs along the keys
+      const unsigned a01 = __byte_perm(x.v[0][c], x.v[1][c], 0x5140), a23 = __byte_perm(x.v[0][c], x.v[1][c], 0x7362);
+      const unsigned b01 = __byte_perm(x.v[2][c], x.v[3][c], 0x5140), b23 = __byte_perm(x.v[2][c], x.v[3][c], 0x7362);
+      const unsigned a[2][4] = {{kv8_halves_lo(a01), kv8_halves_hi(a01), kv8_halves_lo(b01), kv8_halves_hi(b01)},
+                                {kv8_halves_lo(a23), kv8_halves_hi(a23), kv8_halves_lo(b23), kv8_halves_hi(b23)}};
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+          e4_mma(o[nb][2 * c + i], a[i], pb[nb][0], pb[nb][1]);
+          if (TERMS == 2) e4_mma(o[nb][2 * c + i], a[i], pb[nb][2 * TERMS - 2], pb[nb][2 * TERMS - 1]);
+        }
+    }
+  };
+
+  {
+    E4Tile<D> buf[PF];
+    int t = (kmin >> 4) + rank * E4_WARPS + warp;
+#pragma unroll
+    for (int i = 0; i < PF; ++i) load(buf[i], t + i * stride);
+    for (; t < t_hi; t += PF * stride) {
+#pragma unroll
+      for (int i = 0; i < PF; ++i) {
+        if (t + i * stride < t_hi) {
+          compute(buf[i], t + i * stride);
+          load(buf[i], t + (i + PF) * stride);
+        }
+      }
+    }
+  }
+
+  // the CTA's result: parts [warps][R][D], and every warp's maximum and sum of each row
+  float* part = e4_smem;
+  float* sM = part + E4_WARPS * R * D;               // [warps][R]
+  float* sL = sM + E4_WARPS * R;
+  float* cM = sL + E4_WARPS * R;                     // [R] the CTA's
+  float* cL = cM + R;
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+#pragma unroll
+      for (int x = 4; x < 32; x <<= 1) l[nb][c] += __shfl_xor_sync(0xffffffffu, l[nb][c], x);
+  __syncthreads();                                   // the queries have been read
+  if (gid == 0) {
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        sM[warp * R + nb * 8 + 2 * tig + c] = m[nb][c];
+        sL[warp * R + nb * 8 + 2 * tig + c] = l[nb][c];
+      }
+  }
+  __syncthreads();
+  const float fe = E < 0 ? 0.f : kv8_power(E) * (1.0f / (1 << E4_SHIFT));
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const int r = nb * 8 + 2 * tig + c;
+      float top = sM[r];
+#pragma unroll
+      for (int w = 1; w < E4_WARPS; ++w) top = fmaxf(top, sM[w * R + r]);
+      const float f = m[nb][c] == -INFINITY ? (l[nb][c] == 0.f ? 0.f : l[nb][c]) : e4_ex2(m[nb][c] - top) * fe;
+      float* dst = part + ((size_t)warp * R + r) * D + gid * (D / 8);
+#pragma unroll
+      for (int j = 0; j < D / 16; ++j) *(float2*)(dst + 2 * j) = make_float2(o[nb][j][c] * f, o[nb][j][c + 2] * f);
+    }
+  if (threadIdx.x < R) {
+    const int r = threadIdx.x;
+    float top = sM[r], sum = 0.f;
+#pragma unroll
+    for (int w = 1; w < E4_WARPS; ++w) top = fmaxf(top, sM[w * R + r]);
+#pragma unroll
+    for (int w = 0; w < E4_WARPS; ++w) sum += sL[w * R + r] * (sM[w * R + r] == -INFINITY ? 1.0f : e4_ex2(sM[w * R + r] - top));
+    cM[r] = top;
+    cL[r] = sum;
+  }
+  __syncthreads();
+  auto store = [&](int i, float x, float sum) {
+    const int r = i / D, row = r0 + r;
+    if (row < rows) {
+      const float inv = sum == 0.f ? 0.f : 1.0f / sum;   // NaN stays NaN
+      out[((size_t)(qs + row / g) * nq + kvh * g + row % g) * D + (i - r * D)] = from_f32<T>(x * inv);
+    }
+  };
+  for (int i = threadIdx.x; i < R * D; i += 32 * E4_WARPS) {
+    float x = part[i];
+#pragma unroll
+    for (int w = 1; w < E4_WARPS; ++w) x += part[w * R * D + i];
+    if (C == 1) store(i, x, cL[i / D]);
+    else part[i] = x;
+  }
+  if (C == 1) return;
+  namespace cg = cooperative_groups;
+  cg::cluster_group cluster = cg::this_cluster();
+  cluster.sync();
+  for (int i = rank * 32 * E4_WARPS + threadIdx.x; i < R * D; i += C * 32 * E4_WARPS) {
+    const int r = i / D;
+    float top = -INFINITY, x = 0.f, sum = 0.f;
+    for (int c = 0; c < C; ++c) top = fmaxf(top, cluster.map_shared_rank(cM, c)[r]);
+    for (int c = 0; c < C; ++c) {
+      const float mc = cluster.map_shared_rank(cM, c)[r];
+      const float f = mc == -INFINITY ? 1.0f : e4_ex2(mc - top);
+      x += cluster.map_shared_rank(part, c)[i] * f;
+      sum += cluster.map_shared_rank(cL, c)[r] * f;
+    }
+    store(i, x, sum);
+  }
+  cluster.sync();                                    // nobody leaves while its shared memory is being read
+}
+
+template <int D, int NB, int PF, typename T>
+static int e4_rows_launch(const void* q, int q_stride, void* out, const void* kcache, const void* vcache, const void* kscale,
+                          const void* vscale, const int* block_table, int max_blocks, const int* q_start, const int* seq_lens,
+                          int seq_begin, int num_seqs, int max_q_len, int max_keys, int nq, int nkv, int page_size,
+                          int num_pages, int window, float scale, int* err, cudaStream_t stream) {
+  constexpr int R = 8 * NB;
+  auto* kernel = attention_e4m3_rows_kernel<D, NB, PF, T>;
+  const size_t stage = sizeof(float) * R * (D + 4), merge = sizeof(float) * (E4_WARPS * R * (D + 2) + 2 * R);
+  const size_t smem = stage > merge ? stage : merge;
+  static SmemLimit limit;
+  if (const int e = limit.allow(kernel, (int)smem)) return e;
+  const long long tiles = ((long long)max_q_len * (nq / nkv) + R - 1) / R, units = tiles * nkv * num_seqs;
+  if (tiles * nkv > 65535 || num_seqs > 65535) return RLLM_E_UNSUPPORTED;
+  // CTAs a unit: enough for the GPU, but two tiles of keys a warp at least
+  int C = 1;
+  while (C < 8 && units * C * 2 <= 592 && C * 2 * E4_WARPS * 32 <= max_keys) C *= 2;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)C, (unsigned)(tiles * nkv), (unsigned)num_seqs);
+  cfg.blockDim = dim3(32 * E4_WARPS);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)C;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = rllm_pdl_enabled() ? 2 : 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, (const T*)q, q_stride, (T*)out, (const unsigned char*)kcache,
+                                           (const unsigned char*)vcache, (const unsigned char*)kscale, (const unsigned char*)vscale,
+                                           block_table, max_blocks, q_start, seq_lens, seq_begin, nq, nkv, page_size, num_pages,
+                                           window, scale * 1.4426950408889634f, err);
+  if (e != cudaSuccess) { cudaGetLastError(); return (int)e; }
+  RLLM_LAUNCH_CHECK();
+  return 0;
+}
+
+// Sequences seq_begin .. seq_end - 1, of at most max_q_len tokens each; no query sees more than max_keys keys.  Heads of 64,
+// 128 or 256, pages of a multiple of 16 keys.
+RLLM_EXPORT int rllm_attention_e4m3_rows(const void* q, int q_stride, void* out, const void* kcache, const void* vcache,
+                                         const void* kscale, const void* vscale, int dtype, const int* block_table,
+                                         int max_blocks, const int* q_start, const int* seq_lens, int seq_begin, int seq_end,
+                                         int max_q_len, int max_keys, int nq, int nkv, int d, int page_size, int num_pages,
+                                         int window, float scale, int* err, cudaStream_t stream) {
+  if (max_q_len <= 0 || seq_end <= seq_begin) return 0;
+  if (const int rc = e4_check(q, out, kcache, vcache, kscale, vscale, block_table, max_blocks, q_start, seq_lens, seq_begin,
+                              seq_end, nq, nkv, d, page_size, num_pages, window, scale, err)) return rc;
+  if (page_size % 16 || !(d == 64 || d == 128 || d == 256)) return RLLM_E_UNSUPPORTED;
+#define E4_ROWS(DD, NBB, PFF, TT)                                                                                              \
+  return e4_rows_launch<DD, NBB, PFF, TT>(q, q_stride, out, kcache, vcache, kscale, vscale, block_table, max_blocks, q_start, \
+                                          seq_lens, seq_begin, seq_end - seq_begin, max_q_len, max_keys, nq, nkv, page_size,  \
+                                          num_pages, window, scale, err, stream)
+  const bool one = (long long)max_q_len * (nq / nkv) <= 8;
+  if (dtype == RLLM_DT_BF16) {
+    if (d == 64) { if (one) E4_ROWS(64, 1, 2, bf16); E4_ROWS(64, 2, 2, bf16); }
+    if (d == 128) { if (one) E4_ROWS(128, 1, 2, bf16); E4_ROWS(128, 2, 1, bf16); }
+    E4_ROWS(256, 1, 1, bf16);
+  }
+  if (dtype == RLLM_DT_F32) {
+    if (d == 64) { if (one) E4_ROWS(64, 1, 2, float); E4_ROWS(64, 2, 1, float); }
+    if (d == 128) { if (one) E4_ROWS(128, 1, 1, float); E4_ROWS(128, 2, 1, float); }
+    E4_ROWS(256, 1, 1, float);
+  }
+  return RLLM_E_BADARG;
 }
 
 RLLM_EXPORT int rllm_attention_e4m3_simt(const void* q, int q_stride, void* out, const void* kcache, const void* vcache,

@@ -62,6 +62,7 @@ def _check(code: int, what: str) -> None:
 _TABLE = {
     "rllm_kv_e4m3_write": ("kv_e4m3", "piplpppipiippppiiiiiip", "rope_kv_write_e4m3"),
     "rllm_kv_e4m3_read": ("kv_e4m3", "pppiippppppiiiiiip", "kv_read_e4m3"),
+    "rllm_attention_e4m3_rows": ("attention_e4m3", "pipppppipippiiiiiiiiiifp", "attention_e4m3"),
     "rllm_attention_e4m3_simt": ("attention_e4m3", "pipppppipippiiiiiiiiifp", "attention_e4m3"),
     "rllm_softcap": ("elementwise", "plf", "softcap_rows"),
     "rllm_shared_key_attention_mma": ("shared_key_attention", "pppppippiiiiiiiiiiifiipp", "shared_key_attention_mma"),
@@ -2169,4 +2170,11 @@ def attention_e4m3(q: torch.Tensor, out: torch.Tensor, kcache: torch.Tensor, vca
         return
     cache = (kcache, vcache, kscale, vscale, dt, block_table, block_table.shape[1], q_start, seq_lens)
     heads = (nq, nkv, d, kcache.shape[2], kcache.shape[0], window, scale, err)
-    _entries.rllm_attention_e4m3_simt(q, q.stride(0), out, *cache, 0, S, T, *heads)
+    if d not in (64, 128, 256) or kcache.shape[2] % 16:
+        _entries.rllm_attention_e4m3_simt(q, q.stride(0), out, *cache, 0, S, T, *heads)
+        return
+    keys = max_seq_len if window <= 0 else min(max_seq_len, window + max_q_len)
+    if num_decode:
+        _entries.rllm_attention_e4m3_rows(q, q.stride(0), out, *cache, 0, num_decode, 1, keys, *heads)
+    if num_decode < S:
+        _entries.rllm_attention_e4m3_rows(q, q.stride(0), out, *cache, num_decode, S, max_q_len, keys, *heads)

@@ -98,7 +98,8 @@ const Row kSignatures[] = {
     ROW("piiiiippfpppipppfiiiiiip"), ROW("piiippipp"), ROW("piiippp"), ROW("piiippppp"), ROW("piiippppppp"),
     ROW("piiipppppppi"), ROW("piippifpppfippppiiiiiippip"), ROW("piippippppiiipiiip"),
     ROW("piippppifpippiiiiiiipiiippififiip"), ROW("piippppippiiiiiiiiifiifppiipp"), ROW("piippppippiiiiiiiiifpi"),
-    ROW("piipppppipipppippiiiiiiiiipp"), ROW("piplpppipiippppiiiiiip"), ROW("pppiippppppiiiiiip"), ROW("pipppppipippiiiiiiiiifp"), ROW("piippppppppiiiiff"), ROW("piiipppppppppiiipiiiip"), ROW("pipifpipiiiiifff"),
+    ROW("piipppppipipppippiiiiiiiiipp"), ROW("piplpppipiippppiiiiiip"), ROW("pppiippppppiiiiiip"), ROW("pipppppipippiiiiiiiiifp"),
+    ROW("pipppppipippiiiiiiiiiifp"), ROW("piippppppppiiiiff"), ROW("piiipppppppppiiipiiiip"), ROW("pipifpipiiiiifff"),
     ROW("pipipiiii"), ROW("pipipiiiiifff"), ROW("pipipiiiiifffp"), ROW("pipipippipippiii"), ROW("pippifpppfipppppiiiiiiipp"),
     ROW("pippiiipppiiiiiiiifpp"), ROW("pippippppipppppppiiiiiiiiiiiiifffip"), ROW("pipppipippiiiiiiifp"),
     ROW("pipppipippiiiiiiiifiifppiipiip"), ROW("pipppipippiiiiiiip"), ROW("pipppippiiiiiiiiifpp"),

@@ -103,7 +103,9 @@ class Step:
         the products' absolute sum (the last 4: scale and power factors), q itself being exact as one or two halves or off by
         2^-22; a weight p is off by that, by 2^-21 (the exponential and its argument, of up to 2^5 in the log2 domain times
         2^-24, counted with 2^-17) and by the rounding of p to a half (2^-11), or to two of them (2^-22); the sums over the keys
-        add n 2^-24; the result is rounded once to its type."""
+        add n 2^-24; the result is rounded once to its type.  A half's step does not fall below 2^-24, so a weight, held as
+        p 2^ev 2^7 over a power of two that is at most the largest 2^ev in sight, is off by 2^-32 of that at least: over n keys
+        with numbers of at most 448, n 448 2^-32 max 2^ev, p being 1 at the row's reference and the weights' sum 1 at least."""
         scale = self.d ** -0.5 if scale is None else scale
         half = 2.0 ** -11 if self.dtype is torch.bfloat16 else 2.0 ** -22
         outs, bounds = [], []
@@ -136,7 +138,9 @@ class Step:
                 arg = torch.nan_to_num(sc.masked_fill(~seen, 0).abs()).amax(-1, keepdim=True) * 1.4427 * 2.0 ** -23
                 rel = 2 * (off + arg) + 2.0 ** -17 * (1.0 if self.dtype is torch.bfloat16 else 2.0 ** -4) + half + key.numel() * 2.0 ** -24
                 outs.append(out)
-                bounds.append(rel * (w @ vz.abs()) + torch.finfo(self.dtype).eps / 2 * out.abs() + 1e-30)
+                power = torch.where(seen.any(0)[:, None], vz.abs(), torch.zeros_like(vz)).amax() / 224        # 2^ev <= max|v| / 224
+                floor = key.numel() * 448 * 2.0 ** -32 * power
+                bounds.append(rel * (w @ vz.abs()) + floor + torch.finfo(self.dtype).eps / 2 * out.abs() + 1e-30)
         T = sum(self.lens)
         place = []
         i = 0
