@@ -152,6 +152,7 @@ static int e4_check(const void* q, const void* out, const void* kcache, const vo
 #define E4_WARPS 4
 #define E4_SLACK 4                   // log2 of how far a score may pass the row's reference, and a value's power the warp's
 #define E4_SHIFT 7                   // log2 of the weights' factor: 2 E4_SLACK + E4_SHIFT = 15
+#define E4_NONE -3.0e38f             // the reference of a row that has seen nothing: 2^(s - reference) is 0 for a masked s, and any score moves it
 __device__ __forceinline__ void e4_mma(float* c, const unsigned* a, unsigned b0, unsigned b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
@@ -172,53 +173,177 @@ __device__ __forceinline__ unsigned e4_pack(float a, float b) {
   return *(const unsigned*)&h;
 }
 __device__ __forceinline__ float2 e4_unpack(unsigned h) { return __half22float2(*(const __half2*)&h); }
+__device__ __forceinline__ unsigned e4_word(const uint4& x, int i) { return i == 0 ? x.x : i == 1 ? x.y : i == 2 ? x.z : x.w; }
 
-// a lane's part of a tile of 16 keys
-template <int D> struct E4Tile {
-  uint4 k[2][D / 64];
-  unsigned v[4][D / 32];
-  int kb[2], vb[2];                  // scale bytes of keys gid and gid + 8
-  bool held;
-};
+// N bytes from global to shared memory on their way; e4_copy_or_zero: zeros where the source is not to be read
+template <int N> __device__ __forceinline__ void e4_copy(unsigned dst, const void* src) {
+  if constexpr (N == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(N) : "memory");
+}
+template <int N> __device__ __forceinline__ void e4_copy_or_zero(unsigned dst, const void* src, bool valid) {
+  const int n = valid ? N : 0;
+  if constexpr (N == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], %3, %2;" ::"r"(dst), "l"(src), "r"(n), "n"(N) : "memory");
+}
+__device__ __forceinline__ void e4_copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void e4_copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+// a tile of 16 keys in shared memory: K's pieces, V's, 16 + 16 scale bytes; a pair is two of them
+template <int D, int NB, typename T> constexpr int e4_ctas() {  // of an SM
+  if (sizeof(T) == 2 && NB == 1) return D == 64 ? 5 : D == 128 ? 4 : 2;
+  return D == 64 ? 3 : D == 128 ? (NB == 1 ? 3 : 2) : 2;
+}
+template <int D> __host__ __device__ constexpr int e4_tile_bytes() { return 32 * D + 32; }
 
-template <int D, int NB, int PF, typename T>
-__global__ void __launch_bounds__(32 * E4_WARPS)
+template <int D, int NB, typename T>
+__global__ void __launch_bounds__(32 * E4_WARPS, e4_ctas<D, NB, T>())
 attention_e4m3_rows_kernel(const T* q, int q_stride, T* __restrict__ out, const unsigned char* __restrict__ kcache,
                            const unsigned char* __restrict__ vcache, const unsigned char* __restrict__ kscale,
                            const unsigned char* __restrict__ vscale, const int* __restrict__ block_table, int max_blocks,
                            const int* __restrict__ q_start, const int* __restrict__ seq_lens, int seq_begin, int nq, int nkv,
-                           int page_size, int num_pages, int window, float scale_log2, int* __restrict__ err) {
-  constexpr int R = 8 * NB, TERMS = sizeof(T) == 4 ? 2 : 1, KC = D / 64, VW = D / 32;
+                           int page_size, int num_pages, int window, float scale_log2, int q_wide, int* __restrict__ err) {
+  constexpr int R = 8 * NB, TERMS = sizeof(T) == 4 ? 2 : 1, KC = D / 64, VW = D / 32, TB = e4_tile_bytes<D>();
   extern __shared__ __align__(16) float e4_smem[];
-  pdl_wait_on(q, kcache, vcache, kscale, vscale);
-  pdl_launch();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, gid = lane >> 2, tig = lane & 3;
   const int C = gridDim.x, rank = blockIdx.x;      // the cluster is the grid's x
   const int kvh = blockIdx.y % nkv, s = seq_begin + blockIdx.z;
   const int g = nq / nkv;
   const int qs = q_start[s], qlen = q_start[s + 1] - qs, len = seq_lens[s];
   const int rows = qlen * g, r0 = blockIdx.y / nkv * R;
-  if (r0 >= rows) return;                          // the whole cluster
+  if (r0 >= rows) { pdl_wait(); return; }          // the whole cluster (a CTA that exits lets the next kernel in: it waits first)
   const int pos0 = len - qlen;
   const int t_first = r0 / g, t_last = (min(r0 + R, rows) - 1) / g;
   const int hi_first = pos0 + t_first + 1, kend = min(pos0 + t_last + 1, max_blocks * page_size);
   const int kmin = window > 0 ? max(0, hi_first - window) : 0;
   const int lo_last = window > 0 ? max(0, pos0 + t_last + 1 - window) : 0;
-  const int t_hi = (kend + 15) >> 4, stride = C * E4_WARPS;
   const int* bt = block_table + (size_t)s * max_blocks;
+  // A warp's pairs of tiles of 16 keys: tiles t0 + i stride and the next.  Lane l holds where tile (l & 1) of pair i lies, l / 2 =
+  // i % 16 (its first cache row / 16; -1: not held or behind the end): 16 pairs are looked up at a time, for a lookup a tile
+  // would stand, as a second trip to memory, between a tile and its loads.
+  const int page_tiles = page_size >> 4, page_shift = (page_tiles & (page_tiles - 1)) == 0 ? __ffs(page_tiles) - 1 : -1;
+  const int t_hi = (kend + 15) >> 4, stride = 2 * C * E4_WARPS, t0 = (kmin >> 4) + 2 * (rank * E4_WARPS + warp);
+  const int pairs = t_hi > t0 ? (t_hi - t0 + stride - 1) / stride : 0;
+  int places0 = -1, places1 = -1;      // of the even and the odd 16s: pairs on their way may lie 16 beyond the one at hand
+  bool missing = false;                // a page of the warp's is not held (from where it is looked up on)
+  auto look_up = [&](int i) {
+    const int t = t0 + (i + (lane >> 1)) * stride + (lane & 1);
+    int place = -1;
+    bool bad = false;
+    if (t < t_hi) {
+      const int at = page_shift >= 0 ? t >> page_shift : t / page_tiles, page = bt[at];
+      bad = page < 0 || page >= num_pages;
+      if (!bad) place = (page * nkv + kvh) * page_tiles + (t - at * page_tiles);
+    }
+    if (__any_sync(0xffffffffu, bad)) {
+      missing = true;
+      if (bad) atomicOr(err, 4);
+    }
+    if (i & 16) places1 = place; else places0 = place;
+  };
+  auto place_of = [&](int i, int u) { return __shfl_sync(0xffffffffu, (i & 16) ? places1 : places0, (2 * i + u) & 31); };
+  look_up(0);
+  pdl_wait_on(q, kcache, vcache, kscale, vscale);
+  pdl_launch();
+  // A warp's pair lies behind the queries: for each tile [pieces][32 lanes] of 16 bytes of K, then of V, and its scales.  A lane
+  // reads back what it copied itself (the scales apart), each of its accesses 16 bytes beside its neighbour's.  There is one
+  // place for K and one for V: the next pair's keys are asked for when this pair's scores are made, its values behind this
+  // pair's products, so that each is on its way for about half a pair's time; twice the places left room for 12 warps an SM
+  // instead of 16, which is what bounds the kernel (see below).
+  constexpr int VP = D == 64 ? 8 : 16, VN = D / 8 / VP;           // bytes and number of a lane's pieces of a value row
+  constexpr int RING = (int)sizeof(float) * R * (D + 4);
+  const unsigned char* st = (const unsigned char*)e4_smem + RING + warp * 2 * TB;
+  const unsigned ring = (unsigned)__cvta_generic_to_shared(st);
+  auto whole_pair = [&](int j0) { return !missing && j0 >= kmin && j0 + 32 <= kend; };
+  // rows outside [kmin, kend) or not held come in as zeros: whatever lies there stays out
+  auto issue_k = [&](int i) {
+    if (i < pairs) {
+      if ((i & 15) == 0 && i > 0) look_up(i);
+      const int j0 = (t0 + i * stride) << 4;
+      const bool whole = whole_pair(j0);
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int place = place_of(i, u);
+        const long long row = (long long)place * 16;
+        const unsigned char* kp = kcache + row * D + gid * D + tig * 16;
+        const unsigned dst = ring + u * TB + lane * 16, sdst = ring + u * TB + 32 * D;
+        if (whole) {
+#pragma unroll
+          for (int r = 0; r < 2; ++r)
+#pragma unroll
+            for (int c = 0; c < KC; ++c) e4_copy<16>(dst + (r * KC + c) * 512, kp + r * 8 * D + c * 64);
+          if (lane == 0) e4_copy<16>(sdst, kscale + row);
+        } else {
+          const int lo = kmin - j0 - 16 * u, hi = place >= 0 ? kend - j0 - 16 * u : -1000;
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            const bool ok = gid + 8 * r >= lo && gid + 8 * r < hi;
+#pragma unroll
+            for (int c = 0; c < KC; ++c) e4_copy_or_zero<16>(dst + (r * KC + c) * 512, ok ? kp + r * 8 * D + c * 64 : kcache, ok);
+          }
+          if (lane == 0) e4_copy_or_zero<16>(sdst, place >= 0 ? kscale + row : kscale, place >= 0);
+        }
+      }
+    }
+    e4_copy_commit();
+  };
+  auto issue_v = [&](int i) {
+    if (i < pairs) {
+      const int j0 = (t0 + i * stride) << 4;
+      const bool whole = whole_pair(j0);
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int place = place_of(i, u);
+        const long long row = (long long)place * 16;
+        const unsigned char* vp = vcache + row * D + 2 * tig * D + gid * (D / 8);
+        const unsigned dst = ring + u * TB + 16 * D + lane * VP, sdst = ring + u * TB + 32 * D + 16;
+        if (whole) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int c = 0; c < VN; ++c) e4_copy<VP>(dst + (r * VN + c) * 32 * VP, vp + ((r & 1) + 8 * (r >> 1)) * D + c * VP);
+          if (lane == 0) e4_copy<16>(sdst, vscale + row);
+        } else {
+          const int lo = kmin - j0 - 16 * u, hi = place >= 0 ? kend - j0 - 16 * u : -1000;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int at = (r & 1) + 8 * (r >> 1);
+            const bool ok = 2 * tig + at >= lo && 2 * tig + at < hi;
+#pragma unroll
+            for (int c = 0; c < VN; ++c) e4_copy_or_zero<VP>(dst + (r * VN + c) * 32 * VP, ok ? vp + at * D + c * VP : vcache, ok);
+          }
+          if (lane == 0) e4_copy_or_zero<16>(sdst, place >= 0 ? vscale + row : vscale, place >= 0);
+        }
+      }
+    }
+    e4_copy_commit();
+  };
+  issue_k(0);
+  issue_v(0);
 
   // the tile's queries, as float32 rows of D + 4
   float* sQ = e4_smem;
-  for (int i = threadIdx.x; i < R * D; i += 32 * E4_WARPS) {
+  constexpr int QV = sizeof(T) == 4 ? 4 : 8;         // values of 16 bytes
+  for (int i = threadIdx.x * QV; i < R * D; i += 32 * E4_WARPS * QV) {
     const int r = i / D, c = i - r * D, row = r0 + r;
-    float x = 0.f;
-    if (row < rows) x = to_f32(q[(size_t)(qs + row / g) * q_stride + (size_t)(kvh * g + row % g) * D + c]);
-    sQ[r * (D + 4) + c] = x;
+    float x[QV];
+#pragma unroll
+    for (int e = 0; e < QV; ++e) x[e] = 0.f;
+    if (row < rows) {
+      const int tok = row / g;
+      const T* src = q + (size_t)(qs + tok) * q_stride + (size_t)(kvh * g + row - tok * g) * D + c;
+      if (q_wide) {
+        if constexpr (sizeof(T) == 4) { const float4 y = *(const float4*)src; x[0] = y.x; x[1] = y.y; x[2] = y.z; x[3] = y.w; }
+        else load8(src, x);
+      } else {
+#pragma unroll
+        for (int e = 0; e < QV; ++e) x[e] = to_f32(src[e]);
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < QV; e += 4) *(float4*)(sQ + r * (D + 4) + c + e) = make_float4(x[e], x[e + 1], x[e + 2], x[e + 3]);
   }
   __syncthreads();
   unsigned qf[NB][D / 16][2 * TERMS];
   float rfc[NB][2];
-  int hi[NB][2];
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) {
     const float* qr = sQ + (nb * 8 + gid) * (D + 4) + tig * 16;
@@ -233,7 +358,7 @@ attention_e4m3_rows_kernel(const T* q, int q_stride, T* __restrict__ out, const 
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
     const int e = min(max((int)(__float_as_uint(top) >> 23) - 127, -100), 127);     // top < 2^(e + 1)
-    const float down = __uint_as_float((unsigned)(127 + 13 - e) << 23), up = __uint_as_float((unsigned)max(127 - 13 + e, 1) << 23) * scale_log2;
+    const float down = __uint_as_float((unsigned)(127 + 13 - e) << 23), up = __uint_as_float((unsigned)(127 - 13 + e) << 23) * scale_log2;
 #pragma unroll
     for (int kk = 0; kk < D / 16; ++kk) {
       const float4 x = *(const float4*)(qr + (kk >> 2) * 64 + (kk & 3) * 4);
@@ -247,104 +372,115 @@ attention_e4m3_rows_kernel(const T* q, int q_stride, T* __restrict__ out, const 
       }
     }
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      rfc[nb][c] = __shfl_sync(0xffffffffu, up, (2 * tig + c) * 4);
-      hi[nb][c] = pos0 + min(r0 + nb * 8 + 2 * tig + c, rows - 1) / g + 1;
-    }
+    for (int c = 0; c < 2; ++c) rfc[nb][c] = __shfl_sync(0xffffffffu, up, (2 * tig + c) * 4);
   }
 
   float o[NB][D / 16][4], m[NB][2], l[NB][2];
-  int E = -1000;
+  int E = -1000;                       // the warp's reference of the values' powers, as a scale byte
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) {
-    m[nb][0] = m[nb][1] = -INFINITY;
+    m[nb][0] = m[nb][1] = E4_NONE;
     l[nb][0] = l[nb][1] = 0.f;
 #pragma unroll
     for (int j = 0; j < D / 16; ++j) o[nb][j][0] = o[nb][j][1] = o[nb][j][2] = o[nb][j][3] = 0.f;
   }
 
-  auto load = [&](E4Tile<D>& x, int t) {
-    x.held = false;
-    if (t >= t_hi) return;
-    const int j0 = t << 4, pi = j0 / page_size;
-    const int page = bt[pi];
-    x.held = page >= 0 && page < num_pages;
-    if (!x.held && lane == 0) atomicOr(err, 4);
-    const long long row = x.held ? ((long long)page * nkv + kvh) * page_size + (j0 - pi * page_size) : 0;
-    const unsigned char *kp = kcache + row * D, *vp = vcache + row * D;
+  for (int i = 0; i < pairs; ++i) {
+    const int j0 = (t0 + i * stride) << 4;
+    const bool whole = whole_pair(j0);
+    const bool clear = whole && j0 >= lo_last && j0 + 32 <= hi_first;
+    e4_copy_wait<1>();                 // the keys are here; the values may be on their way
+    __syncwarp();
+    int kb[4];                         // scale bytes of keys gid and gid + 8 of the two tiles
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int r = gid + 8 * i;
-      const bool ok = x.held && j0 + r >= kmin && j0 + r < kend;
+    for (int x = 0; x < 4; ++x) kb[x] = st[(x >> 1) * TB + 32 * D + gid + 8 * (x & 1)];
+    // the products of the two tiles in turn (each waits for the one before it of its own sum), and two sums a tile where
+    // registers allow
+    constexpr int SUMS = NB == 1 && TERMS == 1 ? 2 : 1;
+    float sc[2][NB][4], sd[2][NB][4];
 #pragma unroll
-      for (int c = 0; c < KC; ++c) x.k[i][c] = ok ? *(const uint4*)(kp + r * D + c * 64 + tig * 16) : make_uint4(0u, 0u, 0u, 0u);
-      x.kb[i] = ok ? kscale[row + r] : 0;
-      x.vb[i] = ok ? vscale[row + r] : 0;
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int r = 2 * tig + (i & 1) + 8 * (i >> 1);
-      const bool ok = x.held && j0 + r >= kmin && j0 + r < kend;
-      const unsigned char* p = vp + r * D + gid * (D / 8);
-      if constexpr (D == 64) {
-        const uint2 y = ok ? *(const uint2*)p : make_uint2(0u, 0u);
-        x.v[i][0] = y.x; x.v[i][1] = y.y;
-      } else {
-#pragma unroll
-        for (int c = 0; c < VW; c += 4) {
-          const uint4 y = ok ? *(const uint4*)(p + c * 4) : make_uint4(0u, 0u, 0u, 0u);
-          x.v[i][c] = y.x; x.v[i][c + 1] = y.y; x.v[i][c + 2] = y.z; x.v[i][c + 3] = y.w;
-        }
-      }
-    }
-  };
-
-  auto compute = [&](const E4Tile<D>& x, int t) {
-    const int j0 = t << 4;
-    float sc[NB][4];
-#pragma unroll
-    for (int nb = 0; nb < NB; ++nb) sc[nb][0] = sc[nb][1] = sc[nb][2] = sc[nb][3] = 0.f;
-#pragma unroll
-    for (int kk = 0; kk < D / 16; ++kk) {
-      const uint4 ka = x.k[0][kk >> 2], kb = x.k[1][kk >> 2];
-      const unsigned wa = (kk & 3) == 0 ? ka.x : (kk & 3) == 1 ? ka.y : (kk & 3) == 2 ? ka.z : ka.w;
-      const unsigned wb = (kk & 3) == 0 ? kb.x : (kk & 3) == 1 ? kb.y : (kk & 3) == 2 ? kb.z : kb.w;
-      const unsigned a[4] = {kv8_halves_lo(wa), kv8_halves_lo(wb), kv8_halves_hi(wa), kv8_halves_hi(wb)};
-#pragma unroll
-      for (int nb = 0; nb < NB; ++nb) {
-        e4_mma(sc[nb], a, qf[nb][kk][0], qf[nb][kk][1]);
-        if (TERMS == 2) e4_mma(sc[nb], a, qf[nb][kk][2 * TERMS - 2], qf[nb][kk][2 * TERMS - 1]);
-      }
-    }
-    const bool clear = x.held && j0 >= lo_last && j0 >= kmin && j0 + 16 <= hi_first && j0 + 16 <= kend;
-    const float kf[2] = {kv8_power(x.kb[0]), kv8_power(x.kb[1])};
-    unsigned seen = 0xffffffffu;                       // bit nb * 4 + e
-    if (!clear) {
-      seen = 0u;
+    for (int u = 0; u < 2; ++u)
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int j = j0 + gid + 8 * (e >> 1), h = min(hi[nb][e & 1], kend);
-          if (x.held && j < h && (window == 0 || j >= hi[nb][e & 1] - window)) seen |= 1u << (nb * 4 + e);
+        for (int e = 0; e < 4; ++e) sc[u][nb][e] = sd[u][nb][e] = 0.f;
+#pragma unroll
+    for (int c = 0; c < KC; ++c) {
+      uint4 kx[2][2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) kx[u][r] = *(const uint4*)(st + u * TB + (r * KC + c) * 512 + lane * 16);
+#pragma unroll
+      for (int w = 0; w < 4; ++w)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const unsigned wa = e4_word(kx[u][0], w), wc = e4_word(kx[u][1], w);
+          const unsigned a[4] = {kv8_halves_lo(wa), kv8_halves_lo(wc), kv8_halves_hi(wa), kv8_halves_hi(wc)};
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb) {
+            e4_mma(SUMS == 2 && (w & 1) ? sd[u][nb] : sc[u][nb], a, qf[nb][c * 4 + w][0], qf[nb][c * 4 + w][1]);
+            if (TERMS == 2) e4_mma(sc[u][nb], a, qf[nb][c * 4 + w][2 * TERMS - 2], qf[nb][c * 4 + w][2 * TERMS - 1]);
+          }
         }
     }
-    const int v0 = x.vb[0] == KV8_NAN_SCALE ? 0 : x.vb[0], v1 = x.vb[1] == KV8_NAN_SCALE ? 0 : x.vb[1];
-    bool need = max(v0, v1) > E + E4_SLACK;
+    __syncwarp();                      // every lane has read the keys and their scales
+    issue_k(i + 1);
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      // 2^ek; 255 becomes infinity, which makes NaN of the row's zeros (and 0 a zero: such rows are below 2^-118)
+      const float kf = __uint_as_float((unsigned)kb[x] << 23);
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          float& v = sc[x >> 1][nb][2 * (x & 1) + c];
+          if (SUMS == 2) v += sd[x >> 1][nb][2 * (x & 1) + c];
+          v = v * rfc[nb][c] * kf;
+        }
+    }
+    unsigned seen = 0xffffffffu;       // bit nb * 8 + u * 4 + e
+    if (!clear) {
+      seen = 0u;
+      const bool held[2] = {place_of(i, 0) >= 0, place_of(i, 1) >= 0};
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const int hi = pos0 + min(r0 + nb * 8 + 2 * tig + c, rows - 1) / g + 1, lo = window > 0 ? hi - window : 0;
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            const int j = j0 + gid + 8 * x;
+            if (held[x >> 1] && j < min(hi, kend) && j >= lo) seen |= 1u << (nb * 8 + 2 * x + c);
+            else sc[x >> 1][nb][2 * (x & 1) + c] = -INFINITY;
+          }
+        }
+    }
+    e4_copy_wait<1>();                 // the values are here; the next keys may be on their way
+    __syncwarp();
+    int vb[4];
+#pragma unroll
+    for (int x = 0; x < 4; ++x) vb[x] = st[(x >> 1) * TB + 32 * D + 16 + gid + 8 * (x & 1)];
+    if (!whole) {                      // (a row that was not read has zeros, whatever its scale)
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const int j = j0 + gid + 8 * x;
+        if (j < kmin || j >= kend) vb[x] = 0;
+      }
+    }
+    bool need = max(max(vb[0], vb[1]), max(vb[2], vb[3])) > E + E4_SLACK;
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        float v = sc[nb][e] * rfc[nb][e & 1] * kf[e >> 1];
-        if (!(seen >> (nb * 4 + e) & 1u)) v = -INFINITY;
-        sc[nb][e] = v;
-        need = need || v > m[nb][e & 1] + (float)E4_SLACK;
-      }
+      for (int e = 0; e < 8; ++e) need = need || sc[e >> 2][nb][e & 3] > m[nb][e & 1] + (float)E4_SLACK;
     if (__any_sync(0xffffffffu, need)) {
-      const int vmax = __reduce_max_sync(0xffffffffu, max(v0, v1));
+      int vmax = 0;
+#pragma unroll
+      for (int x = 0; x < 4; ++x) vmax = max(vmax, vb[x] == KV8_NAN_SCALE ? 0 : vb[x]);
+      vmax = __reduce_max_sync(0xffffffffu, vmax);
       float fe = 1.0f;
       if (vmax > E + E4_SLACK) {
-        fe = E - vmax < -126 ? 0.f : __uint_as_float((unsigned)(127 + E - vmax) << 23);
+        fe = __uint_as_float((unsigned)max(127 + E - vmax, 0) << 23);
         E = vmax;
       }
 #pragma unroll
@@ -352,7 +488,7 @@ attention_e4m3_rows_kernel(const T* q, int q_stride, T* __restrict__ out, const 
         float corr[2];
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          float mx = fmaxf(sc[nb][c], sc[nb][c + 2]);
+          float mx = fmaxf(fmaxf(sc[0][nb][c], sc[0][nb][c + 2]), fmaxf(sc[1][nb][c], sc[1][nb][c + 2]));
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
@@ -366,68 +502,77 @@ attention_e4m3_rows_kernel(const T* q, int q_stride, T* __restrict__ out, const 
         for (int j = 0; j < D / 16; ++j) { o[nb][j][0] *= corr[0]; o[nb][j][1] *= corr[1]; o[nb][j][2] *= corr[0]; o[nb][j][3] *= corr[1]; }
       }
     }
-    // 2^(ev - E + E4_SHIFT) of the lane's two keys
-    float vf[2];
+    float vf[4];                       // 2^(ev - E + E4_SHIFT); infinity for a NaN scale
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-      vf[i] = x.vb[i] == KV8_NAN_SCALE ? __uint_as_float(0x7FC00000u)
-                                       : (x.vb[i] - E + E4_SHIFT < -126 ? 0.f : __uint_as_float((unsigned)(127 + E4_SHIFT + x.vb[i] - E) << 23));
-    unsigned pb[NB][2 * TERMS];
+    for (int x = 0; x < 4; ++x) vf[x] = __uint_as_float((unsigned)min(max(vb[x] == KV8_NAN_SCALE ? 255 : 127 + E4_SHIFT + vb[x] - E, 0), 255) << 23);
+    unsigned pb[2][NB][2 * TERMS];
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb) {
-      float w[4];
+    for (int u = 0; u < 2; ++u) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float mm = m[nb][e & 1] == -INFINITY ? 0.f : m[nb][e & 1];
-        const float p = e4_ex2(sc[nb][e] - mm);
-        l[nb][e & 1] += p;
-        w[e] = (seen >> (nb * 4 + e) & 1u) ? p * vf[e >> 1] : 0.f;
-      }
-      const unsigned h0 = e4_pack(w[0], w[1]), h1 = e4_pack(w[2], w[3]);
-      pb[nb][0] = e4_turn(h0);
-      pb[nb][1] = e4_turn(h1);
-      if (TERMS == 2) {
-        const float2 a = e4_unpack(h0), b = e4_unpack(h1);
-        pb[nb][2 * TERMS - 2] = e4_turn(e4_pack(w[0] - a.x, w[1] - a.y));
-        pb[nb][2 * TERMS - 1] = e4_turn(e4_pack(w[2] - b.x, w[3] - b.y));
-      }
-    }
+      for (int nb = 0; nb < NB; ++nb) {
+        float w[4];
 #pragma unroll
-    for (int c = 0; c < VW; ++c) {
-      // bytes 4 c .. 4 c + 3 of keys 2 tig and 2 tig + 1, and of the two 8 keys on, as pairs along the keys
-      const unsigned a01 = __byte_perm(x.v[0][c], x.v[1][c], 0x5140), a23 = __byte_perm(x.v[0][c], x.v[1][c], 0x7362);
-      const unsigned b01 = __byte_perm(x.v[2][c], x.v[3][c], 0x5140), b23 = __byte_perm(x.v[2][c], x.v[3][c], 0x7362);
-      const unsigned a[2][4] = {{kv8_halves_lo(a01), kv8_halves_hi(a01), kv8_halves_lo(b01), kv8_halves_hi(b01)},
-                                {kv8_halves_lo(a23), kv8_halves_hi(a23), kv8_halves_lo(b23), kv8_halves_hi(b23)}};
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int nb = 0; nb < NB; ++nb) {
-          e4_mma(o[nb][2 * c + i], a[i], pb[nb][0], pb[nb][1]);
-          if (TERMS == 2) e4_mma(o[nb][2 * c + i], a[i], pb[nb][2 * TERMS - 2], pb[nb][2 * TERMS - 1]);
+        for (int e = 0; e < 4; ++e) {
+          const float p = e4_ex2(sc[u][nb][e] - m[nb][e & 1]);
+          l[nb][e & 1] += p;
+          w[e] = p * vf[2 * u + (e >> 1)];
         }
-    }
-  };
-
-  {
-    E4Tile<D> buf[PF];
-    int t = (kmin >> 4) + rank * E4_WARPS + warp;
+        if (!clear) {                  // 0 times an infinite power is not 0
 #pragma unroll
-    for (int i = 0; i < PF; ++i) load(buf[i], t + i * stride);
-    for (; t < t_hi; t += PF * stride) {
-#pragma unroll
-      for (int i = 0; i < PF; ++i) {
-        if (t + i * stride < t_hi) {
-          compute(buf[i], t + i * stride);
-          load(buf[i], t + (i + PF) * stride);
+          for (int e = 0; e < 4; ++e)
+            if (!(seen >> (nb * 8 + u * 4 + e) & 1u)) w[e] = 0.f;
+        }
+        const unsigned h0 = e4_pack(w[0], w[1]), h1 = e4_pack(w[2], w[3]);
+        pb[u][nb][0] = e4_turn(h0);
+        pb[u][nb][1] = e4_turn(h1);
+        if (TERMS == 2) {
+          const float2 a = e4_unpack(h0), b = e4_unpack(h1);
+          pb[u][nb][2 * TERMS - 2] = e4_turn(e4_pack(w[0] - a.x, w[1] - a.y));
+          pb[u][nb][2 * TERMS - 1] = e4_turn(e4_pack(w[2] - b.x, w[3] - b.y));
         }
       }
     }
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      unsigned xv[4][VW];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        if constexpr (D == 64) {
+          const uint2 y = *(const uint2*)(st + u * TB + 16 * D + r * 256 + lane * 8);
+          xv[r][0] = y.x; xv[r][1] = y.y;
+        } else {
+#pragma unroll
+          for (int c = 0; c < VN; ++c) {
+            const uint4 y = *(const uint4*)(st + u * TB + 16 * D + (r * VN + c) * 512 + lane * 16);
+            xv[r][4 * c] = y.x; xv[r][4 * c + 1] = y.y; xv[r][4 * c + 2] = y.z; xv[r][4 * c + 3] = y.w;
+          }
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < VW; ++c) {
+        // bytes 4 c .. 4 c + 3 of keys 2 tig and 2 tig + 1, and of the two 8 keys on, as pairs along the keys
+        const unsigned a01 = __byte_perm(xv[0][c], xv[1][c], 0x5140), a23 = __byte_perm(xv[0][c], xv[1][c], 0x7362);
+        const unsigned b01 = __byte_perm(xv[2][c], xv[3][c], 0x5140), b23 = __byte_perm(xv[2][c], xv[3][c], 0x7362);
+        const unsigned a[2][4] = {{kv8_halves_lo(a01), kv8_halves_hi(a01), kv8_halves_lo(b01), kv8_halves_hi(b01)},
+                                  {kv8_halves_lo(a23), kv8_halves_hi(a23), kv8_halves_lo(b23), kv8_halves_hi(b23)}};
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb) {
+            e4_mma(o[nb][2 * c + x], a[x], pb[u][nb][0], pb[u][nb][1]);
+            if (TERMS == 2) e4_mma(o[nb][2 * c + x], a[x], pb[u][nb][2 * TERMS - 2], pb[u][nb][2 * TERMS - 1]);
+          }
+      }
+    }
+    __syncwarp();                      // every lane has read the values and their scales
+    issue_v(i + 1);
   }
+  e4_copy_wait<0>();
 
-  // the CTA's result: parts [warps][R][D], and every warp's maximum and sum of each row
+  // the CTA's result: parts [warps][R][D + 4], and every warp's reference and sum of each row
+  constexpr int LD = D + 4;
   float* part = e4_smem;
-  float* sM = part + E4_WARPS * R * D;               // [warps][R]
+  float* sM = part + E4_WARPS * R * LD;              // [warps][R]
   float* sL = sM + E4_WARPS * R;
   float* cM = sL + E4_WARPS * R;                     // [R] the CTA's
   float* cL = cM + R;
@@ -437,7 +582,7 @@ attention_e4m3_rows_kernel(const T* q, int q_stride, T* __restrict__ out, const 
     for (int c = 0; c < 2; ++c)
 #pragma unroll
       for (int x = 4; x < 32; x <<= 1) l[nb][c] += __shfl_xor_sync(0xffffffffu, l[nb][c], x);
-  __syncthreads();                                   // the queries have been read
+  __syncthreads();                                   // the queries and all tiles have been read
   if (gid == 0) {
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb)
@@ -457,10 +602,11 @@ attention_e4m3_rows_kernel(const T* q, int q_stride, T* __restrict__ out, const 
       float top = sM[r];
 #pragma unroll
       for (int w = 1; w < E4_WARPS; ++w) top = fmaxf(top, sM[w * R + r]);
-      const float f = m[nb][c] == -INFINITY ? (l[nb][c] == 0.f ? 0.f : l[nb][c]) : e4_ex2(m[nb][c] - top) * fe;
-      float* dst = part + ((size_t)warp * R + r) * D + gid * (D / 8);
+      const float f = e4_ex2(m[nb][c] - top) * fe;
+      float* dst = part + (warp * R + r) * LD + gid * (D / 8);
 #pragma unroll
-      for (int j = 0; j < D / 16; ++j) *(float2*)(dst + 2 * j) = make_float2(o[nb][j][c] * f, o[nb][j][c + 2] * f);
+      for (int j = 0; j < D / 16; j += 2)
+        *(float4*)(dst + 2 * j) = make_float4(o[nb][j][c] * f, o[nb][j][c + 2] * f, o[nb][j + 1][c] * f, o[nb][j + 1][c + 2] * f);
     }
   if (threadIdx.x < R) {
     const int r = threadIdx.x;
@@ -468,60 +614,74 @@ attention_e4m3_rows_kernel(const T* q, int q_stride, T* __restrict__ out, const 
 #pragma unroll
     for (int w = 1; w < E4_WARPS; ++w) top = fmaxf(top, sM[w * R + r]);
 #pragma unroll
-    for (int w = 0; w < E4_WARPS; ++w) sum += sL[w * R + r] * (sM[w * R + r] == -INFINITY ? 1.0f : e4_ex2(sM[w * R + r] - top));
+    for (int w = 0; w < E4_WARPS; ++w) sum += sL[w * R + r] * e4_ex2(sM[w * R + r] - top);
     cM[r] = top;
     cL[r] = sum;
   }
   __syncthreads();
-  auto store = [&](int i, float x, float sum) {
-    const int r = i / D, row = r0 + r;
+  auto store = [&](int r, int c, const float4& x, float sum) {
+    const int row = r0 + r;
     if (row < rows) {
       const float inv = sum == 0.f ? 0.f : 1.0f / sum;   // NaN stays NaN
-      out[((size_t)(qs + row / g) * nq + kvh * g + row % g) * D + (i - r * D)] = from_f32<T>(x * inv);
+      const int tok = row / g;
+      T* dst = out + ((size_t)(qs + tok) * nq + kvh * g + row - tok * g) * D + c;
+      if constexpr (sizeof(T) == 4) {
+        *(float4*)dst = make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv);
+      } else {
+        const __nv_bfloat162 lo = __floats2bfloat162_rn(x.x * inv, x.y * inv), hi = __floats2bfloat162_rn(x.z * inv, x.w * inv);
+        *(uint2*)dst = make_uint2(*(const unsigned*)&lo, *(const unsigned*)&hi);
+      }
     }
   };
-  for (int i = threadIdx.x; i < R * D; i += 32 * E4_WARPS) {
-    float x = part[i];
+  for (int i = threadIdx.x * 4; i < R * D; i += 32 * E4_WARPS * 4) {
+    const int r = i / D, c = i - r * D;
+    float4 x = *(const float4*)(part + r * LD + c);
 #pragma unroll
-    for (int w = 1; w < E4_WARPS; ++w) x += part[w * R * D + i];
-    if (C == 1) store(i, x, cL[i / D]);
-    else part[i] = x;
+    for (int w = 1; w < E4_WARPS; ++w) {
+      const float4 y = *(const float4*)(part + (w * R + r) * LD + c);
+      x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
+    }
+    if (C == 1) store(r, c, x, cL[r]);
+    else *(float4*)(part + r * LD + c) = x;
   }
   if (C == 1) return;
   namespace cg = cooperative_groups;
   cg::cluster_group cluster = cg::this_cluster();
   cluster.sync();
-  for (int i = rank * 32 * E4_WARPS + threadIdx.x; i < R * D; i += C * 32 * E4_WARPS) {
-    const int r = i / D;
-    float top = -INFINITY, x = 0.f, sum = 0.f;
+  for (int i = (rank * 32 * E4_WARPS + threadIdx.x) * 4; i < R * D; i += C * 32 * E4_WARPS * 4) {
+    const int r = i / D, at = r * LD + i - r * D;
+    float top = E4_NONE, sum = 0.f;
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int c = 0; c < C; ++c) top = fmaxf(top, cluster.map_shared_rank(cM, c)[r]);
     for (int c = 0; c < C; ++c) {
-      const float mc = cluster.map_shared_rank(cM, c)[r];
-      const float f = mc == -INFINITY ? 1.0f : e4_ex2(mc - top);
-      x += cluster.map_shared_rank(part, c)[i] * f;
+      const float f = e4_ex2(cluster.map_shared_rank(cM, c)[r] - top);
+      const float4 y = *(const float4*)(cluster.map_shared_rank(part, c) + at);
+      x.x = fmaf(y.x, f, x.x); x.y = fmaf(y.y, f, x.y); x.z = fmaf(y.z, f, x.z); x.w = fmaf(y.w, f, x.w);
       sum += cluster.map_shared_rank(cL, c)[r] * f;
     }
-    store(i, x, sum);
+    store(r, i - r * D, x, sum);
   }
   cluster.sync();                                    // nobody leaves while its shared memory is being read
 }
 
-template <int D, int NB, int PF, typename T>
+template <int D, int NB, typename T>
 static int e4_rows_launch(const void* q, int q_stride, void* out, const void* kcache, const void* vcache, const void* kscale,
                           const void* vscale, const int* block_table, int max_blocks, const int* q_start, const int* seq_lens,
                           int seq_begin, int num_seqs, int max_q_len, int max_keys, int nq, int nkv, int page_size,
                           int num_pages, int window, float scale, int* err, cudaStream_t stream) {
   constexpr int R = 8 * NB;
-  auto* kernel = attention_e4m3_rows_kernel<D, NB, PF, T>;
-  const size_t stage = sizeof(float) * R * (D + 4), merge = sizeof(float) * (E4_WARPS * R * (D + 2) + 2 * R);
-  const size_t smem = stage > merge ? stage : merge;
+  auto* kernel = attention_e4m3_rows_kernel<D, NB, T>;
+  const size_t stage = sizeof(float) * R * (D + 4), merge = sizeof(float) * (E4_WARPS * R * (D + 6) + 2 * R);
+  const size_t rings = stage + E4_WARPS * 2 * e4_tile_bytes<D>(), smem = rings > merge ? rings : merge;
   static SmemLimit limit;
   if (const int e = limit.allow(kernel, (int)smem)) return e;
   const long long tiles = ((long long)max_q_len * (nq / nkv) + R - 1) / R, units = tiles * nkv * num_seqs;
   if (tiles * nkv > 65535 || num_seqs > 65535) return RLLM_E_UNSUPPORTED;
-  // CTAs a unit: enough for the GPU, but two tiles of keys a warp at least
+  // CTAs a unit: to fill the GPU's places, of 128 keys at least (a CTA costs 2 us beside its keys); where there are enough of
+  // them and keys are many, several rounds of CTAs, so that the last round is short beside the rest (64 sequences of 4,000 to
+  // 12,000 keys, 32/8 heads of 128: 270 us with one CTA, 252 with two, 238 with four, 242 with eight)
   int C = 1;
-  while (C < 8 && units * C * 2 <= 592 && C * 2 * E4_WARPS * 32 <= max_keys) C *= 2;
+  while (C < 8 && ((units * C * 2 <= 592 && C * 2 * 128 <= max_keys) || (units * C * 2 <= 2368 && C * 2 * 1024 <= max_keys))) C *= 2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)C, (unsigned)(tiles * nkv), (unsigned)num_seqs);
   cfg.blockDim = dim3(32 * E4_WARPS);
@@ -539,7 +699,8 @@ static int e4_rows_launch(const void* q, int q_stride, void* out, const void* kc
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, (const T*)q, q_stride, (T*)out, (const unsigned char*)kcache,
                                            (const unsigned char*)vcache, (const unsigned char*)kscale, (const unsigned char*)vscale,
                                            block_table, max_blocks, q_start, seq_lens, seq_begin, nq, nkv, page_size, num_pages,
-                                           window, scale * 1.4426950408889634f, err);
+                                           window, scale * 1.4426950408889634f,
+                                           (((uintptr_t)q | ((uintptr_t)q_stride * sizeof(T))) & 15) == 0 ? 1 : 0, err);
   if (e != cudaSuccess) { cudaGetLastError(); return (int)e; }
   RLLM_LAUNCH_CHECK();
   return 0;
@@ -555,21 +716,22 @@ RLLM_EXPORT int rllm_attention_e4m3_rows(const void* q, int q_stride, void* out,
   if (max_q_len <= 0 || seq_end <= seq_begin) return 0;
   if (const int rc = e4_check(q, out, kcache, vcache, kscale, vscale, block_table, max_blocks, q_start, seq_lens, seq_begin,
                               seq_end, nq, nkv, d, page_size, num_pages, window, scale, err)) return rc;
-  if (page_size % 16 || !(d == 64 || d == 128 || d == 256)) return RLLM_E_UNSUPPORTED;
-#define E4_ROWS(DD, NBB, PFF, TT)                                                                                              \
-  return e4_rows_launch<DD, NBB, PFF, TT>(q, q_stride, out, kcache, vcache, kscale, vscale, block_table, max_blocks, q_start, \
+  if (page_size % 16 || !(d == 64 || d == 128 || d == 256) || (((uintptr_t)kscale | (uintptr_t)vscale) & 15)) return RLLM_E_UNSUPPORTED;
+  if ((long long)num_pages * nkv * (page_size >> 4) > 0x7fffffffLL) return RLLM_E_UNSUPPORTED;      // tiles of 16 rows are counted in 32 bits
+#define E4_ROWS(DD, NBB, TT)                                                                                                   \
+  return e4_rows_launch<DD, NBB, TT>(q, q_stride, out, kcache, vcache, kscale, vscale, block_table, max_blocks, q_start, \
                                           seq_lens, seq_begin, seq_end - seq_begin, max_q_len, max_keys, nq, nkv, page_size,  \
                                           num_pages, window, scale, err, stream)
   const bool one = (long long)max_q_len * (nq / nkv) <= 8;
   if (dtype == RLLM_DT_BF16) {
-    if (d == 64) { if (one) E4_ROWS(64, 1, 2, bf16); E4_ROWS(64, 2, 2, bf16); }
-    if (d == 128) { if (one) E4_ROWS(128, 1, 2, bf16); E4_ROWS(128, 2, 1, bf16); }
-    E4_ROWS(256, 1, 1, bf16);
+    if (d == 64) { if (one) E4_ROWS(64, 1, bf16); E4_ROWS(64, 2, bf16); }
+    if (d == 128) { if (one) E4_ROWS(128, 1, bf16); E4_ROWS(128, 2, bf16); }
+    E4_ROWS(256, 1, bf16);
   }
   if (dtype == RLLM_DT_F32) {
-    if (d == 64) { if (one) E4_ROWS(64, 1, 2, float); E4_ROWS(64, 2, 1, float); }
-    if (d == 128) { if (one) E4_ROWS(128, 1, 1, float); E4_ROWS(128, 2, 1, float); }
-    E4_ROWS(256, 1, 1, float);
+    if (d == 64) { if (one) E4_ROWS(64, 1, float); E4_ROWS(64, 2, float); }
+    if (d == 128) { if (one) E4_ROWS(128, 1, float); E4_ROWS(128, 2, float); }
+    E4_ROWS(256, 1, float);
   }
   return RLLM_E_BADARG;
 }
