@@ -37,7 +37,14 @@
 // without any of it.
 // Every mbarrier wait is bounded (bit 16 of the error word, then wind-down).
 // No cluster, no multicast.
+// The DENSE form reads keys and values that a kernel has widened from a cache kept in 8 bits (attention_e4m3.cu) into bfloat16
+// tiles of BN keys, [sequence][tile][kv head][BN][D], a tile a box; a mark beside a tile says whether it has keys that are NaN
+// (then no exponential goes the polynomial's way, which knows none) or that are missing (then they are masked one by one).
+// There, a cluster of CTAs may share a tile of rows, each with a part of the keys; their results are merged through
+// distributed shared memory.
 #include "attention_tcgen05.cuh"
+#include "attention_dense.h"
+#include <cooperative_groups.h>
 
 #ifndef AT_POLY
 // With heads of 64 the special-function unit bounds the kernel (1,024 cycles of ex2 a tile against 512 of MMA):
@@ -56,12 +63,15 @@ struct AtOpts {
   const bf16* gate;
   int gate_stride, gate_mode;
   const float* slopes;          // float32 [nq] or null: slopes[h] * (query position - key position) comes off the score
+  // DENSE: CTAs of a cluster, tiles of a sequence's place, and the tiles' marks [sequence][tile][kv head][AT_MARK]
+  int splits, dense_tiles;
+  const unsigned* marks;
 };
 
 // Q, two stages of K and of V, barriers: two CTAs fit one SM
 template <int AT_D> constexpr int at_smem_bytes() { return (AT_D / 64) * 16384 + 2 * AT_STAGE + 2 * AT_STAGE + 512; }
 
-template <int AT_D, bool OPT>
+template <int AT_D, bool OPT, bool DENSE>
 __global__ void __launch_bounds__(AT_THREADS, 2)
 attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                          const __grid_constant__ CUtensorMap map_v, bf16* __restrict__ out,
@@ -100,11 +110,13 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int g = nq / nkv;
   const int bq = AT_BM / g;                        // query tokens per tile
-  const int kvh = blockIdx.x % nkv;
+  const int splits = DENSE ? opt.splits : 1, rank = DENSE ? (int)blockIdx.x % splits : 0;
+  const int unit = DENSE ? (int)blockIdx.x / splits : (int)blockIdx.x;
+  const int kvh = unit % nkv;
   // which (sequence, tile): the tiles that see the most keys get the lowest block indices, for every kv head
   int s = -1, tile = 0;
   {
-    int left = blockIdx.x / nkv;
+    int left = unit / nkv;
     for (int i = seq_begin; i < seq_end; ++i) {
       const int n = (q_start[i + 1] - q_start[i] + bq - 1) / bq;
       if (left < n) { s = i; tile = n - 1 - left; break; }
@@ -125,7 +137,10 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
   };
   const int kmin = oldest(first_pos);
   const int kend = last_pos + 1;
-  const int tile_lo = kmin / AT_BN, tile_hi = (kend + AT_BN - 1) / AT_BN;
+  const int all_lo = kmin / AT_BN, all_hi = (kend + AT_BN - 1) / AT_BN;
+  const int tile_lo = DENSE ? all_lo + (all_hi - all_lo) * rank / splits : all_lo;
+  const int tile_hi = DENSE ? all_lo + (all_hi - all_lo) * (rank + 1) / splits : all_hi;
+  const int dense_lo = DENSE ? oldest(pos0) / AT_BN : 0;       // the first tile that the sequence's place holds
   // OPT: the kept first keys ahead of kmin and the key tiles ahead of tile_lo that hold them: walked first
   const int keep = (OPT && window > 0) ? opt.keep_first : 0;
   const int keep_tiles = OPT ? min((min(keep, kmin) + AT_BN - 1) / AT_BN, tile_lo) : 0;
@@ -160,7 +175,7 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
   const unsigned tmem_s = __shfl_sync(0xffffffffu, *tmem_slot, 0), tmem_o = tmem_s + AT_BN, tmem_p = tmem_o + AT_D;   // BN + D + BN / 2 <= 256 columns
 
   if (warp == 0) {
-    if (lane == 0) {
+    if (lane == 0 && (!DENSE || num_tiles > 0)) {
       mbar_expect_tx(q_full, (unsigned)(DP * bq * g * 128));     // bq * g rows of the 128 (all of them if g divides 128)
       for (int dp = 0; dp < DP; ++dp) tma_load_3d(sQ + dp * 16384, &map_q, dp * 64, kvh * g, qs + t0, q_full);
     }
@@ -175,6 +190,7 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     // is on its way while the warp polls), checked when the tile's keys are asked for, and kept in shared
     // memory until the tile's values are asked for (K runs at most three tiles ahead of V).
     auto fetch = [&](int it) {
+      if constexpr (DENSE) return (lane < boxes && it < ntiles) ? (s - seq_begin) * opt.dense_tiles + tile_at(it) - dense_lo : -2;
       const int j = tile_at(it) * AT_BN + bpage * page_size;
       return (lane < boxes && it < ntiles && j < kend) ? bt[j / page_size] : -2;      // -2: no box
     };
@@ -252,7 +268,7 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
       }
       __syncwarp();
     };
-    bool ok = wait(q_full, 0) && wait(&k_full[0], 0);
+    bool ok = (!DENSE || ntiles > 0) && wait(q_full, 0) && wait(&k_full[0], 0);
     if (ok) {
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       scores(0);
@@ -320,6 +336,12 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     bool ok = true;
     for (int it = 0; it < ntiles; ++it) {
       const int j0 = tile_at(it) * AT_BN;
+      unsigned mark = 0;
+      const unsigned* marks = nullptr;
+      if constexpr (DENSE) {
+        marks = opt.marks + ((size_t)((s - seq_begin) * opt.dense_tiles + tile_at(it) - dense_lo) * nkv + kvh) * AT_MARK;
+        mark = marks[0];
+      }
       ok = __all_sync(0xffffffffu, mbar_wait(s_full, it & 1, err));
       if (!ok) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -347,6 +369,11 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
 #pragma unroll
         for (int j = 0; j < HC; ++j)
           if (!((unsigned)j - lo_rel < span || (OPT && j < keep_rel))) sc[j] = -INFINITY;
+      }
+      if (DENSE && (mark & AT_MARK_MISSING)) {
+#pragma unroll
+        for (int j = 0; j < HC; ++j)
+          if (marks[1 + (half * HC + j) / 32] >> (j & 31) & 1u) sc[j] = -INFINITY;
       }
       float mx0 = fmaxf(sc[0], sc[1]), mx1 = fmaxf(sc[2], sc[3]), mx2 = fmaxf(sc[4], sc[5]), mx3 = fmaxf(sc[6], sc[7]);
 #pragma unroll
@@ -378,10 +405,11 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
       unsigned pk[HC / 2];
       const unsigned long long scale2 = at_pack2(sl2, sl2), shift2 = at_pack2(-m_safe, -m_safe);
       unsigned long long sum01 = at_pack2(0.f, 0.f), sum23 = sum01;
+      const bool exact = DENSE && (mark & AT_MARK_NAN);
 #pragma unroll
       for (int j = 0; j < HC; j += 4) {
         float p0, p1, p2, p3;
-        if (AT_POLY > 0 && AT_D == 64 && (j / 4) % AT_POLY == AT_POLY - 1) {
+        if (!exact && AT_POLY > 0 && AT_D == 64 && (j / 4) % AT_POLY == AT_POLY - 1) {
           at_exp2_poly2(at_fma2(at_pack2(sc[j], sc[j + 1]), scale2, shift2), p0, p1);
           at_exp2_poly2(at_fma2(at_pack2(sc[j + 2], sc[j + 3]), scale2, shift2), p2, p3);
         } else {
@@ -425,11 +453,11 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
       else tmem_st16(tmem_p + lane_sel + half * (HC / 2), pk);
       // rows of V at and behind the last visible key were never written by this sequence: whatever
       // they hold must not reach the product (0 x inf), so they are cleared before P V is issued
-      if (it == ntiles - 1) {
+      if (!DENSE && it == ntiles - 1) {
         ok = __all_sync(0xffffffffu, mbar_wait(&v_full[it & 1], (it >> 1) & 1, err));   // V has landed: nothing overwrites the zeros
         if (!ok) break;
       }
-      if (it == ntiles - 1) {
+      if (!DENSE && it == ntiles - 1) {
         if (r < AT_BN && j0 + r >= kend) {            // thread r: key row r, half a row of every panel
 #pragma unroll
           for (int dp = 0; dp < DP; ++dp) {
@@ -446,13 +474,36 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
       __syncwarp();
       if (lane == 0) mbar_arrive(p_full);
     }
+    if (DENSE && ntiles <= 0) ok = false;
     if (ok) ok = __all_sync(0xffffffffu, mbar_wait(pv_full, (ntiles - 1) & 1, err));
     // the row's sum is the two halves' sums (an exchange slot no tile is using: the pair's last
     // exchange was for tile ntiles-1, this one takes the other parity)
     float lother = 0.f;
     if (ok) ok = pair_exchange(x_mine + (ntiles & 1), x_theirs + (ntiles & 1), &xbar[quarter], ntiles, l, &lother, err);
     float lsum = half == 0 ? l + lother : lother + l;
-    if (ok) {
+    if (DENSE && splits > 1) {
+      // this CTA's part of the row, float32, where its queries, keys and values were (all of them have been read); then the
+      // row's reference and sum
+      float* mine = (float*)sQ + r * (AT_D + 4) + half * (AT_D / 2);
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll
+      for (int c0 = 0; c0 < AT_D / 2; c0 += 32) {
+        unsigned v[32];
+        if (ok) {
+          tmem_ld32(tmem_o + lane_sel + half * (AT_D / 2) + c0, v);
+          asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+        }
+#pragma unroll
+        for (int c = 0; c < 32; c += 4)
+          *(float4*)(mine + c0 + c) = ok ? make_float4(__uint_as_float(v[c]), __uint_as_float(v[c + 1]), __uint_as_float(v[c + 2]), __uint_as_float(v[c + 3]))
+                                         : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+      if (half == 0) {
+        float* ml = (float*)sQ + AT_BM * (AT_D + 4);
+        ml[r] = ok ? m_ref : -INFINITY;
+        ml[AT_BM + r] = ok ? lsum : 0.f;
+      }
+    } else if (ok) {
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       const int head = kvh * g + hl;
       float keepf = 1.f;
@@ -463,6 +514,7 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
         lsum = lsum * keepf + exp2f(sk - top);
       }
       float inv = lsum > 0.f ? keepf / lsum : 0.f;
+      if (DENSE && lsum != lsum) inv = lsum;           // a key that is NaN
       const size_t tok = (size_t)(qs + t0 + (live ? tl : 0));
       const bf16* grow = (OPT && opt.gate_mode) ? opt.gate + tok * opt.gate_stride : nullptr;
       // sigmoid(x) = 1 / (1 + 2^(-x log2 e))
@@ -512,10 +564,38 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     pdl_wait();
     pdl_launch();
   }
+  if constexpr (DENSE) {
+    if (splits > 1) {
+      namespace cg = cooperative_groups;
+      cg::cluster_group cluster = cg::this_cluster();
+      cluster.sync();
+      float* part = (float*)sQ;
+      float* ml = part + AT_BM * (AT_D + 4);
+      const int first = AT_BM * rank / splits, last = AT_BM * (rank + 1) / splits;     // this CTA's rows
+      for (int i = threadIdx.x; i < (last - first) * (AT_D / 4); i += AT_THREADS) {
+        const int row = first + i / (AT_D / 4), c = (i % (AT_D / 4)) * 4, tok = row / g;
+        if (tok >= ntok) break;                        // rows behind: none of them is live
+        float top = -INFINITY, sum = 0.f;
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int k = 0; k < splits; ++k) top = fmaxf(top, cluster.map_shared_rank(ml, k)[row]);
+        for (int k = 0; k < splits; ++k) {
+          const float* other = cluster.map_shared_rank(ml, k);
+          const float f = other[row] == -INFINITY ? 1.0f : at_ex2(other[row] - top);     // (with nothing seen, zeros or NaN)
+          const float4 y = *(const float4*)(cluster.map_shared_rank(part, k) + row * (AT_D + 4) + c);
+          x.x = fmaf(y.x, f, x.x); x.y = fmaf(y.y, f, x.y); x.z = fmaf(y.z, f, x.z); x.w = fmaf(y.w, f, x.w);
+          sum = fmaf(other[AT_BM + row], f, sum);
+        }
+        const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+        const __nv_bfloat162 lo = __floats2bfloat162_rn(x.x * inv, x.y * inv), hi = __floats2bfloat162_rn(x.z * inv, x.w * inv);
+        *(uint2*)(out + ((size_t)(qs + t0 + tok) * nq + kvh * g + row - tok * g) * AT_D + c) = make_uint2(*(const unsigned*)&lo, *(const unsigned*)&hi);
+      }
+      cluster.sync();                                  // nobody leaves while its shared memory is being read
+    }
+  }
 }
 
 // ---------------------------------------------------------------------------
-template <int D, bool OPT>
+template <int D, bool OPT, bool DENSE = false>
 static int at_launch(const void* q, int q_stride, int num_q_rows, void* out, const void* kcache, const void* vcache,
                      const int* block_table, int max_blocks, const int* q_start, const int* seq_lens, int seq_begin,
                      int seq_end, int num_tokens, int nq, int nkv, int page_size, int num_pages, int window,
@@ -540,12 +620,39 @@ static int at_launch(const void* q, int q_stride, int num_q_rows, void* out, con
     if (rc) return rc;
   }
   static SmemLimit limit;
-  if (const int e = limit.allow(attention_tcgen05_kernel<D, OPT>, at_smem_bytes<D>())) return e;
+  if (const int e = limit.allow(attention_tcgen05_kernel<D, OPT, DENSE>, at_smem_bytes<D>())) return e;
   const int bq = AT_BM / g;
   const long long tiles = (num_tokens + bq - 1) / bq + (seq_end - seq_begin);
+  if constexpr (DENSE) {
+    // CTAs that share a tile of rows: to fill two places an SM, with four tiles of keys each at least
+    const long long units = tiles * nkv;
+    int splits = 1;
+    while (splits < 8 && units * splits * 2 <= 296 && splits * 2 * 4 <= opt.dense_tiles) splits *= 2;
+    opt.splits = splits;
+    if (units * splits > 0x7fffffffLL) return RLLM_E_UNSUPPORTED;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(units * splits));
+    cfg.blockDim = dim3(AT_THREADS);
+    cfg.dynamicSmemBytes = (size_t)at_smem_bytes<D>();
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)splits;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = rllm_pdl_enabled() ? 2 : 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, attention_tcgen05_kernel<D, OPT, DENSE>, mq, mk, mv, (bf16*)out, block_table, max_blocks,
+                                             q_start, seq_lens, seq_begin, seq_end, nq, nkv, page_size, num_pages, window,
+                                             scale * 1.4426950408889634f, err, opt, beside);
+    if (e != cudaSuccess) { cudaGetLastError(); return (int)e; }
+    return 0;
+  }
   if (tiles * nkv > 0x7fffffffLL) return RLLM_E_UNSUPPORTED;
   dim3 grid((unsigned)(tiles * nkv));
-  rllm_launch_pdl(attention_tcgen05_kernel<D, OPT>, grid, dim3(AT_THREADS), (size_t)at_smem_bytes<D>(), stream, mq, mk, mv, (bf16*)out,
+  rllm_launch_pdl(attention_tcgen05_kernel<D, OPT, DENSE>, grid, dim3(AT_THREADS), (size_t)at_smem_bytes<D>(), stream, mq, mk, mv, (bf16*)out,
                   block_table, max_blocks, q_start, seq_lens, seq_begin, seq_end, nq, nkv, page_size, num_pages, window,
                   scale * 1.4426950408889634f, err, opt, beside);
   RLLM_LAUNCH_CHECK();
@@ -604,4 +711,27 @@ RLLM_EXPORT int rllm_attention_prefill_tcgen05_opts(const void* q, int q_stride,
   return at_prefill<true>(q, q_stride, num_q_rows, out, kcache, vcache, block_table, max_blocks, q_start, seq_lens,
                           seq_begin, seq_end, num_tokens, nq, nkv, d, page_size, num_pages, window, scale, err, stream,
                           AtOpts{keep_first, chunk, softcap, sinks, (const bf16*)gate, gate_stride, gate_mode, slopes});
+}
+
+// The DENSE form: kdense, vdense [num_seqs][dense_tiles][nkv][8192 / d][d] and their marks, of sequences seq_begin ..
+// seq_begin + num_seqs - 1 (each from the tile of its portion's oldest visible key on).
+RLLM_EXPORT int rllm_attention_dense_tcgen05(const void* q, int q_stride, int num_q_rows, void* out, const void* kdense,
+                                             const void* vdense, const void* marks, int dense_tiles, const int* q_start,
+                                             const int* seq_lens, int seq_begin, int num_seqs, int num_tokens, int nq, int nkv,
+                                             int d, int window, float scale, int* err, cudaStream_t stream) {
+  if (num_seqs <= 0 || num_tokens <= 0) return 0;
+  if (!q || !out || !kdense || !vdense || !marks || !q_start || !seq_lens || nq <= 0 || nkv <= 0 || nq % nkv || dense_tiles <= 0 ||
+      seq_begin < 0 || window < 0 || !(scale > 0.f) || !err)
+    return RLLM_E_BADARG;
+  const int g = nq / nkv;
+  if (!(d == 64 || d == 128) || g > AT_BM || q_stride % 8 || (((uintptr_t)q | (uintptr_t)out | (uintptr_t)kdense | (uintptr_t)vdense) & 15))
+    return RLLM_E_UNSUPPORTED;
+  const int bn = 8192 / d;
+  const long long pages = (long long)num_seqs * dense_tiles;
+  if (pages * nkv * bn > 0x7fffffffLL) return RLLM_E_UNSUPPORTED;      // rows are TMA coordinates
+  AtOpts opt{0, 0, 0.f, nullptr, nullptr, 0, 0, nullptr, 1, dense_tiles, (const unsigned*)marks};
+#define AT_DENSE(DD) return (at_launch<DD, false, true>(q, q_stride, num_q_rows, out, kdense, vdense, nullptr, 0, q_start, seq_lens, seq_begin, \
+      seq_begin + num_seqs, num_tokens, nq, nkv, bn, (int)pages, window, scale, err, stream, opt, 0))
+  if (d == 64) AT_DENSE(64);
+  AT_DENSE(128);
 }

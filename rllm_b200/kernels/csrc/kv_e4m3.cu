@@ -1,5 +1,6 @@
 // Writing a cache that is kept in 8 bits, and reading it back (see kv_e4m3.cuh for what a row becomes).
 #include "kv_e4m3.cuh"
+#include "attention_dense.h"
 
 // ---------------------------------------------------------------------------
 // write: rotation of q, rotation and quantisation of k, quantisation of v
@@ -174,6 +175,107 @@ RLLM_EXPORT int rllm_kv_e4m3_read(const int* positions, const int* token_seq, co
                     max_blocks, num_seqs, (const unsigned char*)kcache, (const unsigned char*)vcache,
                     (const unsigned char*)kscale, (const unsigned char*)vscale, (T_*)out_k, (T_*)out_v, T, nkv, d, page_size,
                     num_pages, err));
+  RLLM_LAUNCH_CHECK();
+  return 0;
+}
+
+// ---------------------------------------------------------------------------
+// widen: what the prompt attention on tcgen05 reads of a step's sequences, as dense bfloat16 tiles
+// ---------------------------------------------------------------------------
+// A tile of the attention is BN = 8192 / D keys; one block widens the keys and values of a (tile, kv head, sequence), once for
+// all the tiles of rows that read it (widened inside the attention they would be so by every CTA: 32 times for 1,024 tokens
+// and 4 heads a kv head).  The values are exact (kv_e4m3.cuh), but for the rows that are NaN: such a token's key is NaN and its
+// value 0, so that the product with the probabilities stays clean for the rows that do not see it, and those that do are NaN by
+// its score.  Rows behind the sequence's end, and of pages that are not held, are zeros.
+template <int D>
+__global__ void __launch_bounds__(128)
+kv_e4m3_widen_kernel(const int* __restrict__ block_table, int max_blocks, const int* __restrict__ q_start,
+                     const int* __restrict__ seq_lens, int seq_begin, const unsigned char* __restrict__ kcache,
+                     const unsigned char* __restrict__ vcache, const unsigned char* __restrict__ kscale,
+                     const unsigned char* __restrict__ vscale, bf16* __restrict__ kdense, bf16* __restrict__ vdense,
+                     unsigned* __restrict__ marks, int nkv, int page_size, int num_pages, int window, int* __restrict__ err) {
+  constexpr int BN = 8192 / D, PIECES = D / 16, STEPS = BN * PIECES / 128;
+  __shared__ unsigned mark[AT_MARK];
+  const int page_shift = (page_size & (page_size - 1)) == 0 ? __ffs(page_size) - 1 : -1;
+  const int s = seq_begin + blockIdx.z, kvh = blockIdx.y;
+  const int len = seq_lens[s], pos0 = len - (q_start[s + 1] - q_start[s]);
+  const int lo = window > 0 ? max(0, pos0 - window + 1) : 0, tile = lo / BN + blockIdx.x;
+  if (threadIdx.x < AT_MARK) mark[threadIdx.x] = 0u;
+  __syncthreads();
+  const bool empty = tile * BN >= len;             // (nothing reads it)
+  long long row[STEPS];
+#pragma unroll
+  for (int i = 0; i < STEPS; ++i) {
+    const int r = (threadIdx.x + i * 128) / PIECES, j = tile * BN + r;
+    row[i] = -1;
+    if (!empty && j >= lo && j < len) {
+      const int at = page_shift >= 0 ? j >> page_shift : j / page_size;
+      const int page = at < max_blocks ? block_table[(size_t)s * max_blocks + at] : -1;
+      if (page >= 0 && page < num_pages) {
+        row[i] = ((long long)page * nkv + kvh) * page_size + (j - at * page_size);
+      } else if (threadIdx.x % PIECES == 0) {
+        atomicOr(err, 4);
+        atomicOr(&mark[1 + r / 32], 1u << (r & 31));
+        atomicOr(&mark[0], AT_MARK_MISSING);
+      }
+    }
+  }
+  pdl_wait_on(kcache, vcache, kscale, vscale, kdense, vdense, marks);
+  pdl_launch();
+  if (empty) return;                               // (the whole block)
+  const int c = (threadIdx.x % PIECES) * 16;
+  uint4 kx[STEPS], vx[STEPS];
+  int kb[STEPS], vb[STEPS];
+#pragma unroll
+  for (int i = 0; i < STEPS; ++i) {
+    const bool held = row[i] >= 0;
+    kx[i] = held ? *(const uint4*)(kcache + row[i] * D + c) : make_uint4(0u, 0u, 0u, 0u);
+    vx[i] = held ? *(const uint4*)(vcache + row[i] * D + c) : make_uint4(0u, 0u, 0u, 0u);
+    kb[i] = held ? kscale[row[i]] : 0;
+    vb[i] = held ? vscale[row[i]] : 0;
+  }
+  const size_t base = (((size_t)blockIdx.z * gridDim.x + blockIdx.x) * nkv + kvh) * BN * D;
+#pragma unroll
+  for (int i = 0; i < STEPS; ++i) {
+    const bool odd = kb[i] == KV8_NAN_SCALE || vb[i] == KV8_NAN_SCALE;
+    if (odd) atomicOr(&mark[0], AT_MARK_NAN);
+    const size_t at = base + (size_t)(threadIdx.x + i * 128) * 16;
+#pragma unroll
+    for (int v = 0; v < 2; ++v) {
+      const uint4 raw = v ? vx[i] : kx[i];
+      const float power = odd ? 0.f : kv8_power(v ? vb[i] : kb[i]), more = odd && !v ? __uint_as_float(0x7FC00000u) : 0.f;
+      float x[16];
+      kv8_floats(raw.x, x); kv8_floats(raw.y, x + 4); kv8_floats(raw.z, x + 8); kv8_floats(raw.w, x + 12);
+      float a[8], b[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) { a[k] = fmaf(x[k], power, more); b[k] = fmaf(x[k + 8], power, more); }
+      bf16* dst = (v ? vdense : kdense) + at;
+      store8(dst, a);
+      store8(dst + 8, b);
+    }
+  }
+  __syncthreads();
+  if (threadIdx.x < AT_MARK) marks[(((size_t)blockIdx.z * gridDim.x + blockIdx.x) * nkv + kvh) * AT_MARK + threadIdx.x] = mark[threadIdx.x];
+}
+
+// Sequences seq_begin .. seq_begin + num_seqs - 1, each from the tile of its portion's oldest visible key on, dense_tiles
+// tiles at most: kdense, vdense [num_seqs][dense_tiles][nkv][8192 / d][d], marks [num_seqs][dense_tiles][nkv][AT_MARK].
+RLLM_EXPORT int rllm_kv_e4m3_widen(const int* block_table, int max_blocks, const int* q_start, const int* seq_lens, int seq_begin,
+                                   int num_seqs, int dense_tiles, const void* kcache, const void* vcache, const void* kscale,
+                                   const void* vscale, void* kdense, void* vdense, void* marks, int nkv, int d, int page_size,
+                                   int num_pages, int window, int* err, cudaStream_t stream) {
+  if (num_seqs <= 0) return 0;
+  if (!block_table || !q_start || !seq_lens || !kcache || !vcache || !kscale || !vscale || !kdense || !vdense || !marks || !err ||
+      seq_begin < 0 || dense_tiles <= 0 || nkv <= 0 || page_size <= 0 || num_pages <= 0 || max_blocks <= 0 || window < 0)
+    return RLLM_E_BADARG;
+  if (!(d == 64 || d == 128) || nkv > 65535 || num_seqs > 65535 ||
+      (((uintptr_t)kcache | (uintptr_t)vcache | (uintptr_t)kdense | (uintptr_t)vdense) & 15))
+    return RLLM_E_UNSUPPORTED;
+#define KV8_WIDEN(DD) rllm_launch_pdl(kv_e4m3_widen_kernel<DD>, dim3(dense_tiles, nkv, num_seqs), dim3(128), (size_t)0, stream, block_table, \
+      max_blocks, q_start, seq_lens, seq_begin, (const unsigned char*)kcache, (const unsigned char*)vcache, (const unsigned char*)kscale,  \
+      (const unsigned char*)vscale, (bf16*)kdense, (bf16*)vdense, (unsigned*)marks, nkv, page_size, num_pages, window, err)
+  if (d == 64) KV8_WIDEN(64);
+  else KV8_WIDEN(128);
   RLLM_LAUNCH_CHECK();
   return 0;
 }

@@ -62,6 +62,8 @@ def _check(code: int, what: str) -> None:
 _TABLE = {
     "rllm_kv_e4m3_write": ("kv_e4m3", "piplpppipiippppiiiiiip", "rope_kv_write_e4m3"),
     "rllm_kv_e4m3_read": ("kv_e4m3", "pppiippppppiiiiiip", "kv_read_e4m3"),
+    "rllm_kv_e4m3_widen": ("kv_e4m3", "pippiiipppppppiiiiip", "attention_e4m3"),
+    "rllm_attention_dense_tcgen05": ("attention_tcgen05", "piippppippiiiiiiifp", "attention_e4m3"),
     "rllm_attention_e4m3_rows": ("attention_e4m3", "pipppppipippiiiiiiiiiifp", "attention_e4m3"),
     "rllm_attention_e4m3_simt": ("attention_e4m3", "pipppppipippiiiiiiiiifp", "attention_e4m3"),
     "rllm_softcap": ("elementwise", "plf", "softcap_rows"),
@@ -2140,6 +2142,20 @@ def kv_read_e4m3(positions: torch.Tensor, token_seq: torch.Tensor, block_table: 
                                kcache.shape[0], err)
 
 
+E4M3_DENSE_SCRATCH = 512 << 20      # bytes of widened keys and values at a time; more only where one sequence needs more
+
+
+def attention_e4m3_dense_takes(dtype: torch.dtype, nq: int, nkv: int, d: int, scale: float) -> bool:
+    """The sizes of the prompt attention on tcgen05 over widened keys and values."""
+    return dtype is torch.bfloat16 and d in (64, 128) and nq // nkv <= 128 and scale > 0 and \
+        os.environ.get("RLLM_ATTENTION") not in ("simt", "mma")
+
+
+def attention_e4m3_dense_pays(max_q_len: int, nq: int, nkv: int) -> bool:
+    """Whether sequences of up to so many tokens are faster that way than a tile of 16 rows at a time."""
+    return max_q_len * (nq // nkv) >= 64
+
+
 def attention_e4m3(q: torch.Tensor, out: torch.Tensor, kcache: torch.Tensor, vcache: torch.Tensor, kscale: torch.Tensor,
                    vscale: torch.Tensor, block_table: torch.Tensor, q_start: torch.Tensor, seq_lens: torch.Tensor,
                    num_decode: int, max_q_len: int, max_seq_len: int, nq: int, nkv: int, window: int, scale: float,
@@ -2176,5 +2192,22 @@ def attention_e4m3(q: torch.Tensor, out: torch.Tensor, kcache: torch.Tensor, vca
     keys = max_seq_len if window <= 0 else min(max_seq_len, window + max_q_len)
     if num_decode:
         _entries.rllm_attention_e4m3_rows(q, q.stride(0), out, *cache, 0, num_decode, 1, keys, *heads)
-    if num_decode < S:
-        _entries.rllm_attention_e4m3_rows(q, q.stride(0), out, *cache, num_decode, S, max_q_len, keys, *heads)
+    if num_decode == S:
+        return
+    if attention_e4m3_dense_takes(q.dtype, nq, nkv, d, scale) and attention_e4m3_dense_pays(max_q_len, nq, nkv) and \
+            q.stride(0) % 8 == 0 and q.data_ptr() % 16 == 0:
+        bn = 8192 // d
+        tiles = keys // bn + 2
+        a_sequence = 2 * tiles * nkv * bn * d
+        group = max(1, min(S - num_decode, E4M3_DENSE_SCRATCH // (2 * a_sequence), 65535))
+        dense = torch.empty((2, group * a_sequence // 2), dtype=torch.bfloat16, device=q.device)
+        marks = torch.empty(group * tiles * nkv * 8, dtype=torch.int32, device=q.device)
+        for first in range(num_decode, S, group):
+            n = min(group, S - first)
+            _entries.rllm_kv_e4m3_widen(block_table, block_table.shape[1], q_start, seq_lens, first, n, tiles, kcache, vcache,
+                                        kscale, vscale, dense[0], dense[1], marks, nkv, d, kcache.shape[2], kcache.shape[0],
+                                        window, err)
+            _entries.rllm_attention_dense_tcgen05(q, q.stride(0), q.shape[0], out, dense[0], dense[1], marks, tiles, q_start,
+                                                  seq_lens, first, n, min(T, n * max_q_len), nq, nkv, d, window, scale, err)
+        return
+    _entries.rllm_attention_e4m3_rows(q, q.stride(0), out, *cache, num_decode, S, max_q_len, keys, *heads)
