@@ -568,7 +568,7 @@ BIKOVIK_SIZES = {
 STEP_KERNELS = (
     "latent_attention_mma", "latent_attention_tcgen05", "latent_expanded_tcgen05", "latent_expand_prep",
     "attention_prefill_tcgen05", "attention_prefill_bf16",
-    "attention_decode_bf16", "moe_experts", "moe_route", "head_gemm", "mingru_scan", "gated_postnorm_add",
+    "attention_decode_bf16", "attention_e4m3", "rope_kv_write_e4m3", "moe_experts", "moe_route", "head_gemm", "mingru_scan", "gated_postnorm_add",
     "depth_average", "rmsnorm", "silu_mul", "latent_prep", "latent_q_rot", "rope_kv_write", "gemm_small_m",
     "moe_choose", "gemm_small_m_residual", "gemm_small_m_rstd", "gemm_tcgen05", "embedding", "lightning_scan",
     "selective_scan", "causal_conv", "streams_read", "streams_write", "head_norm_kv_write", "attention_simt_kv",

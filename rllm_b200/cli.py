@@ -22,6 +22,8 @@ import sys
 import time
 from typing import List
 
+from .config.engine_args import KV_CACHE_DTYPES
+
 
 def _gpu_util(s: str) -> float:
     v = float(s)
@@ -80,6 +82,8 @@ def build_parser() -> argparse.ArgumentParser:
     g.add_argument("--step-row-multiple", type=int, default=128,
                    help="a step that ends up to a quarter of this many rows over a multiple of it gives them back (0: off)")
     g.add_argument("--block-size", type=int, default=16)
+    g.add_argument("--kv-cache-dtype", choices=list(KV_CACHE_DTYPES), default="auto",
+                   help="keys and values in the run's type (auto), or in 8 bits with a power of two a row (fp8, fp8_e4m3)")
     g.add_argument("--num-gpu-blocks", type=int, default=None)
     g.add_argument("--random-weights", action="store_true",
                    help="draw weights from --weights-seed; the folder needs config.json only")
@@ -137,7 +141,7 @@ def cmd_generate(args) -> int:
               enable_prefix_caching=args.enable_prefix_caching, block_size=args.block_size,
               num_gpu_blocks=args.num_gpu_blocks,
               long_prefill_token_threshold=args.long_prefill_token_threshold,
-              step_row_multiple=args.step_row_multiple, scheduling_policy=args.scheduling_policy,
+              step_row_multiple=args.step_row_multiple, scheduling_policy=args.scheduling_policy, kv_cache_dtype=args.kv_cache_dtype,
               random_weights=args.random_weights, seed=args.weights_seed)
     params = [SamplingParams(temperature=args.temperature, top_k=args.top_k, top_p=args.top_p,
                              min_p=args.min_p, repetition_penalty=args.repetition_penalty,

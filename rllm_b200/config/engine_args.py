@@ -8,7 +8,8 @@
 ``enable_chunked_prefill`` are fields of the reference's ``CacheConfig`` and
 ``SchedulerConfig`` (crates/rllm-core/src/config.rs:67-77, 92-101); the server
 fixes the block size at 16 (crates/rllm-server/src/server.rs:34) and the
-threshold at 2048 (:330).
+threshold at 2048 (:330).  ``kv_cache_dtype`` has the name and the fp8 meaning of the reference's ``--kv-cache-dtype``; its
+e4m3 numbers have a scale a row of their own here.
 """
 from __future__ import annotations
 
@@ -16,6 +17,8 @@ from dataclasses import dataclass
 from typing import Optional
 
 from .model_config import ConfigError, normalize_dtype_name
+
+KV_CACHE_DTYPES = ("auto", "fp8", "fp8_e4m3")
 
 
 @dataclass
@@ -34,6 +37,7 @@ class EngineArgs:
     step_row_multiple: int = 128         # this engine's own: see Scheduler._trim_to_row_multiple; 0 = off
     scheduling_policy: str = "fcfs"      # or "priority" (crates/rllm-core/src/config.rs:86-98)
     seed: int = 0
+    kv_cache_dtype: str = "auto"         # keys and values in the run's type, or "fp8_e4m3" ("fp8"): in 8 bits with a power of two a row
 
     def validate(self) -> None:
         if not 0.01 <= self.gpu_memory_utilization <= 1.0:
@@ -55,7 +59,13 @@ class EngineArgs:
             raise ConfigError("step_row_multiple must be >= 0")
         if self.scheduling_policy not in ("fcfs", "priority"):
             raise ConfigError(f"scheduling_policy must be fcfs or priority, got {self.scheduling_policy!r}")
+        if self.kv_cache_dtype not in KV_CACHE_DTYPES:
+            raise ConfigError(f"kv_cache_dtype must be one of {', '.join(KV_CACHE_DTYPES)}, got {self.kv_cache_dtype!r}")
         normalize_dtype_name(self.dtype)
+
+    @property
+    def cache_in_8_bits(self) -> bool:
+        return self.kv_cache_dtype in ("fp8", "fp8_e4m3")
 
     def run_dtype(self, model_dtype: str) -> str:
         """The dtype the engine computes in: ``auto`` follows config.json's

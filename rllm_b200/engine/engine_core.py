@@ -80,7 +80,7 @@ def plan_cache_pages(model: DecoderModel, args: EngineArgs, max_model_len: int, 
     ``gpu_memory_utilization`` of the device leaves beside the weights and a reserve for activations
     is shared so that every group gets the same fraction of what it can use."""
     bs = args.block_size
-    elem = 2 if model.dtype is torch.bfloat16 else 4
+    elem, scale = (1, 1) if args.cache_in_8_bits else (2 if model.dtype is torch.bfloat16 else 4, 0)
     portion = args.max_num_batched_tokens
     if args.long_prefill_token_threshold > 0:
         portion = min(portion, args.long_prefill_token_threshold)
@@ -92,7 +92,7 @@ def plan_cache_pages(model: DecoderModel, args: EngineArgs, max_model_len: int, 
         per_request = full if need.span is None else \
             min(full, -(-(need.span + portion) // bs) + 1 + -(-need.keep_first // bs))
         useful.append(args.max_num_seqs * per_request)
-        nbytes.append(page_bytes(need, bs, elem) * len(model.layout.owners[g]))
+        nbytes.append(page_bytes(need, bs, elem, scale) * len(model.layout.owners[g]))
     if not useful:
         return []
     if args.num_gpu_blocks is not None:
@@ -103,7 +103,10 @@ def plan_cache_pages(model: DecoderModel, args: EngineArgs, max_model_len: int, 
     spec = model.spec
     act = args.max_num_batched_tokens * (spec.hidden_size * 16 + 64 * 1024) + \
         min(args.max_num_seqs, args.max_num_batched_tokens) * spec.vocab_size * 8 + (1 << 30)
-    act += model.step_scratch() if hasattr(model, "step_scratch") else 0
+    if args.cache_in_8_bits:
+        act += model.step_scratch_8_bit(max_model_len)
+    else:
+        act += model.step_scratch() if hasattr(model, "step_scratch") else 0
     budget = int(total * args.gpu_memory_utilization) - (total - free) - act
     if budget < 4 * sum(nbytes):
         raise RuntimeError(f"no room for a KV cache: {free >> 20} MiB free of {total >> 20} MiB with "
@@ -144,12 +147,14 @@ class EngineCore:
         self.device = model.device
         spec = model.spec
         self.max_model_len = min(self.args.max_model_len or spec.max_positions, spec.max_positions)
+        if self.args.cache_in_8_bits:
+            model.check_8_bit_cache()
         pages = plan_cache_pages(model, self.args, self.max_model_len, self.device)
         self.num_pages = list(pages)
         self.cache = CacheManager(model.layout.groups, self.args.block_size, pages,
                                   self.args.max_num_seqs, self.args.enable_prefix_caching)
         self.storage = CacheStorage(model.layout, self.args.block_size, pages,
-                                    self.args.max_num_seqs, model.dtype, self.device)
+                                    self.args.max_num_seqs, model.dtype, self.device, self.args.cache_in_8_bits)
         self.runner = ModelRunner(model, self.cache, self.storage, self.args.enable_cuda_graphs)
         self.sampler = Sampler(self.device)
         self.scheduler = Scheduler(SchedulerConfig(

@@ -35,6 +35,8 @@ import os
 import sys
 from typing import Dict, List
 
+from ..config.engine_args import KV_CACHE_DTYPES, EngineArgs
+
 PAGE_SIZE = 16
 
 
@@ -48,6 +50,8 @@ def build_parser() -> argparse.ArgumentParser:
     p.add_argument("--block-size", type=int, default=PAGE_SIZE, help="tokens per cache page")
     p.add_argument("--max-live", type=int, default=4,
                    help="most requests that are live at a time (state slots of the cache manager)")
+    p.add_argument("--kv-cache-dtype", choices=list(KV_CACHE_DTYPES), default="auto",
+                   help="keys and values in the run's type (auto), or in 8 bits with a power of two a row (fp8, fp8_e4m3)")
     p.add_argument("--device", default="cuda:0")
     return p
 
@@ -62,17 +66,19 @@ class TraceSession:
     generation uses.  ``step`` takes one record of the trace and returns the logits
     at the wanted places (float32 [wanted, vocab] on the device)."""
 
-    def __init__(self, model, max_tokens: int, block_size: int = PAGE_SIZE, max_live: int = 8):
+    def __init__(self, model, max_tokens: int, block_size: int = PAGE_SIZE, max_live: int = 8, e4m3: bool = False):
         from ..cache import CacheManager, CacheStorage
         from .runner import ModelRunner
         self.model = model
+        if e4m3:
+            model.check_8_bit_cache()
         page = int(block_size)
         num_pages = max(1, -(-int(max_tokens) // page))
         paged = [n for n in model.layout.groups if hasattr(n, "num_kv_heads")]
         self.max_tokens, self.max_live = int(max_tokens), max(1, int(max_live))
         self.cache = CacheManager(model.layout.groups, page, [num_pages] * len(paged), self.max_live)
         self.storage = CacheStorage(model.layout, page, [num_pages] * len(paged), self.max_live, model.dtype,
-                                    model.device)
+                                    model.device, e4m3)
         self.runner = ModelRunner(model, self.cache, self.storage)
         self.fed: Dict[str, int] = {}
 
@@ -128,7 +134,8 @@ def main(argv=None) -> int:
 
     os.makedirs(args.out, exist_ok=True)
     _, model = load_model(args.model, dtype=args.dtype, device=args.device)
-    session = TraceSession(model, args.max_tokens, args.block_size, args.max_live)
+    session = TraceSession(model, args.max_tokens, args.block_size, args.max_live,
+                           EngineArgs(kv_cache_dtype=args.kv_cache_dtype).cache_in_8_bits)
     for line in sys.stdin:
         line = line.strip()
         if not line:

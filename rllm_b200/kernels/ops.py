@@ -2145,6 +2145,14 @@ def kv_read_e4m3(positions: torch.Tensor, token_seq: torch.Tensor, block_table: 
 E4M3_DENSE_SCRATCH = 512 << 20      # bytes of widened keys and values at a time; more only where one sequence needs more
 
 
+def e4m3_dense_scratch(nkv: int, d: int, max_seq_len: int) -> int:
+    """The most bytes that ``attention_e4m3`` takes for a while for prompt portions of sequences of up to so many tokens."""
+    if d not in (64, 128):
+        return 0
+    bn = 8192 // d
+    return max(E4M3_DENSE_SCRATCH, 4 * (max_seq_len // bn + 2) * nkv * bn * d)
+
+
 def attention_e4m3_dense_takes(dtype: torch.dtype, nq: int, nkv: int, d: int, scale: float) -> bool:
     """The sizes of the prompt attention on tcgen05 over widened keys and values."""
     return dtype is torch.bfloat16 and d in (64, 128) and nq // nkv <= 128 and scale > 0 and \

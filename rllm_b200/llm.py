@@ -28,7 +28,7 @@ class LLM:
                  long_prefill_token_threshold: int = 2048, enable_chunked_prefill: bool = True,
                  enable_cuda_graphs: bool = True, random_weights: bool = False, seed: int = 0,
                  device: Optional[str] = None, draw_on_device: bool = False, step_row_multiple: int = 128,
-                 scheduling_policy: str = "fcfs"):
+                 scheduling_policy: str = "fcfs", kv_cache_dtype: str = "auto"):
         self.args = EngineArgs(dtype=dtype, max_model_len=max_model_len, max_num_seqs=max_num_seqs,
                                max_num_batched_tokens=max_num_batched_tokens,
                                gpu_memory_utilization=gpu_memory_utilization,
@@ -37,7 +37,8 @@ class LLM:
                                long_prefill_token_threshold=long_prefill_token_threshold,
                                enable_chunked_prefill=enable_chunked_prefill,
                                enable_cuda_graphs=enable_cuda_graphs, seed=seed,
-                               step_row_multiple=step_row_multiple, scheduling_policy=scheduling_policy)
+                               step_row_multiple=step_row_multiple, scheduling_policy=scheduling_policy,
+                               kv_cache_dtype=kv_cache_dtype)
         self.args.validate()
         self.config, self.model = load_model(model, dtype=dtype, device=device,
                                              random_weights=random_weights, seed=seed,

@@ -18,6 +18,7 @@ from typing import Dict, List, Optional, Sequence, Tuple
 
 import torch
 
+from ..config.model_config import ConfigError
 from ..parts import registry as part_registry
 from ..parts.base import KVCacheView, PendingSum, StateCacheView, StepContext
 from ..parts.embedding import OutputHead, TokenEmbedding
@@ -102,7 +103,25 @@ class DecoderModel:
         """Bytes that a step may take by what the cache holds; layers run one after the other."""
         return max((b.mixer.step_scratch() for b in self.blocks), default=0)
 
+    def step_scratch_8_bit(self, max_model_len: int) -> int:
+        return max((b.mixer.step_scratch_8_bit(max_model_len) for b in self.blocks), default=0)
+
     # -- cache ------------------------------------------------------------
+    def check_8_bit_cache(self) -> None:
+        """Raise a ConfigError unless every layer that keeps pages can keep them in 8 bits."""
+        paged = False
+        for i, run in enumerate(self.spec.order):
+            g = self.layout.run_group[i]
+            groups = g if isinstance(g, tuple) else () if g is None else (g,)
+            if not any(isinstance(self.layout.groups[x], KVPagesNeed) for x in groups):
+                continue
+            paged = True
+            why = self.blocks[run.layer].mixer.no_8_bit_cache()
+            if why is not None:
+                raise ConfigError(f"kv_cache_dtype fp8_e4m3: layer {run.layer}: {why}")
+        if not paged:
+            raise ConfigError("kv_cache_dtype fp8_e4m3: no layer of the model keeps keys and values")
+
     def _cache_layout(self) -> CacheLayout:
         groups: List[object] = []
         owners: List[list] = []

@@ -51,6 +51,10 @@ With ``head_mix`` the mixture is moved to the queries: a token's keys of all kv 
 reads, q'_h = [sum over the heads g of kv head 0 of talk[h, g] q_g | ... | of the last kv head], and q'_h . row is the
 mixed score (``kernels/csrc/talking_heads.cu``); the pages keep that row and the values of all kv heads side by side.
 
+Where the engine keeps its cache in 8 bits (``KVCacheView.k_scale``), the Llama's form goes through the kernels of
+``kernels/csrc/kv_e4m3.cu`` and ``attention_e4m3.cu``: one writes the tokens' rows, the attention reads them back from there.  The
+other options have no such form (``no_8_bit_cache``).
+
 A position part that rotates pairs (2i, 2i + 1) is served by the same kernels, which rotate halves: the rows of
 W_q, W_k, their biases and norm weights are put into the part's ``half_order`` when they are loaded.
 
@@ -295,6 +299,14 @@ class PagedAttention(Mixer):
         return KVPagesNeed(self.nkv, self.d, self.window, v_dim=None if self.dv == self.d else self.dv,
                            keep_first=self.keep_first, chunk=self.chunk or None)
 
+    def no_8_bit_cache(self) -> Optional[str]:
+        if not self.plain:
+            return "attention with head norms, biases, value heads of their own size or other options keeps its pages in the run's type"
+        return None
+
+    def step_scratch_8_bit(self, max_model_len: int) -> int:
+        return max(self.step_scratch(), ops.e4m3_dense_scratch(self.nkv, self.d, max_model_len))
+
     # -- compute ----------------------------------------------------------
     def fused_residual(self, num_rows: int, dtype: torch.dtype) -> bool:
         # talking heads: the output product of a decode step can carry the residual add and the next norm
@@ -425,6 +437,7 @@ class PagedAttention(Mixer):
         x = qkv
         T = qkv.shape[0]
         nkv_here = 0 if self.shares_kv else self.nkv
+        in_8_bits = cache.k_scale is not None
         table = ctx.block_tables[cache.group]
         fused = self.position.fused_rotary(x.device)
         writes = cache.writes and not self.shares_kv
@@ -436,6 +449,18 @@ class PagedAttention(Mixer):
             fused = (None, 0)
         inv_freq, rd = fused
         out = torch.empty((T, self.nq * self.d), dtype=x.dtype, device=x.device)
+        if in_8_bits:
+            # one kernel rotates the queries in place and writes the tokens' keys and values; everything is read from the pages
+            pages = (cache.k, cache.v, cache.k_scale, cache.v_scale)
+            if writes:
+                ops.rope_kv_write_e4m3(qkv, ctx.positions, ctx.token_seq, inv_freq, rd, table, *pages, self.nq, self.nkv,
+                                       self.d, ctx.err)
+            elif rd:
+                ops.rope_kv_write(qkv, ctx.positions, ctx.token_seq, inv_freq, rd, None, None, None, self.nq, nkv_here,
+                                  self.d, ctx.err, write_kv=False)
+            ops.attention_e4m3(qkv, out, *pages, table, ctx.q_start, ctx.seq_lens, ctx.num_decode, ctx.max_q_len,
+                               ctx.max_seq_len, self.nq, self.nkv, int(self.window or 0), self.scale, ctx.err)
+            return out
         window = int(self.window or 0)
         stride = qkv.shape[1]
         use_mma = ops.use_mma_attention(x.dtype, self.nq, self.nkv, self.d)

@@ -171,12 +171,16 @@ class ScaledRows:
 @dataclass
 class KVCacheView:
     """The pages of one run's attention: K and V [pages, nkv, page_size, d]; ``v`` is None
-    where a token keeps one row that serves as both (``KVPagesNeed.values`` False)."""
+    where a token keeps one row that serves as both (``KVPagesNeed.values`` False).  ``k_scale``
+    and ``v_scale`` [pages, nkv, page_size]: the rows' powers of two where the pages are kept in
+    8 bits (float8_e4m3fn pages, float8_e8m0fnu scales); None: pages in the run's type."""
 
     k: torch.Tensor
     v: Optional[torch.Tensor]
     group: int
     writes: bool
+    k_scale: Optional[torch.Tensor] = None
+    v_scale: Optional[torch.Tensor] = None
 
 
 @dataclass
@@ -236,6 +240,15 @@ class PositionEncoding(Part):
 class Mixer(Part):
     def cache_need(self):
         return None
+
+    def no_8_bit_cache(self) -> Optional[str]:
+        """Why this mixer cannot keep its pages in 8 bits; None: it can (its ``forward`` then gets a ``KVCacheView`` with
+        scales)."""
+        return "its mixer keeps its pages in the run's type"
+
+    def step_scratch_8_bit(self, max_model_len: int) -> int:
+        """``step_scratch`` where the pages are kept in 8 bits and no sequence passes ``max_model_len`` tokens."""
+        return self.step_scratch()
 
     def step_scratch(self) -> int:
         """Bytes that a step may take for a while by what the cache holds, beside those that grow with its tokens."""
