@@ -83,6 +83,95 @@ kv_e4m3_write_kernel(const T* qkv, T* q_out, long long q_stride, const int* __re
   }
 }
 
+// bfloat16 heads of 32, 64, 128 or 256, rotated whole or not at all, rows on 16 bytes: D / 16 lanes a row, each with 8 dims of its
+// first half and the 8 that pair with them, two 16-byte loads.  A thread's loads of KV8_ROWS rows are on their way while the block
+// makes the token's angles.  Bound by memory: 6,327 tokens of 32/8 heads of 128, 143 MB, 28 us (5.1 TB/s; a warp a row: 126 us;
+// two rows a thread 31, four 33 to 36, by the registers that they leave to blocks in flight).
+#define KV8_ROWS 3
+template <int D>
+__global__ void __launch_bounds__(128, 8)
+kv_e4m3_write_bf16_kernel(const bf16* qkv, bf16* q_out, long long q_stride, const int* __restrict__ positions,
+                          const int* __restrict__ token_seq, const double* __restrict__ inv_freq, int rotary_dim,
+                          const int* __restrict__ block_table, int max_blocks, int num_seqs, unsigned char* __restrict__ kcache,
+                          unsigned char* __restrict__ vcache, unsigned char* __restrict__ kscale,
+                          unsigned char* __restrict__ vscale, int nq, int nkv, int page_size, int num_pages,
+                          int* __restrict__ err) {
+  constexpr int L = D / 16, H = D / 2;
+  __shared__ __align__(16) float cs[D];                // cosines, sines
+  pdl_wait_on(qkv, positions, token_seq, block_table, q_out);
+  pdl_launch();
+  const int t = blockIdx.x, heads = nq + 2 * nkv, c = (threadIdx.x % L) * 8;
+  const bf16* row = qkv + (size_t)t * heads * D + c;
+  uint4 lo[KV8_ROWS], hi[KV8_ROWS];
+  auto load = [&](int base) {
+#pragma unroll
+    for (int k = 0; k < KV8_ROWS; ++k) {
+      const int h = base + (threadIdx.x + k * 128) / L;
+      if (h < heads) {
+        lo[k] = *(const uint4*)(row + (size_t)h * D);
+        hi[k] = *(const uint4*)(row + (size_t)h * D + H);
+      }
+    }
+  };
+  load(0);
+  const int pos = positions[t], seq = token_seq[t];
+  long long slot = -1;                                 // row of kv head 0; a head further: page_size rows on
+  if (pos >= 0 && pos / page_size < max_blocks && seq >= 0 && seq < num_seqs) {
+    const int page = block_table[(size_t)seq * max_blocks + pos / page_size];
+    if (page >= 0 && page < num_pages) slot = (long long)page * nkv * page_size + pos % page_size;
+  }
+  if (slot < 0 && threadIdx.x == 0) atomicOr(err, 2);
+  if (rotary_dim) {
+    for (int i = threadIdx.x; i < H; i += 128) rope_cos_sin(pos, inv_freq[i], &cs[i], &cs[H + i]);
+    __syncthreads();
+  }
+  float cx[8], sx[8];
+  if (rotary_dim) { load8(cs + c, cx); load8(cs + H + c, sx); }
+  for (int base = 0; base < heads; base += KV8_ROWS * 128 / L) {
+    if (base) load(base);
+#pragma unroll
+    for (int k = 0; k < KV8_ROWS; ++k) {
+      const int h = base + (threadIdx.x + k * 128) / L;
+      const bool live = h < heads;
+      float a[8], b[8];
+      unpack8(lo[k], a);
+      unpack8(hi[k], b);
+      if (rotary_dim && h < nq + nkv) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float x = a[e], y = b[e];
+          a[e] = x * cx[e] - y * sx[e];
+          b[e] = y * cx[e] + x * sx[e];
+        }
+      }
+      if (live && h < nq) {
+        bf16* dst = q_out + (size_t)t * q_stride + (size_t)h * D + c;
+        store8(dst, a);
+        store8(dst + H, b);
+      }
+      // the row's largest magnitude; NaN and infinities by their bits, which are the largest of all
+      unsigned top = 0u;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) top = max(top, max(__float_as_uint(a[e]) & 0x7fffffffu, __float_as_uint(b[e]) & 0x7fffffffu));
+#pragma unroll
+      for (int x = L / 2; x > 0; x >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, x));
+      if (!live || h < nq || slot < 0) continue;
+      const bool odd = top >= 0x7f800000u;
+      const int byte = odd ? KV8_NAN_SCALE : kv8_scale_byte(__uint_as_float(top));
+      const float inv = odd ? 0.f : kv8_inverse(byte);
+      const bool value = h >= nq + nkv;
+      const long long r = slot + (long long)(value ? h - nq - nkv : h - nq) * page_size;
+      unsigned char* dst = (value ? vcache : kcache) + r * D + c;
+      uint2 ca = make_uint2(kv8_pack4(a[0] * inv, a[1] * inv, a[2] * inv, a[3] * inv), kv8_pack4(a[4] * inv, a[5] * inv, a[6] * inv, a[7] * inv));
+      uint2 cb = make_uint2(kv8_pack4(b[0] * inv, b[1] * inv, b[2] * inv, b[3] * inv), kv8_pack4(b[4] * inv, b[5] * inv, b[6] * inv, b[7] * inv));
+      if (odd) ca = cb = make_uint2(0u, 0u);
+      *(uint2*)dst = ca;
+      *(uint2*)(dst + H) = cb;
+      if (c == 0) (value ? vscale : kscale)[r] = (unsigned char)byte;
+    }
+  }
+}
+
 RLLM_EXPORT int rllm_kv_e4m3_write(const void* qkv, int dtype, void* q_out, long long q_stride, const int* positions,
                                    const int* token_seq, const double* inv_freq, int rotary_dim, const int* block_table,
                                    int max_blocks, int num_seqs, void* kcache, void* vcache, void* kscale, void* vscale,
@@ -94,6 +183,18 @@ RLLM_EXPORT int rllm_kv_e4m3_write(const void* qkv, int dtype, void* q_out, long
       page_size <= 0 || num_pages <= 0 || max_blocks <= 0 || num_seqs <= 0 || q_stride < (long long)nq * d)
     return RLLM_E_BADARG;
   if (d % 16 || d > 256) return RLLM_E_UNSUPPORTED;
+  if (dtype == RLLM_DT_BF16 && (d == 32 || d == 64 || d == 128 || d == 256) && (rotary_dim == d || rotary_dim == 0) &&
+      (((uintptr_t)qkv | (uintptr_t)q_out | (uintptr_t)q_stride * 2) & 15) == 0 && (((uintptr_t)kcache | (uintptr_t)vcache) & 7) == 0) {
+#define KV8_WRITE(DD) rllm_launch_pdl(kv_e4m3_write_bf16_kernel<DD>, dim3(T), dim3(128), (size_t)0, stream, (const bf16*)qkv, (bf16*)q_out, \
+      q_stride, positions, token_seq, inv_freq, rotary_dim, block_table, max_blocks, num_seqs, (unsigned char*)kcache,                   \
+      (unsigned char*)vcache, (unsigned char*)kscale, (unsigned char*)vscale, nq, nkv, page_size, num_pages, err)
+    if (d == 32) KV8_WRITE(32);
+    else if (d == 64) KV8_WRITE(64);
+    else if (d == 128) KV8_WRITE(128);
+    else KV8_WRITE(256);
+    RLLM_LAUNCH_CHECK();
+    return 0;
+  }
   const size_t smem = (size_t)rotary_dim * sizeof(float);
   RLLM_DISPATCH_DTYPE(dtype, T_,
     rllm_launch_pdl(kv_e4m3_write_kernel<T_>, dim3(T), dim3(256), smem, stream, (const T_*)qkv, (T_*)q_out, q_stride, positions,
@@ -106,7 +207,9 @@ RLLM_EXPORT int rllm_kv_e4m3_write(const void* qkv, int dtype, void* q_out, long
 // ---------------------------------------------------------------------------
 // read: out_k[t], out_v[t] = the rows of (token_seq[t], positions[t])
 // ---------------------------------------------------------------------------
-// A thread reads 16 numbers (16 bytes) of a row and writes them as 16 values.
+// A thread takes the same 16 numbers (16 bytes) of KV8_TOKENS tokens' rows, all of them on their way at once, and writes them as
+// 16 values each.
+#define KV8_TOKENS 4
 template <typename T>
 __global__ void __launch_bounds__(256)
 kv_e4m3_read_kernel(const int* __restrict__ positions, const int* __restrict__ token_seq, const int* __restrict__ block_table,
@@ -116,44 +219,55 @@ kv_e4m3_read_kernel(const int* __restrict__ positions, const int* __restrict__ t
                     int nkv, int d, int page_size, int num_pages, int* __restrict__ err) {
   pdl_wait_on(positions, token_seq, block_table, kcache, vcache, kscale, vscale);
   pdl_launch();
-  const int pieces = nkv * (d >> 4);                   // of a token's keys; as many of its values
-  const long long all = (long long)T_tokens * 2 * pieces;
-  for (long long at = (long long)blockIdx.x * blockDim.x + threadIdx.x; at < all; at += (long long)gridDim.x * blockDim.x) {
-    const int t = (int)(at / (2 * pieces));
-    int c = (int)(at - (long long)t * 2 * pieces);
-    const bool value = c >= pieces;
-    if (value) c -= pieces;
-    const int h = c / (d >> 4), i = (c - h * (d >> 4)) << 4;
-    const int pos = positions[t], seq = token_seq[t];
-    long long r = -1;
-    if (pos >= 0 && pos / page_size < max_blocks && seq >= 0 && seq < num_seqs) {
-      const int page = block_table[(size_t)seq * max_blocks + pos / page_size];
-      if (page >= 0 && page < num_pages) r = ((long long)page * nkv + h) * page_size + pos % page_size;
+  const int per_row = d >> 4, pieces = nkv * per_row;  // pieces of a token's keys; as many of its values
+  const long long t0 = (long long)blockIdx.x * KV8_TOKENS;
+  int page[KV8_TOKENS], at[KV8_TOKENS];
+#pragma unroll
+  for (int u = 0; u < KV8_TOKENS; ++u) {
+    const long long t = t0 + u;
+    page[u] = -1;
+    at[u] = 0;
+    if (t < T_tokens) {
+      const int pos = positions[t], seq = token_seq[t];
+      if (pos >= 0 && pos / page_size < max_blocks && seq >= 0 && seq < num_seqs) {
+        page[u] = block_table[(size_t)seq * max_blocks + pos / page_size];
+        at[u] = pos % page_size;
+        if (page[u] >= num_pages) page[u] = -1;
+      }
+      if (page[u] < 0 && threadIdx.x == 0) atomicOr(err, 4);
     }
-    float x[16];
-    if (r < 0) {
-      if (c == 0) atomicOr(err, 4);
+  }
+  for (int x = threadIdx.x; x < 2 * pieces; x += blockDim.x) {
+    const bool value = x >= pieces;
+    const int c = value ? x - pieces : x, h = c / per_row, i = (c - h * per_row) << 4;
+    const unsigned char *codes = value ? vcache : kcache, *scale = value ? vscale : kscale;
+    uint4 raw[KV8_TOKENS];
+    int byte[KV8_TOKENS];
 #pragma unroll
-      for (int k = 0; k < 16; ++k) x[k] = 0.f;
-    } else {
-      const uint4 raw = *(const uint4*)((value ? vcache : kcache) + r * d + i);
-      const float power = kv8_power((value ? vscale : kscale)[r]);
-      kv8_floats(raw.x, x); kv8_floats(raw.y, x + 4); kv8_floats(raw.z, x + 8); kv8_floats(raw.w, x + 12);
-#pragma unroll
-      for (int k = 0; k < 16; ++k) x[k] *= power;
+    for (int u = 0; u < KV8_TOKENS; ++u) {
+      const long long r = ((long long)page[u] * nkv + h) * page_size + at[u];
+      raw[u] = page[u] >= 0 ? *(const uint4*)(codes + r * d + i) : make_uint4(0u, 0u, 0u, 0u);
+      byte[u] = page[u] >= 0 ? scale[r] : 0;
     }
-    T* dst = (value ? out_v : out_k) + (size_t)t * nkv * d + (size_t)h * d + i;
-    float lo[8], hi[8];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) { lo[k] = x[k]; hi[k] = x[k + 8]; }
-    if constexpr (sizeof(T) == 4) {
-      *(float4*)dst = make_float4(lo[0], lo[1], lo[2], lo[3]);
-      *(float4*)(dst + 4) = make_float4(lo[4], lo[5], lo[6], lo[7]);
-      *(float4*)(dst + 8) = make_float4(hi[0], hi[1], hi[2], hi[3]);
-      *(float4*)(dst + 12) = make_float4(hi[4], hi[5], hi[6], hi[7]);
-    } else {
-      store8(dst, lo);
-      store8(dst + 8, hi);
+    for (int u = 0; u < KV8_TOKENS; ++u) {
+      if (t0 + u >= T_tokens) break;
+      const float power = kv8_power(byte[u]);
+      float y[16];
+      kv8_floats(raw[u].x, y); kv8_floats(raw[u].y, y + 4); kv8_floats(raw[u].z, y + 8); kv8_floats(raw[u].w, y + 12);
+      T* dst = (value ? out_v : out_k) + (size_t)(t0 + u) * nkv * d + (size_t)h * d + i;
+      float lo[8], hi[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) { lo[k] = y[k] * power; hi[k] = y[k + 8] * power; }
+      if constexpr (sizeof(T) == 4) {
+        *(float4*)dst = make_float4(lo[0], lo[1], lo[2], lo[3]);
+        *(float4*)(dst + 4) = make_float4(lo[4], lo[5], lo[6], lo[7]);
+        *(float4*)(dst + 8) = make_float4(hi[0], hi[1], hi[2], hi[3]);
+        *(float4*)(dst + 12) = make_float4(hi[4], hi[5], hi[6], hi[7]);
+      } else {
+        store8(dst, lo);
+        store8(dst + 8, hi);
+      }
     }
   }
 }
@@ -168,10 +282,10 @@ RLLM_EXPORT int rllm_kv_e4m3_read(const int* positions, const int* token_seq, co
     return RLLM_E_BADARG;
   if (d % 16 || d > 256) return RLLM_E_UNSUPPORTED;
   if (((uintptr_t)kcache | (uintptr_t)vcache | (uintptr_t)out_k | (uintptr_t)out_v) & 15) return RLLM_E_UNSUPPORTED;
-  const long long threads = (long long)T * 2 * nkv * (d >> 4), blocks = (threads + 255) / 256;
-  const unsigned grid = (unsigned)(blocks < (1 << 20) ? blocks : (1 << 20));
+  const int threads = 2 * nkv * (d >> 4), block = threads >= 256 ? 256 : (threads + 31) / 32 * 32;
+  const unsigned grid = (unsigned)(((long long)T + KV8_TOKENS - 1) / KV8_TOKENS);
   RLLM_DISPATCH_DTYPE(dtype, T_,
-    rllm_launch_pdl(kv_e4m3_read_kernel<T_>, dim3(grid), dim3(256), (size_t)0, stream, positions, token_seq, block_table,
+    rllm_launch_pdl(kv_e4m3_read_kernel<T_>, dim3(grid), dim3(block), (size_t)0, stream, positions, token_seq, block_table,
                     max_blocks, num_seqs, (const unsigned char*)kcache, (const unsigned char*)vcache,
                     (const unsigned char*)kscale, (const unsigned char*)vscale, (T_*)out_k, (T_*)out_v, T, nkv, d, page_size,
                     num_pages, err));

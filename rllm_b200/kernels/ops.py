@@ -2062,8 +2062,11 @@ E4M3, E8M0 = torch.float8_e4m3fn, torch.float8_e8m0fnu
 
 
 def _e4m3_cache(kcache: torch.Tensor, vcache: torch.Tensor, kscale: torch.Tensor, vscale: torch.Tensor,
-                block_table: torch.Tensor, nkv: int, d: int) -> None:
-    """What every operator over such a cache asks of it."""
+                block_table: torch.Tensor, nkv: int, d: int, *vectors: torch.Tensor) -> None:
+    """Raise unless these are what every operator over such a cache asks for; ``vectors``: int32, one-dimensional.  The
+    extension module answers first, in a fraction of the time; what it turns down is looked at here for the reason."""
+    if _launch().e4m3_ready(kcache, vcache, kscale, vscale, block_table, nkv, d, *vectors):
+        return
     if kcache.dtype is not E4M3 or vcache.dtype is not E4M3 or kscale.dtype is not E8M0 or vscale.dtype is not E8M0:
         raise KernelError("an 8-bit cache has float8_e4m3fn pages and float8_e8m0fnu scales")
     if kcache.dim() != 4 or kcache.shape != vcache.shape or kcache.shape[1] != nkv or kcache.shape[3] != d or \
@@ -2073,6 +2076,11 @@ def _e4m3_cache(kcache: torch.Tensor, vcache: torch.Tensor, kscale: torch.Tensor
         raise KernelError("block_table must be int32 [sequences, blocks]")
     for t, name in ((kcache, "kcache"), (vcache, "vcache"), (kscale, "kscale"), (vscale, "vscale"), (block_table, "block_table")):
         _contig(t, name)
+    for t in vectors:
+        if t.dtype is not torch.int32 or t.dim() != 1 or not t.is_contiguous():
+            raise KernelError("positions, token_seq, q_start, seq_lens and err must be contiguous int32 vectors")
+    _on_current_device(kcache, vcache, kscale, vscale, block_table, *vectors)
+    raise KernelError("these tensors make no 8-bit cache")
 
 
 def _on_current_device(*tensors: torch.Tensor) -> None:
@@ -2086,9 +2094,10 @@ def _on_current_device(*tensors: torch.Tensor) -> None:
             raise KernelError(f"a tensor on {t.device} while cuda:{here} is the current device")
 
 
-def _ints(t: torch.Tensor, name: str, n: Optional[int] = None) -> None:
-    if t.dtype is not torch.int32 or t.dim() != 1 or not t.is_contiguous() or (n is not None and t.numel() != n):
-        raise KernelError(f"{name} must be a contiguous int32 vector" + ("" if n is None else f" of {n}"))
+def _beside(cache: torch.Tensor, *tensors: torch.Tensor) -> None:
+    for t in tensors:
+        if t.get_device() != cache.get_device():
+            raise KernelError(f"a tensor on {t.device} with a cache on {cache.device}")
 
 
 def rope_kv_write_e4m3(qkv: torch.Tensor, positions: torch.Tensor, token_seq: torch.Tensor,
@@ -2100,23 +2109,27 @@ def rope_kv_write_e4m3(qkv: torch.Tensor, positions: torch.Tensor, token_seq: to
 
     The rotation and the row's scale are float32; a number is rounded once, to e4m3.  A (sequence, position) pair may stand
     in the step once.  A token whose page is not held sets bit 2 of ``err`` and is not written (its q is rotated)."""
-    T = qkv.shape[0]
     dt = dtype_code(qkv.dtype)
-    if qkv.dim() != 2 or qkv.shape[1] != (nq + 2 * nkv) * d:
-        raise KernelError("rope_kv_write_e4m3: qkv must be [T, (nq + 2 nkv) d]")
-    _contig(qkv, "qkv")
-    _e4m3_cache(kcache, vcache, kscale, vscale, block_table, nkv, d)
-    _ints(positions, "positions", T); _ints(token_seq, "token_seq", T)
-    if rotary_dim and (inv_freq is None or inv_freq.dtype is not torch.float64 or inv_freq.numel() != rotary_dim // 2):
+    if qkv.dim() != 2 or qkv.shape[1] != (nq + 2 * nkv) * d or not qkv.is_contiguous():
+        raise KernelError("rope_kv_write_e4m3: qkv must be [T, (nq + 2 nkv) d], contiguous")
+    T = qkv.shape[0]
+    if positions.numel() != T or token_seq.numel() != T:
+        raise KernelError("rope_kv_write_e4m3: a position and a sequence for every token of qkv")
+    if rotary_dim and (inv_freq is None or inv_freq.dtype is not torch.float64 or inv_freq.numel() != rotary_dim // 2 or
+                       not inv_freq.is_contiguous()):
         raise KernelError("rope_kv_write_e4m3: inv_freq must be float64 [rotary_dim / 2]")
     if q_out is None:
-        q_out = qkv
-    elif q_out.dtype is not qkv.dtype or q_out.shape != (T, nq * d) or q_out.stride(1) != 1:
-        raise KernelError("rope_kv_write_e4m3: q_out must be [T, nq d] of qkv's type")
-    _on_current_device(qkv, kcache, block_table, q_out)
-    _entries.rllm_kv_e4m3_write(qkv, dt, q_out, q_out.stride(0), positions, token_seq, inv_freq if rotary_dim else None,
-                                rotary_dim, block_table, block_table.shape[1], block_table.shape[0], kcache, vcache, kscale,
-                                vscale, T, nq, nkv, d, kcache.shape[2], kcache.shape[0], err)
+        q_out, stride = qkv, qkv.shape[1]
+    else:
+        if q_out.dtype is not qkv.dtype or q_out.shape != (T, nq * d) or q_out.stride(1) != 1:
+            raise KernelError("rope_kv_write_e4m3: q_out must be [T, nq d] of qkv's type")
+        stride = max(q_out.stride(0), nq * d) if T <= 1 else q_out.stride(0)
+    _e4m3_cache(kcache, vcache, kscale, vscale, block_table, nkv, d, positions, token_seq, err)
+    _beside(kcache, qkv, q_out)
+    pages, _, page_size, _ = kcache.shape
+    seqs, blocks = block_table.shape
+    _entries.rllm_kv_e4m3_write(qkv, dt, q_out, stride, positions, token_seq, inv_freq if rotary_dim else None, rotary_dim,
+                                block_table, blocks, seqs, kcache, vcache, kscale, vscale, T, nq, nkv, d, page_size, pages, err)
 
 
 def kv_read_e4m3(positions: torch.Tensor, token_seq: torch.Tensor, block_table: torch.Tensor, kcache: torch.Tensor,
@@ -2125,21 +2138,21 @@ def kv_read_e4m3(positions: torch.Tensor, token_seq: torch.Tensor, block_table: 
     """Keys and values of given tokens out of a cache kept in 8 bits: out_k, out_v [T, nkv d] (bfloat16 or float32) = the
     rows of sequence ``token_seq[t]``'s token at ``positions[t]``.  Exact in float32, and in bfloat16 down to its smallest
     numbers; NaN where a row's scale is.  A token whose page is not held sets bit 4 of ``err`` and reads as zeros."""
-    T = positions.numel()
+    dt = dtype_code(out_k.dtype)
     if kcache.dim() != 4:
         raise KernelError("kv_read_e4m3: kcache must be [pages, nkv, page_size, d]")
-    nkv, d = kcache.shape[1], kcache.shape[3]
-    _e4m3_cache(kcache, vcache, kscale, vscale, block_table, nkv, d)
-    _ints(positions, "positions"); _ints(token_seq, "token_seq", T)
-    for t, name in ((out_k, "out_k"), (out_v, "out_v")):
-        if t.shape != (T, nkv * d) or t.dtype is not out_k.dtype:
-            raise KernelError("kv_read_e4m3: out_k and out_v must be [T, nkv d] of one type")
-        _contig(t, name)
-    dt = dtype_code(out_k.dtype)
-    _on_current_device(kcache, block_table, out_k)
-    _entries.rllm_kv_e4m3_read(positions, token_seq, block_table, block_table.shape[1], block_table.shape[0], kcache, vcache,
-                               kscale, vscale, out_k, out_v, dt, T, nkv, d, kcache.shape[2],
-                               kcache.shape[0], err)
+    pages, nkv, page_size, d = kcache.shape
+    T = positions.numel()
+    if token_seq.numel() != T:
+        raise KernelError("kv_read_e4m3: a sequence for every position")
+    for t in (out_k, out_v):
+        if t.shape != (T, nkv * d) or t.dtype is not out_k.dtype or not t.is_contiguous():
+            raise KernelError("kv_read_e4m3: out_k and out_v must be [T, nkv d] of one type, contiguous")
+    _e4m3_cache(kcache, vcache, kscale, vscale, block_table, nkv, d, positions, token_seq, err)
+    _beside(kcache, out_k, out_v)
+    seqs, blocks = block_table.shape
+    _entries.rllm_kv_e4m3_read(positions, token_seq, block_table, blocks, seqs, kcache, vcache, kscale, vscale, out_k, out_v,
+                               dt, T, nkv, d, page_size, pages, err)
 
 
 E4M3_DENSE_SCRATCH = 512 << 20      # bytes of widened keys and values at a time; more only where one sequence needs more
@@ -2176,34 +2189,33 @@ def attention_e4m3(q: torch.Tensor, out: torch.Tensor, kcache: torch.Tensor, vca
     in this step and in the cache.  Rows behind the last sequence's stay as they are.  A page that is not held sets bit 4 of
     ``err``, and its keys are left out."""
     dt = dtype_code(q.dtype)
-    S = seq_lens.numel()
-    if q.dim() != 2 or q.stride(1) != 1 or out.dim() != 2 or out.dtype is not q.dtype or out.shape[1] != nq * (kcache.shape[-1]) or \
-            q.shape[1] < out.shape[1] or q.shape[0] < out.shape[0]:
+    S, d = seq_lens.numel(), kcache.shape[-1]
+    if q.dim() != 2 or out.dim() != 2 or out.dtype is not q.dtype:
         raise KernelError("attention_e4m3: q must be [T, >= nq d] and out [T, nq d] of one type")
-    d = kcache.shape[-1]
-    _contig(out, "out")
-    _e4m3_cache(kcache, vcache, kscale, vscale, block_table, nkv, d)
-    _ints(q_start, "q_start", S + 1); _ints(seq_lens, "seq_lens")
-    if not 0 <= num_decode <= S or block_table.shape[0] < S or max_q_len < 0 or max_seq_len < 0:
-        raise KernelError("attention_e4m3: bad counts of sequences or bounds of lengths")
-    if max_seq_len > block_table.shape[1] * kcache.shape[2]:
-        raise KernelError("attention_e4m3: max_seq_len passes what block_table's rows can hold")
-    _on_current_device(q, kcache, block_table, out)
-    T = out.shape[0]
+    (T, width), stride = out.shape, q.stride(0)
+    if q.stride(1) != 1 or width != nq * d or q.shape[1] < width or q.shape[0] < T or not out.is_contiguous():
+        raise KernelError("attention_e4m3: q must be [T, >= nq d] and out [T, nq d] of one type, their rows contiguous")
+    _e4m3_cache(kcache, vcache, kscale, vscale, block_table, nkv, d, q_start, seq_lens, err)
+    _beside(kcache, q, out)
+    pages, _, page_size, _ = kcache.shape
+    seqs, blocks = block_table.shape
+    if q_start.numel() != S + 1 or not 0 <= num_decode <= S or seqs < S or max_q_len < 0 or not 0 <= max_seq_len <= blocks * page_size:
+        raise KernelError("attention_e4m3: q_start [S + 1] and seq_lens [S], num_decode of them with one token, a row of block_table "
+                          "each, that can hold max_seq_len tokens")
     if T == 0 or S == 0:
         return
-    cache = (kcache, vcache, kscale, vscale, dt, block_table, block_table.shape[1], q_start, seq_lens)
-    heads = (nq, nkv, d, kcache.shape[2], kcache.shape[0], window, scale, err)
-    if d not in (64, 128, 256) or kcache.shape[2] % 16:
-        _entries.rllm_attention_e4m3_simt(q, q.stride(0), out, *cache, 0, S, T, *heads)
+    cache = (kcache, vcache, kscale, vscale, dt, block_table, blocks, q_start, seq_lens)
+    heads = (nq, nkv, d, page_size, pages, window, scale, err)
+    if d not in (64, 128, 256) or page_size % 16:
+        _entries.rllm_attention_e4m3_simt(q, stride, out, *cache, 0, S, T, *heads)
         return
     keys = max_seq_len if window <= 0 else min(max_seq_len, window + max_q_len)
     if num_decode:
-        _entries.rllm_attention_e4m3_rows(q, q.stride(0), out, *cache, 0, num_decode, 1, keys, *heads)
+        _entries.rllm_attention_e4m3_rows(q, stride, out, *cache, 0, num_decode, 1, keys, *heads)
     if num_decode == S:
         return
     if attention_e4m3_dense_takes(q.dtype, nq, nkv, d, scale) and attention_e4m3_dense_pays(max_q_len, nq, nkv) and \
-            q.stride(0) % 8 == 0 and q.data_ptr() % 16 == 0:
+            stride % 8 == 0 and q.data_ptr() % 16 == 0:
         bn = 8192 // d
         tiles = keys // bn + 2
         a_sequence = 2 * tiles * nkv * bn * d
@@ -2212,10 +2224,9 @@ def attention_e4m3(q: torch.Tensor, out: torch.Tensor, kcache: torch.Tensor, vca
         marks = torch.empty(group * tiles * nkv * 8, dtype=torch.int32, device=q.device)
         for first in range(num_decode, S, group):
             n = min(group, S - first)
-            _entries.rllm_kv_e4m3_widen(block_table, block_table.shape[1], q_start, seq_lens, first, n, tiles, kcache, vcache,
-                                        kscale, vscale, dense[0], dense[1], marks, nkv, d, kcache.shape[2], kcache.shape[0],
-                                        window, err)
-            _entries.rllm_attention_dense_tcgen05(q, q.stride(0), q.shape[0], out, dense[0], dense[1], marks, tiles, q_start,
+            _entries.rllm_kv_e4m3_widen(block_table, blocks, q_start, seq_lens, first, n, tiles, kcache, vcache, kscale, vscale,
+                                        dense[0], dense[1], marks, nkv, d, page_size, pages, window, err)
+            _entries.rllm_attention_dense_tcgen05(q, stride, q.shape[0], out, dense[0], dense[1], marks, tiles, q_start,
                                                   seq_lens, first, n, min(T, n * max_q_len), nq, nkv, d, window, scale, err)
         return
-    _entries.rllm_attention_e4m3_rows(q, q.stride(0), out, *cache, num_decode, S, max_q_len, keys, *heads)
+    _entries.rllm_attention_e4m3_rows(q, stride, out, *cache, num_decode, S, max_q_len, keys, *heads)

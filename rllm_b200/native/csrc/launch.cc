@@ -275,6 +275,50 @@ PyObject* product(PyObject*, PyObject* const* args, Py_ssize_t n) {
   return guarded([&] { return checked_product(args); });
 }
 
+// ---------------------------------------------------------------------------------------------------------------
+// a cache kept in 8 bits
+// ---------------------------------------------------------------------------------------------------------------
+// e4m3_ready(kcache, vcache, kscale, vscale, block_table, nkv, d, *vectors): whether these are what the operators over such a
+// cache take (see rllm_b200/kernels/ops.py, _e4m3_cache, which holds the same rules and says what is wrong): all on the current
+// device, the vectors contiguous, one-dimensional and int32.  In Python these checks cost as much as the launch three times over.
+bool e4m3_ready_args(PyObject* const* args, Py_ssize_t n) {
+  for (int i = 0; i < 5; ++i)
+    if (!THPVariable_Check(args[i])) return false;
+  const long long nkv = PyLong_AsLongLong(args[5]), d = PyLong_AsLongLong(args[6]);
+  if (PyErr_Occurred()) return false;
+  const at::Tensor &k = THPVariable_Unpack(args[0]), &v = THPVariable_Unpack(args[1]), &ks = THPVariable_Unpack(args[2]),
+                   &vs = THPVariable_Unpack(args[3]), &table = THPVariable_Unpack(args[4]);
+  if (k.scalar_type() != at::kFloat8_e4m3fn || v.scalar_type() != at::kFloat8_e4m3fn || ks.scalar_type() != at::kFloat8_e8m0fnu ||
+      vs.scalar_type() != at::kFloat8_e8m0fnu || table.scalar_type() != at::kInt)
+    return false;
+  if (k.dim() != 4 || k.size(1) != nkv || k.size(3) != d || v.sizes() != k.sizes() || ks.sizes() != k.sizes().slice(0, 3) ||
+      vs.sizes() != ks.sizes() || table.dim() != 2)
+    return false;
+  const int device = c10::cuda::current_device();
+  for (int i = 0; i < 5; ++i) {
+    const at::Tensor& t = THPVariable_Unpack(args[i]);
+    if (!t.is_cuda() || t.get_device() != device || !t.is_contiguous()) return false;
+  }
+  for (Py_ssize_t i = 7; i < n; ++i) {
+    if (!THPVariable_Check(args[i])) return false;
+    const at::Tensor& t = THPVariable_Unpack(args[i]);
+    if (!t.is_cuda() || t.get_device() != device || t.scalar_type() != at::kInt || t.dim() != 1 || !t.is_contiguous()) return false;
+  }
+  return true;
+}
+
+PyObject* e4m3_ready(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (n < 7) return PyErr_Format(PyExc_TypeError, "e4m3_ready(kcache, vcache, kscale, vscale, block_table, nkv, d, *vectors)");
+  // (a tensor without CUDA, before CUDA is asked for its device)
+  for (int i = 0; i < 5; ++i)
+    if (!THPVariable_Check(args[i]) || !THPVariable_Unpack(args[i]).is_cuda()) Py_RETURN_FALSE;
+  return guarded([&]() -> PyObject* {
+    const bool ok = e4m3_ready_args(args, n);
+    if (PyErr_Occurred()) return nullptr;
+    return PyBool_FromLong(ok);
+  });
+}
+
 // setup(exception class, list of one int)
 PyObject* setup(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (n != 2 || !PyList_Check(args[1]) || PyList_GET_SIZE(args[1]) != 1) return PyErr_Format(PyExc_TypeError, "setup(exception, [count])");
@@ -288,6 +332,7 @@ PyMethodDef kMethods[] = {{"setup", (PyCFunction)(void*)setup, METH_FASTCALL, nu
                           {"products", (PyCFunction)(void*)set_products, METH_FASTCALL, nullptr},
                           {"error_word", (PyCFunction)(void*)set_error_word, METH_FASTCALL, nullptr},
                           {"product", (PyCFunction)(void*)product, METH_FASTCALL, nullptr},
+                          {"e4m3_ready", (PyCFunction)(void*)e4m3_ready, METH_FASTCALL, nullptr},
                           {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "launch", nullptr, -1, kMethods};
 
