@@ -64,6 +64,7 @@ _TABLE = {
     "rllm_kv_e4m3_read": ("kv_e4m3", "pppiippppppiiiiiip", "kv_read_e4m3"),
     "rllm_kv_e4m3_widen": ("kv_e4m3", "pippiiipppppppiiiiip", "attention_e4m3"),
     "rllm_attention_dense_tcgen05": ("attention_tcgen05", "piippppippiiiiiiifp", "attention_e4m3"),
+    "rllm_attention_e4m3_tcgen05": ("attention_e4m3_tcgen05", "pippppppippiiiiiiiiiifp", "attention_e4m3"),
     "rllm_attention_e4m3_rows": ("attention_e4m3", "pipppppipippiiiiiiiiiifp", "attention_e4m3"),
     "rllm_attention_e4m3_simt": ("attention_e4m3", "pipppppipippiiiiiiiiifp", "attention_e4m3"),
     "rllm_softcap": ("elementwise", "plf", "softcap_rows"),
@@ -2166,15 +2167,16 @@ def e4m3_dense_scratch(nkv: int, d: int, max_seq_len: int) -> int:
     return max(E4M3_DENSE_SCRATCH, 4 * (max_seq_len // bn + 2) * nkv * bn * d)
 
 
-def attention_e4m3_dense_takes(dtype: torch.dtype, nq: int, nkv: int, d: int, scale: float) -> bool:
-    """The sizes of the prompt attention on tcgen05 over widened keys and values."""
-    return dtype is torch.bfloat16 and d in (64, 128) and nq // nkv <= 128 and scale > 0 and \
-        os.environ.get("RLLM_ATTENTION") not in ("simt", "mma")
-
-
-def attention_e4m3_dense_pays(max_q_len: int, nq: int, nkv: int) -> bool:
-    """Whether sequences of up to so many tokens are faster that way than a tile of 16 rows at a time."""
-    return max_q_len * (nq // nkv) >= 64
+def attention_e4m3_form(dtype: torch.dtype, nq: int, nkv: int, d: int, page_size: int, scale: float, max_q_len: int) -> str:
+    """Which kernel takes sequences of up to ``max_q_len`` tokens: "rows" (mma.sync, 16 rows of a kv head at a time), "tcgen05"
+    (128 rows, keys and values widened inside), "dense" (tcgen05 over keys and values widened once for all rows), or "simt"."""
+    g, forced = nq // nkv, os.environ.get("RLLM_ATTENTION")
+    if dtype is torch.bfloat16 and d in (64, 128) and g <= 128 and scale > 0 and forced not in ("simt", "mma"):
+        if max_q_len * g >= 96:
+            return "dense"
+    if d in (64, 128, 256) and page_size % 16 == 0 and forced != "simt":
+        return "rows"
+    return "simt"
 
 
 def attention_e4m3(q: torch.Tensor, out: torch.Tensor, kcache: torch.Tensor, vcache: torch.Tensor, kscale: torch.Tensor,
@@ -2206,27 +2208,30 @@ def attention_e4m3(q: torch.Tensor, out: torch.Tensor, kcache: torch.Tensor, vca
         return
     cache = (kcache, vcache, kscale, vscale, dt, block_table, blocks, q_start, seq_lens)
     heads = (nq, nkv, d, page_size, pages, window, scale, err)
-    if d not in (64, 128, 256) or page_size % 16:
-        _entries.rllm_attention_e4m3_simt(q, stride, out, *cache, 0, S, T, *heads)
-        return
     keys = max_seq_len if window <= 0 else min(max_seq_len, window + max_q_len)
-    if num_decode:
-        _entries.rllm_attention_e4m3_rows(q, stride, out, *cache, 0, num_decode, 1, keys, *heads)
-    if num_decode == S:
-        return
-    if attention_e4m3_dense_takes(q.dtype, nq, nkv, d, scale) and attention_e4m3_dense_pays(max_q_len, nq, nkv) and \
-            stride % 8 == 0 and q.data_ptr() % 16 == 0:
-        bn = 8192 // d
-        tiles = keys // bn + 2
-        a_sequence = 2 * tiles * nkv * bn * d
-        group = max(1, min(S - num_decode, E4M3_DENSE_SCRATCH // (2 * a_sequence), 65535))
-        dense = torch.empty((2, group * a_sequence // 2), dtype=torch.bfloat16, device=q.device)
-        marks = torch.empty(group * tiles * nkv * 8, dtype=torch.int32, device=q.device)
-        for first in range(num_decode, S, group):
-            n = min(group, S - first)
-            _entries.rllm_kv_e4m3_widen(block_table, blocks, q_start, seq_lens, first, n, tiles, kcache, vcache, kscale, vscale,
-                                        dense[0], dense[1], marks, nkv, d, page_size, pages, window, err)
-            _entries.rllm_attention_dense_tcgen05(q, stride, q.shape[0], out, dense[0], dense[1], marks, tiles, q_start,
-                                                  seq_lens, first, n, min(T, n * max_q_len), nq, nkv, d, window, scale, err)
-        return
-    _entries.rllm_attention_e4m3_rows(q, stride, out, *cache, num_decode, S, max_q_len, keys, *heads)
+    for first, end, longest in ((0, num_decode, 1), (num_decode, S, max_q_len)):
+        if first == end or longest == 0:
+            continue
+        form = attention_e4m3_form(q.dtype, nq, nkv, d, page_size, scale, longest)
+        if form in ("tcgen05", "dense") and (stride % 8 or (q.data_ptr() | out.data_ptr()) % 16):
+            form = "rows" if page_size % 16 == 0 else "simt"
+        if form == "rows":
+            _entries.rllm_attention_e4m3_rows(q, stride, out, *cache, first, end, longest, keys, *heads)
+        elif form == "tcgen05":
+            _entries.rllm_attention_e4m3_tcgen05(q, stride, out, kcache, vcache, kscale, vscale, block_table, blocks, q_start,
+                                                 seq_lens, first, end, longest, keys, *heads)
+        elif form == "simt":
+            _entries.rllm_attention_e4m3_simt(q, stride, out, *cache, first, end, min(T, (end - first) * longest), *heads)
+        else:
+            bn = 8192 // d
+            tiles = keys // bn + 2
+            a_sequence = 2 * tiles * nkv * bn * d
+            group = max(1, min(end - first, E4M3_DENSE_SCRATCH // (2 * a_sequence), 65535))
+            dense = torch.empty((2, group * a_sequence // 2), dtype=torch.bfloat16, device=q.device)
+            marks = torch.empty(group * tiles * nkv * 8, dtype=torch.int32, device=q.device)
+            for s in range(first, end, group):
+                n = min(group, end - s)
+                _entries.rllm_kv_e4m3_widen(block_table, blocks, q_start, seq_lens, s, n, tiles, kcache, vcache, kscale, vscale,
+                                            dense[0], dense[1], marks, nkv, d, page_size, pages, window, err)
+                _entries.rllm_attention_dense_tcgen05(q, stride, q.shape[0], out, dense[0], dense[1], marks, tiles, q_start,
+                                                      seq_lens, s, n, min(T, n * longest), nq, nkv, d, window, scale, err)

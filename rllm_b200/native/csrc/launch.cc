@@ -99,7 +99,7 @@ const Row kSignatures[] = {
     ROW("piiipppppppi"), ROW("piippifpppfippppiiiiiippip"), ROW("piippippppiiipiiip"),
     ROW("piippppifpippiiiiiiipiiippififiip"), ROW("piippppippiiiiiiiiifiifppiipp"), ROW("piippppippiiiiiiiiifpi"),
     ROW("piipppppipipppippiiiiiiiiipp"), ROW("piplpppipiippppiiiiiip"), ROW("pppiippppppiiiiiip"), ROW("pipppppipippiiiiiiiiifp"),
-    ROW("pipppppipippiiiiiiiiiifp"), ROW("pippiiipppppppiiiiip"), ROW("piippppippiiiiiiifp"), ROW("piippppppppiiiiff"), ROW("piiipppppppppiiipiiiip"), ROW("pipifpipiiiiifff"),
+    ROW("pipppppipippiiiiiiiiiifp"), ROW("pippiiipppppppiiiiip"), ROW("pippppppippiiiiiiiiiifp"), ROW("piippppippiiiiiiifp"), ROW("piippppppppiiiiff"), ROW("piiipppppppppiiipiiiip"), ROW("pipifpipiiiiifff"),
     ROW("pipipiiii"), ROW("pipipiiiiifff"), ROW("pipipiiiiifffp"), ROW("pipipippipippiii"), ROW("pippifpppfipppppiiiiiiipp"),
     ROW("pippiiipppiiiiiiiifpp"), ROW("pippippppipppppppiiiiiiiiiiiiifffip"), ROW("pipppipippiiiiiiifp"),
     ROW("pipppipippiiiiiiiifiifppiipiip"), ROW("pipppipippiiiiiiip"), ROW("pipppippiiiiiiiiifpp"),
