@@ -190,7 +190,7 @@ template <int N> __device__ __forceinline__ void e4_copy_wait() { asm volatile("
 // a tile of 16 keys in shared memory: K's pieces, V's, 16 + 16 scale bytes; a pair is two of them
 template <int D, int NB, typename T> constexpr int e4_ctas() {  // of an SM
   if (sizeof(T) == 2 && NB == 1) return D == 64 ? 5 : D == 128 ? 4 : 2;
-  return D == 64 ? 3 : D == 128 ? (NB == 1 ? 3 : 2) : 2;
+  return D == 64 ? (NB <= 2 ? 3 : 2) : D == 128 ? (NB == 1 ? 3 : 2) : 2;
 }
 template <int D> __host__ __device__ constexpr int e4_tile_bytes() { return 32 * D + 32; }
 
@@ -439,7 +439,7 @@ attention_e4m3_rows_kernel(const T* q, int q_stride, T* __restrict__ out, const 
           v = v * rfc[nb][c] * kf;
         }
     }
-    unsigned seen = 0xffffffffu;       // bit nb * 8 + u * 4 + e
+    unsigned seen = 0xffffffffu;       // bit nb * 8 + u * 4 + e (32 of them for NB = 4)
     if (!clear) {
       seen = 0u;
       const bool held[2] = {place_of(i, 0) >= 0, place_of(i, 1) >= 0};
@@ -722,15 +722,16 @@ RLLM_EXPORT int rllm_attention_e4m3_rows(const void* q, int q_stride, void* out,
   return e4_rows_launch<DD, NBB, TT>(q, q_stride, out, kcache, vcache, kscale, vscale, block_table, max_blocks, q_start, \
                                           seq_lens, seq_begin, seq_end - seq_begin, max_q_len, max_keys, nq, nkv, page_size,  \
                                           num_pages, window, scale, err, stream)
-  const bool one = (long long)max_q_len * (nq / nkv) <= 8;
+  // tiles of as many rows as the sequences bring, where registers hold them: every tile reads all keys again
+  const long long rows = (long long)max_q_len * (nq / nkv);
   if (dtype == RLLM_DT_BF16) {
-    if (d == 64) { if (one) E4_ROWS(64, 1, bf16); E4_ROWS(64, 2, bf16); }
-    if (d == 128) { if (one) E4_ROWS(128, 1, bf16); E4_ROWS(128, 2, bf16); }
+    if (d == 64) { if (rows <= 8) E4_ROWS(64, 1, bf16); if (rows <= 16) E4_ROWS(64, 2, bf16); if (rows <= 24) E4_ROWS(64, 3, bf16); E4_ROWS(64, 4, bf16); }
+    if (d == 128) { if (rows <= 8) E4_ROWS(128, 1, bf16); if (rows <= 16) E4_ROWS(128, 2, bf16); E4_ROWS(128, 3, bf16); }
     E4_ROWS(256, 1, bf16);
   }
   if (dtype == RLLM_DT_F32) {
-    if (d == 64) { if (one) E4_ROWS(64, 1, float); E4_ROWS(64, 2, float); }
-    if (d == 128) { if (one) E4_ROWS(128, 1, float); E4_ROWS(128, 2, float); }
+    if (d == 64) { if (rows <= 8) E4_ROWS(64, 1, float); E4_ROWS(64, 2, float); }
+    if (d == 128) { if (rows <= 8) E4_ROWS(128, 1, float); E4_ROWS(128, 2, float); }
     E4_ROWS(256, 1, float);
   }
   return RLLM_E_BADARG;

@@ -7,8 +7,10 @@
 //   warps 0-3   softmax, a thread a row (= TMEM lane): scores from TMEM, mask, running reference and sum in float32, weights as
 //               halves back into TMEM; the output stays in TMEM and is rescaled when a reference moves.  Warps without a live
 //               row only keep the barriers in step: a few rows cost the exponentials of 32.
-//   warps 4-7   widen: 16 bytes of a row a lane, two tiles ahead of their use in registers, to halves in shared memory, in the
-//               128-byte swizzle that the products read.
+//   warps 4-7   widen: copy two tiles of rows ahead into shared memory (a lane its own 16 bytes, asynchronously), and make halves of
+//               them there, in the 128-byte swizzle that the products read.
+//   warp 9      looks ahead: where the rows of a tile lie, their scales, the tile's largest, as factors and notes for the others
+//               (done by every widening warp for itself it was a third of their time: long chains of short instructions).
 //   warp 8      allocates TMEM and issues the products: S = Q K^T (128 x 64 x D), O += P V (128 x D x 64, P in TMEM, V as the
 //               MN-major operand, straight from its rows).
 // Halves, not bfloat16: e4m3 numbers become halves in one instruction a pair, and a weight keeps 11 bits.  Powers of two:
@@ -25,21 +27,27 @@
 
 #define E8_BM 128
 #define E8_BN 64
-#define E8_THREADS 288
+#define E8_THREADS 320
+#define E8_AHEAD 8                   // tiles whose rows and factors are known at a time
 #define E8_SLACK 4.0f
 #define E8_SHIFT 7
 
-// Q, two stages of K and of V, barriers and the stages' notes
-template <int D> constexpr int e8_smem_bytes() { return E8_BM * D * 2 + 4 * E8_BN * D * 2 + 512; }
+// Q, the widened stages of K and of V (two each for heads of 64, one for 128: two CTAs fit one SM), two tiles of K and of V as
+// they come, barriers and the tiles' notes
+template <int D> constexpr int e8_stages() { return D == 64 ? 2 : 1; }
+template <int D> constexpr int e8_smem_bytes() { return E8_BM * D * 2 + 2 * e8_stages<D>() * E8_BN * D * 2 + 4 * E8_BN * D + 512 + E8_AHEAD * 1024; }
 
-// what the widening warps tell the softmax warps of a tile
-struct E8Note {
+// what warp 9 finds out about a tile
+struct E8Tile {
+  int row[E8_BN];                    // a key's cache row; -1: not to be read, or of a page that is not held
+  unsigned kf[E8_BN], vf[E8_BN];     // 2^(ek - EK) and 2^(ev - EV') as pairs of halves
   int ek;                            // EK, a scale byte
   int shift;                         // EV' - reference
   int ref;                           // the reference, a scale byte
   int drop;                          // the one before - it (0: it has not moved, or there was none)
   unsigned missing[2];               // a bit a key whose page is not held
 };
+static_assert(sizeof(E8Tile) <= 1024, "they lie behind the barriers");
 
 template <int D>
 __global__ void __launch_bounds__(E8_THREADS, 2)
@@ -48,7 +56,7 @@ attention_e4m3_tcgen05_kernel(const bf16* q, int q_stride, bf16* __restrict__ ou
                               const unsigned char* __restrict__ vscale, const int* __restrict__ block_table, int max_blocks,
                               const int* __restrict__ q_start, const int* __restrict__ seq_lens, int seq_begin, int nq, int nkv,
                               int page_size, int num_pages, int window, float scale_log2, int* __restrict__ err) {
-  constexpr int DP = D / 64, QPANEL = E8_BM * 128, KPANEL = E8_BN * 128, STAGE = E8_BN * D * 2;
+  constexpr int DP = D / 64, QPANEL = E8_BM * 128, KPANEL = E8_BN * 128, STAGE = E8_BN * D * 2, NS = e8_stages<D>();
   extern __shared__ __align__(1024) unsigned char e8_raw[];
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int splits = gridDim.x, rank = blockIdx.x;       // the cluster is the grid's x
@@ -67,12 +75,13 @@ attention_e4m3_tcgen05_kernel(const bf16* q, int q_stride, bf16* __restrict__ ou
   const int kmin = window > 0 ? max(0, first_pos - window + 1) : 0;
   const int all_lo = kmin / E8_BN, all = max(0, (kend + E8_BN - 1) / E8_BN - all_lo);
   const int tile_lo = all_lo + all * rank / splits, ntiles = all_lo + all * (rank + 1) / splits - tile_lo;
-  unsigned char *sQ = e8_raw, *sK = sQ + DP * QPANEL, *sV = sK + 2 * STAGE;
-  unsigned long long* bars = (unsigned long long*)(sV + 2 * STAGE);
+  unsigned char *sQ = e8_raw, *sK = sQ + DP * QPANEL, *sV = sK + NS * STAGE, *sRaw = sV + NS * STAGE;
+  unsigned long long* bars = (unsigned long long*)(sRaw + 4 * E8_BN * D);
   unsigned long long *k_full = bars, *k_empty = bars + 2, *v_full = bars + 4, *v_empty = bars + 6;      // [2] each
   unsigned long long *s_full = bars + 8, *p_full = bars + 10, *pv_full = bars + 11;                     // s_full: [2]
   unsigned* tmem_slot = (unsigned*)(bars + 12);
-  E8Note* notes = (E8Note*)(bars + 13);                  // [4]: the softmax of a tile may be two behind its widening
+  unsigned long long *t_full = bars + 16, *t_free = bars + 16 + E8_AHEAD;               // [E8_AHEAD] each
+  E8Tile* tiles = (E8Tile*)((unsigned char*)bars + 512);  // [E8_AHEAD]
   const int* bt = block_table + (size_t)s * max_blocks;
   const int page_shift = (page_size & (page_size - 1)) == 0 ? __ffs(page_size) - 1 : -1;
 
@@ -82,20 +91,13 @@ attention_e4m3_tcgen05_kernel(const bf16* q, int q_stride, bf16* __restrict__ ou
     mbar_init(&s_full[1], 1);
     mbar_init(p_full, 4);
     mbar_init(pv_full, 1);
+    for (int i = 0; i < E8_AHEAD; ++i) { mbar_init(&t_full[i], 1); mbar_init(&t_free[i], 8); }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 8) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tg_smem(tmem_slot)), "r"(256) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
-  // where the keys lane and lane + 32 of a tile lie: their cache rows, -1 for those outside [kmin, kend) or of pages not held
-  auto page_of = [&](int it, int h) {
-    const int j = (tile_lo + it) * E8_BN + h * 32 + lane;
-    if (it >= ntiles || j < kmin || j >= kend) return -2;                 // not read
-    return bt[page_shift >= 0 ? j >> page_shift : j / page_size];
-  };
-  int page_next[2] = {-2, -2};
-  if (warp >= 4 && warp < 8) { page_next[0] = page_of(0, 0); page_next[1] = page_of(0, 1); }
   pdl_wait_on(q, kcache, vcache, kscale, vscale);
 
   // Queries as halves: a row by 2^(13 - e) with 2^e its largest's power; eight lanes a row (four for heads of 64)
@@ -162,7 +164,13 @@ attention_e4m3_tcgen05_kernel(const bf16* q, int q_stride, bf16* __restrict__ ou
       ok = __all_sync(0xffffffffu, mbar_wait(&s_full[it & 1], (it >> 1) & 1, err));
       if (!ok) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      const E8Note note = notes[it & 3];
+      struct { int ek, shift, ref, drop; unsigned missing[2]; } note;
+      {
+        const E8Tile& x = tiles[it % E8_AHEAD];
+        note = {x.ek, x.shift, x.ref, x.drop, {x.missing[0], x.missing[1]}};
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&t_free[it % E8_AHEAD]);
       ref = note.ref;
       if (!warp_live) {
         if (it > 0) {
@@ -209,24 +217,6 @@ attention_e4m3_tcgen05_kernel(const bf16* q, int q_stride, bf16* __restrict__ ou
       }
       const bool dropped = note.drop != 0;
       if (dropped) corr *= note.drop < -126 ? 0.f : __uint_as_float((unsigned)(127 + note.drop) << 23);
-      // the product of the tile before has to be through: it wrote the output that is rescaled here
-      if (it > 0) {
-        ok = __all_sync(0xffffffffu, mbar_wait(pv_full, (it - 1) & 1, err));
-        if (!ok) break;
-        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        if (__any_sync(0xffffffffu, moves || dropped)) {
-#pragma unroll
-          for (int c0 = 0; c0 < D; c0 += 32) {
-            unsigned* v = (unsigned*)sc;
-            tmem_ld32(tmem_o + lane_sel + c0, v);
-            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) * corr);
-            tmem_st32(tmem_o + lane_sel + c0, v);
-          }
-          asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-        }
-      }
       // weights times 2^(EV' - reference + 7), in the place of the scores, and the sum without that factor
       const float up = (float)(note.shift + E8_SHIFT), m_safe = ((m_ref == -INFINITY) ? 0.f : m_ref) - up;
       const unsigned long long scale2 = at_pack2(f, f), shift2 = at_pack2(-m_safe, -m_safe);
@@ -255,6 +245,24 @@ attention_e4m3_tcgen05_kernel(const bf16* q, int q_stride, bf16* __restrict__ ou
         at_unpack2(sum01, a, b);
         at_unpack2(sum23, c, d);
         l = fmaf((a + b) + (c + d), at_ex2(-up), l);
+      }
+      // the product of the tile before has to be through: it wrote the output that is rescaled here
+      if (it > 0) {
+        ok = __all_sync(0xffffffffu, mbar_wait(pv_full, (it - 1) & 1, err));
+        if (!ok) break;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        if (__any_sync(0xffffffffu, moves || dropped)) {
+#pragma unroll
+          for (int c0 = 0; c0 < D; c0 += 32) {
+            unsigned* v = (unsigned*)sc;
+            tmem_ld32(tmem_o + lane_sel + c0, v);
+            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) * corr);
+            tmem_st32(tmem_o + lane_sel + c0, v);
+          }
+          asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+        }
       }
       asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -315,105 +323,169 @@ attention_e4m3_tcgen05_kernel(const bf16* q, int q_stride, bf16* __restrict__ ou
     }
   } else if (warp < 8) {
     // ---- widening ----
-    constexpr int L = D / 16, ROWS = 32 / L, STEPS = E8_BN / (4 * ROWS);       // lanes a row, a warp's rows a step, steps a tile
-    const int w = warp - 4, c = lane % L, rl = lane / L;
-    // Of the next tile: rows of the cache of keys lane and lane + 32, their scales, which of them are missing.  Its numbers are asked
-    // for as soon as this tile's are widened, keys and values in turn.
-    int row_n[2] = {-1, -1}, kb_n[2] = {0, 0}, vb_n[2] = {0, 0};
-    unsigned miss_n[2] = {0u, 0u};
-    uint4 kx[STEPS], vx[STEPS];
+    // Four lanes a row and panel of 64 dims, 16 numbers each: a warp's step is 8 rows of a panel, so that a lane's place in the
+    // swizzle does not change, and its two 16-byte stores meet no other's banks.  Warp w has rows 8 w .. 8 w + 7 of either half.
+    const int w = warp - 4, c = lane & 3, rl = lane >> 2;
+    const int even = ((2 * c) ^ rl) << 4, place = (w * 8 + rl) * 128;      // r & 7 = rl
+    // A lane's 16 bytes of its rows of a tile, on their way; [tile & 1][K, V][half][panel][lane] of this warp's.  Copies go out two
+    // tiles ahead, keys and values as groups of their own.
+    constexpr int PART = 2 * DP * 512;                     // bytes of a tile's K (or V) of this warp
+    const unsigned char* const mine = sRaw + w * 4 * PART + lane * 16;
+    const unsigned raw = tg_smem(mine);
+    // the cache rows of this lane's two rows of a tile
+    auto rows_of = [&](int it, int (&at)[2]) {
+      if (it >= ntiles) return true;
+      if (!__all_sync(0xffffffffu, mbar_wait(&t_full[it % E8_AHEAD], (it / E8_AHEAD) & 1, err))) return false;
+      at[0] = tiles[it % E8_AHEAD].row[w * 8 + rl];
+      at[1] = tiles[it % E8_AHEAD].row[32 + w * 8 + rl];
+      return true;
+    };
+    auto copy = [&](int it, int which, const unsigned char* cache, const int (&at)[2]) {
+      if (it < ntiles) {
+        const unsigned dst = raw + ((it & 1) * 2 + which) * PART;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const unsigned char* src = cache + (at[h] >= 0 ? (long long)at[h] * D + c * 16 : 0);
+          const int n = at[h] >= 0 ? 16 : 0;
+#pragma unroll
+          for (int dp = 0; dp < DP; ++dp)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + (h * DP + dp) * 512), "l"(src + dp * 64), "r"(n) : "memory");
+        }
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    // this lane's numbers of half h of a tile times `power`, into their places
+    auto widen = [&](unsigned char* tile, int it, int which, int h, unsigned factor) {
+      const __half2 p2 = *(const __half2*)&factor;
+#pragma unroll
+      for (int dp = 0; dp < DP; ++dp) {
+        const uint4 x = *(const uint4*)(mine + ((it & 1) * 2 + which) * PART + (h * DP + dp) * 512);
+        uint4 y[2];
+        __half2* z = (__half2*)y;
+        const unsigned u[8] = {kv8_halves_lo(x.x), kv8_halves_hi(x.x), kv8_halves_lo(x.y), kv8_halves_hi(x.y),
+                               kv8_halves_lo(x.z), kv8_halves_hi(x.z), kv8_halves_lo(x.w), kv8_halves_hi(x.w)};
+#pragma unroll
+        for (int i = 0; i < 8; ++i) z[i] = __hmul2(*(const __half2*)&u[i], p2);
+        unsigned char* dst = tile + dp * KPANEL + h * 4096 + place;
+        *(uint4*)(dst + even) = y[0];
+        *(uint4*)(dst + (even ^ 16)) = y[1];
+      }
+    };
+    // Where there is one place for widened values, they wait for the product of the tile before, and the next tile's keys are
+    // widened meanwhile: K0 K1 V0 K2 V1 K3 ... (64 sequences of 8,000 keys, heads of 128: 452 -> 359 us); else K0 V0 K1 V1 ...
+    // (heads of 64: 276 us, in the other order 299).  Each makes room for its copy two tiles on.
+    auto keys = [&](int it, const int (&next)[2]) {
+      const int st = it % NS;
+      if (!__all_sync(0xffffffffu, mbar_wait(&k_empty[st], (unsigned)((it / NS) & 1) ^ 1u, err))) return false;
+      const E8Tile& x = tiles[it % E8_AHEAD];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) widen(sK + st * STAGE, it, 0, h, x.kf[h * 32 + w * 8 + rl]);
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&k_full[st]);
+      copy(it + 2, 0, kcache, next);
+      return true;
+    };
+    auto values = [&](int it, const int (&next)[2]) {
+      const int st = it % NS;
+      if (!__all_sync(0xffffffffu, mbar_wait(&v_empty[st], (unsigned)((it / NS) & 1) ^ 1u, err))) return false;
+      const E8Tile& x = tiles[it % E8_AHEAD];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) widen(sV + st * STAGE, it, 1, h, x.vf[h * 32 + w * 8 + rl]);
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) { mbar_arrive(&v_full[st]); mbar_arrive(&t_free[it % E8_AHEAD]); }
+      copy(it + 2, 1, vcache, next);
+      return true;
+    };
+    int a0[2] = {-1, -1}, a1[2] = {-1, -1}, a2[2] = {-1, -1}, a3[2] = {-1, -1};
+    ok = rows_of(0, a0) && rows_of(1, a1);
+    copy(0, 0, kcache, a0);
+    copy(0, 1, vcache, a0);
+    copy(1, 0, kcache, a1);
+    copy(1, 1, vcache, a1);
+    if constexpr (NS == 2) {
+      // (every tile commits a group of keys and one of values, two tiles ahead: three lie behind the one that is waited for)
+      for (int it = 0; it < ntiles && ok; ++it) {
+        ok = rows_of(it + 2, a2);
+        asm volatile("cp.async.wait_group 3;" ::: "memory");
+        ok = ok && keys(it, a2);
+        asm volatile("cp.async.wait_group 3;" ::: "memory");
+        ok = ok && values(it, a2);
+      }
+    } else {
+      ok = ok && rows_of(2, a2);
+      asm volatile("cp.async.wait_group 3;" ::: "memory");
+      if (ntiles > 0) ok = ok && keys(0, a2);
+      for (int it = 0; it < ntiles && ok; ++it) {
+        // the keys of tile it + 1: behind their group lie the next keys' and one of values at most (no group is left out but
+        // behind the last tile's, whose values' group all of these waits then cover)
+        ok = rows_of(it + 3, a3);
+        asm volatile("cp.async.wait_group 2;" ::: "memory");
+        if (it + 1 < ntiles) ok = ok && keys(it + 1, a3);
+        asm volatile("cp.async.wait_group 3;" ::: "memory");
+        ok = ok && values(it, a2);
+        a2[0] = a3[0]; a2[1] = a3[1];
+      }
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+  } else if (warp == 9) {
+    // ---- looking ahead: keys lane and lane + 32 of a tile ----
+    // No condition stands around a load: a value that is chosen between a load's result and a constant is waited for where it is
+    // chosen.  The block table's entries are asked for two tiles ahead, scales one.
+    auto page_of = [&](int it, int h) {
+      const int j = max((tile_lo + it) * E8_BN + h * 32 + lane, 0);
+      return bt[min(page_shift >= 0 ? j >> page_shift : j / page_size, max_blocks - 1)];
+    };
+    int page[2] = {page_of(0, 0), page_of(0, 1)}, row[2], kb[2], vb[2];
+    unsigned miss[2], readable[2];
     auto rows_of = [&](int it) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const int page = page_next[h], j = (tile_lo + it) * E8_BN + h * 32 + lane;
-        const bool bad = page != -2 && (page < 0 || page >= num_pages);
-        if (bad && w == 0) atomicOr(err, 4);
-        miss_n[h] = __ballot_sync(0xffffffffu, bad);
-        row_n[h] = (page == -2 || bad) ? -1 : (page * nkv + kvh) * page_size + (page_shift >= 0 ? j & (page_size - 1) : j % page_size);
-        kb_n[h] = row_n[h] >= 0 ? kscale[row_n[h]] : 0;
-        vb_n[h] = row_n[h] >= 0 ? vscale[row_n[h]] : 0;
-        page_next[h] = page_of(it + 1, h);
+        const int j = (tile_lo + it) * E8_BN + h * 32 + lane;
+        const bool wanted = j >= kmin && j < kend, bad = wanted && (page[h] < 0 || page[h] >= num_pages), read = wanted && !bad;
+        miss[h] = __ballot_sync(0xffffffffu, bad);
+        readable[h] = __ballot_sync(0xffffffffu, read);
+        if (miss[h] && bad) atomicOr(err, 4);
+        row[h] = read ? (page[h] * nkv + kvh) * page_size + (page_shift >= 0 ? j & (page_size - 1) : j % page_size) : -1;
+        kb[h] = kscale[max(row[h], 0)];
+        vb[h] = vscale[max(row[h], 0)];
+        page[h] = page_of(it + 1, h);
       }
     };
-    auto fetch = [&](uint4 (&x)[STEPS], const unsigned char* cache) {
-#pragma unroll
-      for (int i = 0; i < STEPS; ++i) {
-        const int r = (i * 4 + w) * ROWS + rl;
-        const int at = __shfl_sync(0xffffffffu, i * 4 * ROWS >= 32 ? row_n[1] : row_n[0], r & 31);
-        x[i] = at >= 0 ? *(const uint4*)(cache + (long long)at * D + c * 16) : make_uint4(0u, 0u, 0u, 0u);
-      }
+    auto factor = [&](int b, int top) {                    // 2^(b - top) twice, as halves
+      const __half2 p = __float2half2_rn(b - top < -30 ? 0.f : __uint_as_float((unsigned)(127 + b - top) << 23));
+      return *(const unsigned*)&p;
     };
-    // 16 numbers times 2^(b - top) into their places of a tile
-    auto widen = [&](unsigned char* tile, const uint4& raw, int r, float power) {
-      const __half2 p2 = __float2half2_rn(power);
-      const unsigned x[4] = {raw.x, raw.y, raw.z, raw.w};
-      uint4 y[2];
-      __half2* h = (__half2*)y;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const unsigned lo = kv8_halves_lo(x[i]), hi = kv8_halves_hi(x[i]);
-        h[2 * i] = __hmul2(*(const __half2*)&lo, p2);
-        h[2 * i + 1] = __hmul2(*(const __half2*)&hi, p2);
-      }
-      // (the two stores of neighbouring panels' lanes in turn: their banks then do not meet)
-      unsigned char* dst = tile + (c >> 2) * KPANEL + r * 128;
-      const int even = (((c & 3) * 2) ^ (r & 7)) << 4, odd = even ^ 16, first = (c >> 2) & 1;
-      *(uint4*)(dst + (first ? odd : even)) = first ? y[1] : y[0];
-      *(uint4*)(dst + (first ? even : odd)) = first ? y[0] : y[1];
-    };
-    auto power_at = [&](int b, int top) { return b - top < -30 ? 0.f : __uint_as_float((unsigned)(127 + b - top) << 23); };
-    if (ntiles > 0) {
-      rows_of(0);
-      fetch(kx, kcache);
-      fetch(vx, vcache);
-    }
-    for (int it = 0; it < ntiles && ok; ++it) {
-      const int st = it & 1;
-      int kb[2] = {kb_n[0], kb_n[1]}, vb[2] = {vb_n[0], vb_n[1]};
-      const unsigned miss[2] = {miss_n[0], miss_n[1]};
-      if (it + 1 < ntiles) rows_of(it + 1);
+    rows_of(0);
+    for (int it = 0; it < ntiles; ++it) {
+      int r[2] = {row[0], row[1]}, k[2] = {kb[0], kb[1]}, v[2] = {vb[0], vb[1]};
+      const unsigned ms[2] = {miss[0], miss[1]}, rd[2] = {readable[0], readable[1]};
       int kt = 0, vt = 0;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const bool odd = kb[h] == KV8_NAN_SCALE || vb[h] == KV8_NAN_SCALE;
-        if (odd) { kb[h] = KV8_NAN_SCALE; vb[h] = 0; }
-        else { kt = max(kt, kb[h]); vt = max(vt, vb[h]); }
+        if (!(rd[h] >> lane & 1u)) k[h] = v[h] = 0;
+        if (k[h] == KV8_NAN_SCALE || v[h] == KV8_NAN_SCALE) { k[h] = KV8_NAN_SCALE; v[h] = 0; }
+        else { kt = max(kt, k[h]); vt = max(vt, v[h]); }
       }
       kt = __reduce_max_sync(0xffffffffu, kt);
       vt = __reduce_max_sync(0xffffffffu, vt);
-      // the reference of the values' powers: the same walk in every widening warp
+      rows_of(it + 1);
       int drop = 0;
       if (ref < 0) ref = vt;
       else if ((float)vt > (float)ref + E8_SLACK) { drop = ref - vt; ref = vt; }
       const int eff = max(vt, ref - 30);
-      ok = __all_sync(0xffffffffu, mbar_wait(&k_empty[st], ((it >> 1) & 1) ^ 1, err));
-      if (!ok) break;
-      if (w == 0 && lane == 0) {
-        E8Note* n = &notes[it & 3];
-        n->ek = kt; n->shift = eff - ref; n->ref = ref; n->drop = drop; n->missing[0] = miss[0]; n->missing[1] = miss[1];
-      }
+      if (!__all_sync(0xffffffffu, mbar_wait(&t_free[it % E8_AHEAD], ((it / E8_AHEAD) & 1) ^ 1, err))) break;
+      E8Tile& x = tiles[it % E8_AHEAD];
 #pragma unroll
-      for (int i = 0; i < STEPS; ++i) {
-        const int r = (i * 4 + w) * ROWS + rl;
-        const int b = __shfl_sync(0xffffffffu, i * 4 * ROWS >= 32 ? kb[1] : kb[0], r & 31);
-        widen(sK + st * STAGE, kx[i], r, b == KV8_NAN_SCALE ? __uint_as_float(0x7FC00000u) : power_at(b, kt));
+      for (int h = 0; h < 2; ++h) {
+        x.row[h * 32 + lane] = r[h];
+        x.kf[h * 32 + lane] = k[h] == KV8_NAN_SCALE ? 0x7E007E00u : factor(k[h], kt);
+        x.vf[h * 32 + lane] = factor(v[h], eff);
       }
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      if (lane == 0) { x.ek = kt; x.shift = eff - ref; x.ref = ref; x.drop = drop; x.missing[0] = ms[0]; x.missing[1] = ms[1]; }
       __syncwarp();
-      if (lane == 0) mbar_arrive(&k_full[st]);
-      if (it + 1 < ntiles) fetch(kx, kcache);
-      ok = __all_sync(0xffffffffu, mbar_wait(&v_empty[st], ((it >> 1) & 1) ^ 1, err));
-      if (!ok) break;
-#pragma unroll
-      for (int i = 0; i < STEPS; ++i) {
-        const int r = (i * 4 + w) * ROWS + rl;
-        const int b = __shfl_sync(0xffffffffu, i * 4 * ROWS >= 32 ? vb[1] : vb[0], r & 31);
-        widen(sV + st * STAGE, vx[i], r, power_at(b, eff));
-      }
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&v_full[st]);
-      if (it + 1 < ntiles) fetch(vx, vcache);
+      if (lane == 0) mbar_arrive(&t_full[it % E8_AHEAD]);
     }
   } else {
     // ---- products ---- (float32 accumulate, halves; the whole warp walks, one lane issues: see attention_tcgen05.cu)
@@ -424,18 +496,18 @@ attention_e4m3_tcgen05_kernel(const bf16* q, int q_stride, bf16* __restrict__ ou
     auto wait = [&](unsigned long long* bar, unsigned parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity, err)) != 0; };
     // scores of tile it into its half of the score columns, where the weights of the tile two before were
     auto scores = [&](int it) {
-      const int st = it & 1;
+      const int st = it % NS, half = it & 1;
       const unsigned long long dk = umma_desc(sK + st * STAGE);
-      if (!wait(&k_full[st], (it >> 1) & 1)) return false;
+      if (!wait(&k_full[st], (it / NS) & 1)) return false;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       if (umma_elect()) {
 #pragma unroll
         for (int k = 0; k < D / 16; ++k) {
           const unsigned long long a = dq + (unsigned long long)((k >> 2) * (QPANEL >> 4) + 2 * (k & 3));
           const unsigned long long b = dk + (unsigned long long)((k >> 2) * (KPANEL >> 4) + 2 * (k & 3));
-          umma_bf16(tmem_s + st * E8_BN, a, b, idesc_s, k != 0);
+          umma_bf16(tmem_s + half * E8_BN, a, b, idesc_s, k != 0);
         }
-        umma_commit(&s_full[st]);
+        umma_commit(&s_full[half]);
         umma_commit(&k_empty[st]);
       }
       __syncwarp();
@@ -443,15 +515,15 @@ attention_e4m3_tcgen05_kernel(const bf16* q, int q_stride, bf16* __restrict__ ou
     };
     bool go = n > 0 && scores(0) && (n < 2 || scores(1));
     for (int it = 0; it < n && go; ++it) {
-      const int st = it & 1;
-      go = wait(&v_full[st], (it >> 1) & 1) && wait(p_full, it & 1);
+      const int st = it % NS;
+      go = wait(&v_full[st], (it / NS) & 1) && wait(p_full, it & 1);
       if (!go) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       const unsigned long long dv = (umma_desc(sV + st * STAGE) & ~(0x3FFFull << 16)) | ((unsigned long long)(KPANEL >> 4) << 16);
       if (umma_elect()) {
 #pragma unroll
         for (int kk = 0; kk < E8_BN / 16; ++kk)
-          umma_bf16_tmem_a(tmem_o, tmem_s + st * E8_BN + kk * 8, dv + (unsigned long long)(kk * (2048 >> 4)), idesc_pv, (it != 0) || (kk != 0));
+          umma_bf16_tmem_a(tmem_o, tmem_s + (it & 1) * E8_BN + kk * 8, dv + (unsigned long long)(kk * (2048 >> 4)), idesc_pv, (it != 0) || (kk != 0));
         umma_commit(pv_full);
         umma_commit(&v_empty[st]);
       }

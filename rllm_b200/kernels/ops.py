@@ -2167,16 +2167,26 @@ def e4m3_dense_scratch(nkv: int, d: int, max_seq_len: int) -> int:
     return max(E4M3_DENSE_SCRATCH, 4 * (max_seq_len // bn + 2) * nkv * bn * d)
 
 
-def attention_e4m3_form(dtype: torch.dtype, nq: int, nkv: int, d: int, page_size: int, scale: float, max_q_len: int) -> str:
-    """Which kernel takes sequences of up to ``max_q_len`` tokens: "rows" (mma.sync, 16 rows of a kv head at a time), "tcgen05"
-    (128 rows, keys and values widened inside), "dense" (tcgen05 over keys and values widened once for all rows), or "simt"."""
+def attention_e4m3_form(dtype: torch.dtype, nq: int, nkv: int, d: int, page_size: int, scale: float, max_q_len: int,
+                        num_seqs: int, max_keys: int) -> str:
+    """Which kernel takes ``num_seqs`` sequences of up to ``max_q_len`` tokens whose queries see up to ``max_keys`` keys: "rows"
+    (mma.sync, up to 32 rows of a kv head at a time; a row is a token and a head of the kv head's group), "tcgen05" (128 rows,
+    keys and values widened inside), "dense" (tcgen05 over keys and values widened once for all tiles of rows), "simt".
+
+    Measured (microseconds; 8 kv heads with four heads each):
+      rows / tcgen05, heads of 64: 8 sequences of 16,000 keys, 32 rows 72 / 81, 48 rows 138 / 82; one of 4,000, 128 rows 15 / 18;
+        heads of 128: 8 of 16,000, 24 rows 95 / 101, 32 rows 181 / 101; one of 1,000, 64 rows 12 / 15, of 16,000, 128 rows 90 / 48;
+      tcgen05 / dense, heads of 64: 4 of 16,000, 4 tiles of 128 rows 182 / 240, 6 tiles 340 / 287, 16 tiles 682 / 518; heads of
+        128: 216 / 353, 406 / 381, 798 / 666."""
     g, forced = nq // nkv, os.environ.get("RLLM_ATTENTION")
+    rows_take = d in (64, 128, 256) and page_size % 16 == 0 and forced != "simt"
     if dtype is torch.bfloat16 and d in (64, 128) and g <= 128 and scale > 0 and forced not in ("simt", "mma"):
-        if max_q_len * g >= 96:
-            return "dense"
-    if d in (64, 128, 256) and page_size % 16 == 0 and forced != "simt":
-        return "rows"
-    return "simt"
+        most = 32 if d == 64 else 24
+        tiles = -(-max_q_len * g // most)
+        few = tiles == 1 or (num_seqs * nkv * tiles <= 32 and (d == 64 or max_keys <= 2048))
+        if not (few and rows_take):
+            return "tcgen05" if -(-max_q_len // (128 // g)) <= 4 else "dense"
+    return "rows" if rows_take else "simt"
 
 
 def attention_e4m3(q: torch.Tensor, out: torch.Tensor, kcache: torch.Tensor, vcache: torch.Tensor, kscale: torch.Tensor,
@@ -2212,7 +2222,7 @@ def attention_e4m3(q: torch.Tensor, out: torch.Tensor, kcache: torch.Tensor, vca
     for first, end, longest in ((0, num_decode, 1), (num_decode, S, max_q_len)):
         if first == end or longest == 0:
             continue
-        form = attention_e4m3_form(q.dtype, nq, nkv, d, page_size, scale, longest)
+        form = attention_e4m3_form(q.dtype, nq, nkv, d, page_size, scale, longest, end - first, keys)
         if form in ("tcgen05", "dense") and (stride % 8 or (q.data_ptr() | out.data_ptr()) % 16):
             form = "rows" if page_size % 16 == 0 else "simt"
         if form == "rows":

@@ -236,6 +236,80 @@ def test_pages_that_are_not_held_are_left_out_and_reported(dtype, lens, starts):
         st.check(out)
 
 
+FORMS = ["rows", "tcgen05", "dense"]
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("nq,nkv,d,page,lens,starts,window", [
+    (4, 4, 64, 16, [1], [0], 0), (32, 8, 64, 16, [40], [3000], 0), (32, 8, 128, 16, [33, 1, 7], [2500, 64, 0], 0), (8, 2, 64, 16, [64], [0], 0),
+    (8, 8, 128, 32, [127, 129], [1, 63], 0), (24, 8, 128, 16, [43, 42], [64, 65], 0), (32, 1, 64, 16, [9], [500], 70), (16, 2, 128, 64, [100], [300], 1),
+    (8, 1, 128, 16, [20, 50], [1000, 10], 128), (40, 8, 64, 16, [30], [90], 0), (5, 1, 128, 48, [28], [200], 33), (128, 1, 64, 16, [2], [200], 0)])
+def test_every_form_of_the_attention(form, nq, nkv, d, page, lens, starts, window, monkeypatch):
+    monkeypatch.setattr(ops, "attention_e4m3_form", lambda *a: form)
+    for spread, qscale in ((1.0, 1.0), (3.0, 0.3)):
+        st = Step(lens, starts, nq, nkv, d, page, BF16, seed=nq + d, more_rows=2, stride_pad=16, spread=spread, qscale=qscale)
+        out = st.attend(ops, window, num_decode=0)
+        assert int(st.err) == 0 and (out[sum(lens):] == 7).all()
+        st.check(out, window)
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("lens,starts", [([5], [100]), ([3, 150], [40, 30]), ([70, 2], [200, 1000])])
+def test_keys_that_are_nan_missing_or_out_of_sight_in_every_form(form, d, lens, starts, monkeypatch):
+    monkeypatch.setattr(ops, "attention_e4m3_form", lambda *a: form)
+    s, n = len(lens) - 1, lens[-1]
+    for where in (0, 1):                                          # a key, a value that is NaN, of a token of the step
+        st = Step(lens, starts, 8, 2, d, 16, BF16, seed=4)
+        j = starts[s] + n // 2
+        scale, codes = (st.ks, st.k) if where == 0 else (st.vs, st.v)
+        scale.view(torch.uint8)[int(st.table[s, j // 16]), where, j % 16] = 255
+        codes.view(torch.uint8)[int(st.table[s, j // 16]), where, j % 16] = 0
+        out = st.attend(ops, num_decode=0)
+        st.check(out)
+        assert torch.isnan(out[:sum(lens)]).any() and not torch.isnan(out[:sum(lens[:s]) + n // 2]).any()
+    st = Step(lens, starts, 8, 2, d, 16, BF16, seed=5)            # pages that are not held
+    st.table[s, 1], st.table[s, 2] = -1, st.pages
+    out = st.attend(ops, num_decode=0)
+    assert int(st.err) == 4
+    st.check(out)
+    for window in (0, 50):                                        # NaN behind the sequence's end and ahead of the window
+        st = Step(lens, starts, 8, 2, d, 16, BF16, seed=6)
+        plain = st.attend(ops, window, num_decode=0)
+        for i, m in enumerate(st.totals):
+            last = int(st.table[i, (m - 1) // 16])
+            first = int(st.table[i, 0]) if window and m - lens[i] - window > 16 else None
+            for t in (st.k, st.v, st.ks, st.vs):
+                t.view(torch.uint8)[last, :, (m - 1) % 16 + 1:] = 255
+                if first is not None:
+                    t.view(torch.uint8)[first] = 255
+        out = st.attend(ops, window, num_decode=0)
+        assert torch.equal(out, plain) and not torch.isnan(out).any() and int(st.err) == 0
+
+
+@pytest.mark.parametrize("form", FORMS)
+def test_rows_that_are_zeros_in_every_form(form, monkeypatch):
+    """Queries, keys and values of zeros (the least scales of all), alone and beside others."""
+    monkeypatch.setattr(ops, "attention_e4m3_form", lambda *a: form)
+    st = Step([40, 3], [100, 200], 8, 2, 64, 16, BF16, seed=7)
+    st.q[::3] = 0
+    for t in (st.k, st.v, st.ks, st.vs):
+        t.view(torch.uint8)[int(st.table[0, 2])] = 0
+        t.view(torch.uint8)[st.table[1, :13].long()] = 0
+    out = st.attend(ops, num_decode=0)
+    st.check(out)
+    assert (out[40:43] == 0).all()
+
+
+def test_prompts_in_groups_of_what_the_scratch_holds(monkeypatch):
+    monkeypatch.setattr(ops, "attention_e4m3_form", lambda *a: "dense")
+    st = Step([40, 3, 70, 9], [100, 200, 0, 30], 8, 2, 64, 16, BF16, seed=7)
+    whole = st.attend(ops, num_decode=0)
+    monkeypatch.setattr(ops, "E4M3_DENSE_SCRATCH", 1)              # a sequence at a time
+    assert torch.equal(st.attend(ops, num_decode=0), whole) and int(st.err) == 0
+    st.check(whole)
+
+
 def test_a_sequence_all_of_whose_pages_are_missing_gives_zeros():
     for lens, starts in (([1, 1], [60, 30]), ([4, 3], [60, 30]), ([140, 20], [5, 30])):
         st = Step(lens, starts, 4, 2, 64, 16, BF16)
