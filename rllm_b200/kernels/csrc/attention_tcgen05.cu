@@ -39,7 +39,8 @@
 // No cluster, no multicast.
 // The DENSE form reads keys and values that a kernel has widened from a cache kept in 8 bits (attention_e4m3.cu) into bfloat16
 // tiles of BN keys, [sequence][tile][kv head][BN][D], a tile a box; a mark beside a tile says whether it has keys that are NaN
-// (then no exponential goes the polynomial's way, which knows none) or that are missing (then they are masked one by one).
+// (the polynomial for exponentials knows none: the sums of the rows that see one are made NaN by themselves) or that are missing
+// (then they are masked one by one).
 // There, a cluster of CTAs may share a tile of rows, each with a part of the keys; their results are merged through
 // distributed shared memory.
 #include "attention_tcgen05.cuh"
@@ -81,7 +82,8 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                          AtOpts opt, int beside) {
   // beside: the kernel ahead wrote nothing that this one reads or writes (the attention of the tokens that decode), and
   // it lets this one in only when the kernel ahead of it is complete: the two run side by side, and this one ends behind it.
-  if (!beside) pdl_wait();
+  // DENSE: lengths and row ranges are inputs of the step; what the kernel ahead widened is waited for behind the set-up below.
+  if (!beside && !DENSE) pdl_wait();
   constexpr int AT_BN = 8192 / AT_D;              // keys a tile
   constexpr int DP = AT_D / 64;                   // panels of head dims (Q, K, V)
   constexpr int KPANEL = AT_BN * 128;             // bytes of a K or V panel: BN rows of 128 bytes
@@ -123,7 +125,10 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
       left -= n;
     }
   }
-  if (s < 0) return;
+  if (s < 0) {
+    if (DENSE) pdl_wait();                        // (a CTA that exits lets the next kernel in)
+    return;
+  }
   const int qs = q_start[s], qlen = q_start[s + 1] - qs;
   const int pos0 = seq_lens[s] - qlen;
   const int t0 = tile * bq;
@@ -171,6 +176,7 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  if (DENSE) pdl_wait();
   if (!beside) pdl_launch();                       // behind the allocation: see pdl_launch
   const unsigned tmem_s = __shfl_sync(0xffffffffu, *tmem_slot, 0), tmem_o = tmem_s + AT_BN, tmem_p = tmem_o + AT_D;   // BN + D + BN / 2 <= 256 columns
 
@@ -375,6 +381,12 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
         for (int j = 0; j < HC; ++j)
           if (marks[1 + (half * HC + j) / 32] >> (j & 31) & 1u) sc[j] = -INFINITY;
       }
+      if (DENSE && (mark & AT_MARK_NAN)) {             // a visible key that is NaN: the sum becomes it, whatever an exponential makes of it
+        bool odd = false;
+#pragma unroll
+        for (int j = 0; j < HC; ++j) odd = odd || sc[j] != sc[j];
+        if (odd) l = __uint_as_float(0x7FC00000u);
+      }
       float mx0 = fmaxf(sc[0], sc[1]), mx1 = fmaxf(sc[2], sc[3]), mx2 = fmaxf(sc[4], sc[5]), mx3 = fmaxf(sc[6], sc[7]);
 #pragma unroll
       for (int j = 8; j < HC; j += 8) {
@@ -405,11 +417,10 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
       unsigned pk[HC / 2];
       const unsigned long long scale2 = at_pack2(sl2, sl2), shift2 = at_pack2(-m_safe, -m_safe);
       unsigned long long sum01 = at_pack2(0.f, 0.f), sum23 = sum01;
-      const bool exact = DENSE && (mark & AT_MARK_NAN);
 #pragma unroll
       for (int j = 0; j < HC; j += 4) {
         float p0, p1, p2, p3;
-        if (!exact && AT_POLY > 0 && AT_D == 64 && (j / 4) % AT_POLY == AT_POLY - 1) {
+        if (AT_POLY > 0 && AT_D == 64 && (j / 4) % AT_POLY == AT_POLY - 1) {
           at_exp2_poly2(at_fma2(at_pack2(sc[j], sc[j + 1]), scale2, shift2), p0, p1);
           at_exp2_poly2(at_fma2(at_pack2(sc[j + 2], sc[j + 3]), scale2, shift2), p2, p3);
         } else {

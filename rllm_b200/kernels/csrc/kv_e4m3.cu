@@ -28,7 +28,7 @@ kv_e4m3_write_kernel(const T* qkv, T* q_out, long long q_stride, const int* __re
       cs[i] = (float)c;
       cs[half + i] = (float)s;
     } else {
-      kv8_cos_sin(pos, inv_freq[i], &cs[i], &cs[half + i]);
+      rope_cos_sin(pos, inv_freq[i], &cs[i], &cs[half + i]);
     }
   }
   __syncthreads();
@@ -122,7 +122,7 @@ kv_e4m3_write_bf16_kernel(const bf16* qkv, bf16* q_out, long long q_stride, cons
   }
   if (slot < 0 && threadIdx.x == 0) atomicOr(err, 2);
   if (rotary_dim) {
-    for (int i = threadIdx.x; i < H; i += 128) kv8_cos_sin(pos, inv_freq[i], &cs[i], &cs[H + i]);
+    for (int i = threadIdx.x; i < H; i += 128) rope_cos_sin(pos, inv_freq[i], &cs[i], &cs[H + i]);
     __syncthreads();
   }
   float cx[8], sx[8];

@@ -50,17 +50,3 @@ __device__ __forceinline__ void kv8_floats(unsigned four, float* o) {
   const float2 a = __half22float2(*(const __half2*)&lo), b = __half22float2(*(const __half2*)&hi);
   o[0] = a.x; o[1] = a.y; o[2] = b.x; o[3] = b.y;
 }
-
-// Cosine and sine of position * inv_freq as rope_cos_sin has them, with what rounding the reduced angle to float32 leaves behind
-// put back (d cos = -sin d, d sin = cos d): a rotated number next to the middle of two e4m3 ones, which are far apart, should
-// fall to the right side.  Absolute error 1e-7 instead of 2e-7.
-__device__ __forceinline__ void kv8_cos_sin(int pos, double inv_freq, float* c, float* s) {
-  const double a = (double)pos * inv_freq;
-  const double n = rint(a * 0.15915494309189535);
-  const double r = fma(-n, 6.283185307179586, a) - n * 2.4492935982947064e-16;
-  const float rf = (float)r, rest = (float)(r - (double)rf);
-  float sn, cn;
-  sincosf(rf, &sn, &cn);
-  *s = fmaf(cn, rest, sn);
-  *c = fmaf(-sn, rest, cn);
-}
