@@ -212,7 +212,7 @@ attention_e4m3_rows_kernel(const T* q, int q_stride, T* __restrict__ out, const 
   if (r0 >= rows) { pdl_wait(); return; }          // the whole cluster (a CTA that exits lets the next kernel in: it waits first)
   const int pos0 = len - qlen;
   const int t_first = r0 / g, t_last = (min(r0 + R, rows) - 1) / g;
-  const int hi_first = pos0 + t_first + 1, kend = min(pos0 + t_last + 1, max_blocks * page_size);
+  const int hi_first = pos0 + t_first + 1, kend = (int)min((long long)pos0 + t_last + 1, (long long)max_blocks * page_size);
   const int kmin = window > 0 ? max(0, hi_first - window) : 0;
   const int lo_last = window > 0 ? max(0, pos0 + t_last + 1 - window) : 0;
   const int* bt = block_table + (size_t)s * max_blocks;

@@ -71,7 +71,7 @@ attention_e4m3_tcgen05_kernel(const bf16* q, int q_stride, bf16* __restrict__ ou
   }
   const int ntok = min(bq, qlen - t0), live_rows = ntok * g;
   const int pos0 = len - qlen, first_pos = pos0 + t0;
-  const int kend = min(first_pos + ntok, max_blocks * page_size);
+  const int kend = (int)min((long long)first_pos + ntok, (long long)max_blocks * page_size);
   const int kmin = window > 0 ? max(0, first_pos - window + 1) : 0;
   const int all_lo = kmin / E8_BN, all = max(0, (kend + E8_BN - 1) / E8_BN - all_lo);
   const int tile_lo = all_lo + all * rank / splits, ntiles = all_lo + all * (rank + 1) / splits - tile_lo;

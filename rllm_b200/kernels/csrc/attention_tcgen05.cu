@@ -142,10 +142,11 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
   };
   const int kmin = oldest(first_pos);
   const int kend = last_pos + 1;
-  const int all_lo = kmin / AT_BN, all_hi = (kend + AT_BN - 1) / AT_BN;
+  const int dense_lo = DENSE ? oldest(pos0) / AT_BN : 0;       // the first tile that the sequence's place holds
+  const int all_lo = kmin / AT_BN, want_hi = (kend + AT_BN - 1) / AT_BN, all_hi = DENSE ? min(want_hi, dense_lo + opt.dense_tiles) : want_hi;
+  if (DENSE && all_hi < want_hi && threadIdx.x == 0) atomicOr(err, 4);      // longer than the caller said: no keys behind its place
   const int tile_lo = DENSE ? all_lo + (all_hi - all_lo) * rank / splits : all_lo;
   const int tile_hi = DENSE ? all_lo + (all_hi - all_lo) * (rank + 1) / splits : all_hi;
-  const int dense_lo = DENSE ? oldest(pos0) / AT_BN : 0;       // the first tile that the sequence's place holds
   // OPT: the kept first keys ahead of kmin and the key tiles ahead of tile_lo that hold them: walked first
   const int keep = (OPT && window > 0) ? opt.keep_first : 0;
   const int keep_tiles = OPT ? min((min(keep, kmin) + AT_BN - 1) / AT_BN, tile_lo) : 0;

@@ -2179,7 +2179,7 @@ def attention_e4m3_form(dtype: torch.dtype, nq: int, nkv: int, d: int, page_size
       tcgen05 / dense, heads of 64: 4 of 16,000, 4 tiles of 128 rows 182 / 240, 6 tiles 340 / 287, 16 tiles 682 / 518; heads of
         128: 216 / 353, 406 / 381, 798 / 666."""
     g, forced = nq // nkv, os.environ.get("RLLM_ATTENTION")
-    rows_take = d in (64, 128, 256) and page_size % 16 == 0 and forced != "simt"
+    rows_take = d in (64, 128, 256) and page_size % 16 == 0 and forced != "simt" and -(-max_q_len * g // 8) * nkv <= 65535
     if dtype is torch.bfloat16 and d in (64, 128) and g <= 128 and scale > 0 and forced not in ("simt", "mma"):
         most = 32 if d == 64 else 24
         tiles = -(-max_q_len * g // most)
