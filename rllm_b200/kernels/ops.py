@@ -2058,6 +2058,8 @@ def softcap_rows(x: torch.Tensor, cap: float) -> torch.Tensor:
 # ---------------------------------------------------------------------------
 # a cache kept in 8 bits: pages of float8_e4m3fn [pages, nkv, page_size, d] and a power of two a row, float8_e8m0fnu
 # [pages, nkv, page_size], for keys and for values (csrc/kv_e4m3.cuh says what a row becomes)
+# Each operator's common call is checked and launched by the extension module in one go; what it turns down is checked here,
+# for the reason or for another way.
 # ---------------------------------------------------------------------------
 E4M3, E8M0 = torch.float8_e4m3fn, torch.float8_e8m0fnu
 
@@ -2110,6 +2112,9 @@ def rope_kv_write_e4m3(qkv: torch.Tensor, positions: torch.Tensor, token_seq: to
 
     The rotation and the row's scale are float32; a number is rounded once, to e4m3.  A (sequence, position) pair may stand
     in the step once.  A token whose page is not held sets bit 2 of ``err`` and is not written (its q is rotated)."""
+    if _launch().e4m3_write(_entries.rllm_kv_e4m3_write, qkv, q_out, positions, token_seq, err, kcache, vcache, kscale, vscale,
+                            block_table, inv_freq, rotary_dim, nq, nkv, d):
+        return
     dt = dtype_code(qkv.dtype)
     if qkv.dim() != 2 or qkv.shape[1] != (nq + 2 * nkv) * d or not qkv.is_contiguous():
         raise KernelError("rope_kv_write_e4m3: qkv must be [T, (nq + 2 nkv) d], contiguous")
@@ -2126,7 +2131,7 @@ def rope_kv_write_e4m3(qkv: torch.Tensor, positions: torch.Tensor, token_seq: to
             raise KernelError("rope_kv_write_e4m3: q_out must be [T, nq d] of qkv's type")
         stride = max(q_out.stride(0), nq * d) if T <= 1 else q_out.stride(0)
     _e4m3_cache(kcache, vcache, kscale, vscale, block_table, nkv, d, positions, token_seq, err)
-    _beside(kcache, qkv, q_out)
+    _beside(kcache, qkv, q_out, *([inv_freq] if rotary_dim else []))
     pages, _, page_size, _ = kcache.shape
     seqs, blocks = block_table.shape
     _entries.rllm_kv_e4m3_write(qkv, dt, q_out, stride, positions, token_seq, inv_freq if rotary_dim else None, rotary_dim,
@@ -2139,6 +2144,8 @@ def kv_read_e4m3(positions: torch.Tensor, token_seq: torch.Tensor, block_table: 
     """Keys and values of given tokens out of a cache kept in 8 bits: out_k, out_v [T, nkv d] (bfloat16 or float32) = the
     rows of sequence ``token_seq[t]``'s token at ``positions[t]``.  Exact in float32, and in bfloat16 down to its smallest
     numbers; NaN where a row's scale is.  A token whose page is not held sets bit 4 of ``err`` and reads as zeros."""
+    if _launch().e4m3_read(_entries.rllm_kv_e4m3_read, out_k, out_v, positions, token_seq, err, kcache, vcache, kscale, vscale, block_table):
+        return
     dt = dtype_code(out_k.dtype)
     if kcache.dim() != 4:
         raise KernelError("kv_read_e4m3: kcache must be [pages, nkv, page_size, d]")
@@ -2200,6 +2207,10 @@ def attention_e4m3(q: torch.Tensor, out: torch.Tensor, kcache: torch.Tensor, vca
     the first ``num_decode`` sequences bring one token each.  ``max_q_len`` and ``max_seq_len`` bound every sequence's tokens
     in this step and in the cache.  Rows behind the last sequence's stay as they are.  A page that is not held sets bit 4 of
     ``err``, and its keys are left out."""
+    if num_decode == seq_lens.numel() and max_q_len >= 0 and \
+            _launch().e4m3_decode(_entries.rllm_attention_e4m3_rows, q, out, q_start, seq_lens, err, kcache, vcache, kscale, vscale,
+                                  block_table, max_seq_len, nq, nkv, window, scale):
+        return
     dt = dtype_code(q.dtype)
     S, d = seq_lens.numel(), kcache.shape[-1]
     if q.dim() != 2 or out.dim() != 2 or out.dtype is not q.dtype:

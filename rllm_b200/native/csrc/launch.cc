@@ -281,11 +281,11 @@ PyObject* product(PyObject*, PyObject* const* args, Py_ssize_t n) {
 // e4m3_ready(kcache, vcache, kscale, vscale, block_table, nkv, d, *vectors): whether these are what the operators over such a
 // cache take (see rllm_b200/kernels/ops.py, _e4m3_cache, which holds the same rules and says what is wrong): all on the current
 // device, the vectors contiguous, one-dimensional and int32.  In Python these checks cost as much as the launch three times over.
-bool e4m3_ready_args(PyObject* const* args, Py_ssize_t n) {
-  for (int i = 0; i < 5; ++i)
-    if (!THPVariable_Check(args[i])) return false;
-  const long long nkv = PyLong_AsLongLong(args[5]), d = PyLong_AsLongLong(args[6]);
-  if (PyErr_Occurred()) return false;
+bool vector_of_ints(const at::Tensor& t, int device) {
+  return t.is_cuda() && t.get_device() == device && t.scalar_type() == at::kInt && t.dim() == 1 && t.is_contiguous();
+}
+
+bool e4m3_cache(PyObject* const* args, long long nkv, long long d, int device) {      // kcache, vcache, kscale, vscale, block_table
   const at::Tensor &k = THPVariable_Unpack(args[0]), &v = THPVariable_Unpack(args[1]), &ks = THPVariable_Unpack(args[2]),
                    &vs = THPVariable_Unpack(args[3]), &table = THPVariable_Unpack(args[4]);
   if (k.scalar_type() != at::kFloat8_e4m3fn || v.scalar_type() != at::kFloat8_e4m3fn || ks.scalar_type() != at::kFloat8_e8m0fnu ||
@@ -294,28 +294,152 @@ bool e4m3_ready_args(PyObject* const* args, Py_ssize_t n) {
   if (k.dim() != 4 || k.size(1) != nkv || k.size(3) != d || v.sizes() != k.sizes() || ks.sizes() != k.sizes().slice(0, 3) ||
       vs.sizes() != ks.sizes() || table.dim() != 2)
     return false;
-  const int device = c10::cuda::current_device();
   for (int i = 0; i < 5; ++i) {
     const at::Tensor& t = THPVariable_Unpack(args[i]);
     if (!t.is_cuda() || t.get_device() != device || !t.is_contiguous()) return false;
   }
-  for (Py_ssize_t i = 7; i < n; ++i) {
-    if (!THPVariable_Check(args[i])) return false;
-    const at::Tensor& t = THPVariable_Unpack(args[i]);
-    if (!t.is_cuda() || t.get_device() != device || t.scalar_type() != at::kInt || t.dim() != 1 || !t.is_contiguous()) return false;
-  }
+  return true;
+}
+
+// all of args[0 .. n - 1] are tensors on CUDA devices (asked before CUDA is asked for its current one)
+bool cuda_tensors(PyObject* const* args, Py_ssize_t n) {
+  for (Py_ssize_t i = 0; i < n; ++i)
+    if (!THPVariable_Check(args[i]) || !THPVariable_Unpack(args[i]).is_cuda()) return false;
   return true;
 }
 
 PyObject* e4m3_ready(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (n < 7) return PyErr_Format(PyExc_TypeError, "e4m3_ready(kcache, vcache, kscale, vscale, block_table, nkv, d, *vectors)");
-  // (a tensor without CUDA, before CUDA is asked for its device)
-  for (int i = 0; i < 5; ++i)
-    if (!THPVariable_Check(args[i]) || !THPVariable_Unpack(args[i]).is_cuda()) Py_RETURN_FALSE;
+  if (!cuda_tensors(args, 5) || !cuda_tensors(args + 7, n - 7)) Py_RETURN_FALSE;
   return guarded([&]() -> PyObject* {
-    const bool ok = e4m3_ready_args(args, n);
+    const long long nkv = PyLong_AsLongLong(args[5]), d = PyLong_AsLongLong(args[6]);
     if (PyErr_Occurred()) return nullptr;
-    return PyBool_FromLong(ok);
+    const int device = c10::cuda::current_device();
+    if (!e4m3_cache(args, nkv, d, device)) Py_RETURN_FALSE;
+    for (Py_ssize_t i = 7; i < n; ++i)
+      if (!vector_of_ints(THPVariable_Unpack(args[i]), device)) Py_RETURN_FALSE;
+    Py_RETURN_TRUE;
+  });
+}
+
+// The three operators' common calls, checked and launched in one go: True, or False where Python's own way has to look (and
+// refuse, or take the call another way).  Each is given its entry point first.
+int float_code(const at::Tensor& t) { return t.scalar_type() == at::kBFloat16 ? 1 : t.scalar_type() == at::kFloat ? 0 : -1; }
+
+// e4m3_write(entry, qkv, q_out or None, positions, token_seq, err, kcache, vcache, kscale, vscale, block_table, inv_freq or None, rotary_dim,
+//            nq, nkv, d)
+PyObject* e4m3_write(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (n != 16 || Py_TYPE(args[0]) != &EntryType) return PyErr_Format(PyExc_TypeError, "e4m3_write(entry, ... 15 arguments)");
+  const bool in_place = args[2] == Py_None;
+  if (!cuda_tensors(args + 1, 1) || !(in_place || cuda_tensors(args + 2, 1)) || !cuda_tensors(args + 3, 8)) Py_RETURN_FALSE;
+  return guarded([&]() -> PyObject* {
+    bool bad = false;
+    const long long rot = whole(args[12], bad), nq = whole(args[13], bad), nkv = whole(args[14], bad), d = whole(args[15], bad);
+    if (bad) return nullptr;
+    Entry* e = (Entry*)args[0];
+    if (!ready(e)) return nullptr;
+    const at::Tensor &qkv = THPVariable_Unpack(args[1]), &q = THPVariable_Unpack(args[in_place ? 1 : 2]);
+    const int device = c10::cuda::current_device(), dt = float_code(qkv);
+    if (dt < 0 || qkv.dim() != 2 || qkv.size(1) != (nq + 2 * nkv) * d || !qkv.is_contiguous() || qkv.get_device() != device ||
+        q.dim() != 2 || q.size(0) != qkv.size(0) || (!in_place && q.size(1) != nq * d) || q.stride(1) != 1 || q.scalar_type() != qkv.scalar_type() ||
+        q.get_device() != device || !e4m3_cache(args + 6, nkv, d, device))
+      Py_RETURN_FALSE;
+    const long long T = qkv.size(0), stride = T > 1 ? q.stride(0) : q.size(1);
+    for (int i = 3; i < 6; ++i)
+      if (!vector_of_ints(THPVariable_Unpack(args[i]), device)) Py_RETURN_FALSE;
+    if (THPVariable_Unpack(args[3]).numel() != T || THPVariable_Unpack(args[4]).numel() != T) Py_RETURN_FALSE;
+    void* freq = nullptr;
+    if (rot) {
+      if (!cuda_tensors(args + 11, 1)) Py_RETURN_FALSE;
+      const at::Tensor& f = THPVariable_Unpack(args[11]);
+      if (f.scalar_type() != at::kDouble || f.numel() != rot / 2 || !f.is_contiguous() || f.get_device() != device) Py_RETURN_FALSE;
+      freq = f.data_ptr();
+    }
+    const at::Tensor &k = THPVariable_Unpack(args[6]), &table = THPVariable_Unpack(args[10]);
+    auto at_ = [&](int i) { return THPVariable_Unpack(args[i]).data_ptr(); };
+    const cudaStream_t stream = stream_now();
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = reinterpret_cast<int (*)(void*, int, void*, long long, void*, void*, void*, int, void*, int, int, void*, void*, void*, void*, int, int,
+                                  int, int, int, int, void*, cudaStream_t)>(e->fn)(
+        qkv.data_ptr(), dt, q.data_ptr(), stride, at_(3), at_(4), freq, (int)rot, table.data_ptr(), (int)table.size(1), (int)table.size(0),
+        at_(6), at_(7), at_(8), at_(9), (int)T, (int)nq, (int)nkv, (int)d, (int)k.size(2), (int)k.size(0), at_(5), stream);
+    Py_END_ALLOW_THREADS
+    if (!finish(rc, e->what)) return nullptr;
+    Py_RETURN_TRUE;
+  });
+}
+
+// e4m3_read(entry, out_k, out_v, positions, token_seq, err, kcache, vcache, kscale, vscale, block_table)
+PyObject* e4m3_read(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (n != 11 || Py_TYPE(args[0]) != &EntryType) return PyErr_Format(PyExc_TypeError, "e4m3_read(entry, ... 10 arguments)");
+  if (!cuda_tensors(args + 1, 10)) Py_RETURN_FALSE;
+  return guarded([&]() -> PyObject* {
+    Entry* e = (Entry*)args[0];
+    if (!ready(e)) return nullptr;
+    const at::Tensor &ok = THPVariable_Unpack(args[1]), &ov = THPVariable_Unpack(args[2]), &k = THPVariable_Unpack(args[6]),
+                     &table = THPVariable_Unpack(args[10]);
+    const int device = c10::cuda::current_device(), dt = float_code(ok);
+    if (dt < 0 || k.dim() != 4 || !e4m3_cache(args + 6, k.size(1), k.size(3), device)) Py_RETURN_FALSE;
+    for (int i = 3; i < 6; ++i)
+      if (!vector_of_ints(THPVariable_Unpack(args[i]), device)) Py_RETURN_FALSE;
+    const long long T = THPVariable_Unpack(args[3]).numel();
+    if (THPVariable_Unpack(args[4]).numel() != T || ok.dim() != 2 || ok.size(0) != T || ok.size(1) != k.size(1) * k.size(3) ||
+        ov.sizes() != ok.sizes() || ov.scalar_type() != ok.scalar_type() || !ok.is_contiguous() || !ov.is_contiguous() ||
+        ok.get_device() != device || ov.get_device() != device)
+      Py_RETURN_FALSE;
+    auto at_ = [&](int i) { return THPVariable_Unpack(args[i]).data_ptr(); };
+    const cudaStream_t stream = stream_now();
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = reinterpret_cast<int (*)(void*, void*, void*, int, int, void*, void*, void*, void*, void*, void*, int, int, int, int, int, int, void*,
+                                  cudaStream_t)>(e->fn)(
+        at_(3), at_(4), table.data_ptr(), (int)table.size(1), (int)table.size(0), at_(6), at_(7), at_(8), at_(9), ok.data_ptr(), ov.data_ptr(), dt,
+        (int)T, (int)k.size(1), (int)k.size(3), (int)k.size(2), (int)k.size(0), at_(5), stream);
+    Py_END_ALLOW_THREADS
+    if (!finish(rc, e->what)) return nullptr;
+    Py_RETURN_TRUE;
+  });
+}
+
+// e4m3_decode(entry, q, out, q_start, seq_lens, err, kcache, vcache, kscale, vscale, block_table, max_seq_len, nq, nkv, window, scale):
+// every sequence brings one token, and the rows kernel takes it
+PyObject* e4m3_decode(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (n != 16 || Py_TYPE(args[0]) != &EntryType) return PyErr_Format(PyExc_TypeError, "e4m3_decode(entry, ... 15 arguments)");
+  if (!cuda_tensors(args + 1, 10)) Py_RETURN_FALSE;
+  return guarded([&]() -> PyObject* {
+    bool bad = false;
+    const long long most = whole(args[11], bad), nq = whole(args[12], bad), nkv = whole(args[13], bad), window = whole(args[14], bad);
+    const float scale = bad ? 0.f : Arg<'f'>::get(args[15], bad);
+    if (bad) return nullptr;
+    Entry* e = (Entry*)args[0];
+    if (!ready(e)) return nullptr;
+    const at::Tensor &q = THPVariable_Unpack(args[1]), &out = THPVariable_Unpack(args[2]), &k = THPVariable_Unpack(args[6]),
+                     &table = THPVariable_Unpack(args[10]);
+    const int device = c10::cuda::current_device(), dt = float_code(q);
+    if (dt < 0 || k.dim() != 4 || nq <= 0 || nkv <= 0 || nkv > 16383 || nq % nkv || std::getenv("RLLM_ATTENTION")) Py_RETURN_FALSE;
+    const long long d = k.size(3), page = k.size(2), g = nq / nkv;
+    if (!(d == 64 || d == 128 || d == 256) || page % 16 || g > (dt == 1 && d != 256 ? (d == 64 ? 32 : 24) : 16) || !e4m3_cache(args + 6, nkv, d, device))
+      Py_RETURN_FALSE;
+    for (int i = 3; i < 6; ++i)
+      if (!vector_of_ints(THPVariable_Unpack(args[i]), device)) Py_RETURN_FALSE;
+    const long long S = THPVariable_Unpack(args[4]).numel();
+    if (S == 0 || THPVariable_Unpack(args[3]).numel() != S + 1 || table.size(0) < S || most < 0 || most > table.size(1) * page || q.dim() != 2 ||
+        out.dim() != 2 || out.scalar_type() != q.scalar_type() || q.stride(1) != 1 || out.size(1) != nq * d || q.size(1) < nq * d ||
+        q.size(0) < out.size(0) || out.size(0) == 0 || !out.is_contiguous() || q.get_device() != device || out.get_device() != device)
+      Py_RETURN_FALSE;
+    const long long keys = window > 0 && window + 1 < most ? window + 1 : most;
+    auto at_ = [&](int i) { return THPVariable_Unpack(args[i]).data_ptr(); };
+    const cudaStream_t stream = stream_now();
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = reinterpret_cast<int (*)(void*, int, void*, void*, void*, void*, void*, int, void*, int, void*, void*, int, int, int, int, int, int, int,
+                                  int, int, int, float, void*, cudaStream_t)>(e->fn)(
+        q.data_ptr(), (int)q.stride(0), out.data_ptr(), at_(6), at_(7), at_(8), at_(9), dt, table.data_ptr(), (int)table.size(1), at_(3), at_(4), 0,
+        (int)S, 1, (int)keys, (int)nq, (int)nkv, (int)d, (int)page, (int)k.size(0), (int)window, scale, at_(5), stream);
+    Py_END_ALLOW_THREADS
+    if (!finish(rc, e->what)) return nullptr;
+    Py_RETURN_TRUE;
   });
 }
 
@@ -333,6 +457,9 @@ PyMethodDef kMethods[] = {{"setup", (PyCFunction)(void*)setup, METH_FASTCALL, nu
                           {"error_word", (PyCFunction)(void*)set_error_word, METH_FASTCALL, nullptr},
                           {"product", (PyCFunction)(void*)product, METH_FASTCALL, nullptr},
                           {"e4m3_ready", (PyCFunction)(void*)e4m3_ready, METH_FASTCALL, nullptr},
+                          {"e4m3_write", (PyCFunction)(void*)e4m3_write, METH_FASTCALL, nullptr},
+                          {"e4m3_read", (PyCFunction)(void*)e4m3_read, METH_FASTCALL, nullptr},
+                          {"e4m3_decode", (PyCFunction)(void*)e4m3_decode, METH_FASTCALL, nullptr},
                           {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "launch", nullptr, -1, kMethods};
 

@@ -393,3 +393,102 @@ def test_attention_does_not_depend_on_how_a_prompt_was_cut():
         part.seq_lens[0] = 50 + n
         part.num_decode = 1 if n == 1 else 0
         part.check(part.attend(ops))
+
+
+class TheLongWay:
+    """The extension module without its checking and launching in one go."""
+
+    def __init__(self, module):
+        self.module = module
+
+    def __getattr__(self, name):
+        return (lambda *args: False) if name in ("e4m3_write", "e4m3_read", "e4m3_decode") else getattr(self.module, name)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("nq,nkv,d,rd,page,window", [(8, 2, 64, 64, 16, 0), (6, 2, 128, 64, 32, 20), (5, 1, 256, 0, 16, 0), (4, 4, 48, 48, 7, 9),
+                                                     (64, 1, 64, 64, 16, 0), (32, 1, 64, 64, 16, 33)])
+def test_calls_checked_in_one_go_and_the_long_way_give_the_same_bits(dtype, nq, nkv, d, rd, page, window, monkeypatch):
+    results = []
+    for long_way in (False, True):
+        if long_way:
+            module = TheLongWay(ops._launch())
+            monkeypatch.setattr(ops, "_launch", lambda: module)
+        st = Step([1, 1, 1], [37, 100, 15], nq, nkv, d, page, dtype, seed=d, more_rows=1, stride_pad=16)
+        g = torch.Generator().manual_seed(1)
+        qkv = torch.randn(3, (nq + 2 * nkv) * d, generator=g).to(dtype).cuda()
+        cache = (st.k, st.v, st.ks, st.vs)
+        inv = freqs(rd) if rd else None
+        out = [torch.full((4, nq * d + 8), 3.0, dtype=dtype, device="cuda")]
+        ops.rope_kv_write_e4m3(qkv, st.positions, st.token_seq, inv, rd, st.table, *cache, nq, nkv, d, st.err, q_out=out[0][:3, :nq * d])
+        ops.rope_kv_write_e4m3(qkv, st.positions, st.token_seq, inv, rd, st.table, *cache, nq, nkv, d, st.err)
+        out += [qkv, st.attend(ops, window)] + [torch.full((4, nkv * d), 3.0, dtype=dtype, device="cuda") for _ in range(2)]
+        ops.kv_read_e4m3(st.positions, st.token_seq, st.table, *cache, out[3][:3], out[4][:3], st.err)
+        assert int(st.err) == 0
+        results.append(out + [c.view(torch.uint8) for c in cache])
+    assert all(torch.equal(a, b) for a, b in zip(*results))
+
+
+def on_gpu(x):
+    """A copy on the GPU with the same strides."""
+    if not isinstance(x, torch.Tensor):
+        return x
+    y = torch.empty_strided(x.shape, x.stride(), dtype=x.dtype, device="cuda")
+    y.view(torch.uint8).copy_(x.view(torch.uint8)) if x.dtype in (E4M3, E8M0) else y.copy_(x)
+    return y
+
+
+I32 = dict(dtype=torch.int32)
+WRITES = [dict(qkv=torch.zeros(2, 7 * 64, dtype=BF16)), dict(qkv=torch.zeros(2, 8 * 64, dtype=torch.float16)), dict(positions=torch.zeros(1, **I32)),
+          dict(token_seq=torch.zeros(2, dtype=torch.int64)), dict(inv_freq=None), dict(inv_freq=torch.zeros(32)),
+          dict(inv_freq=torch.zeros(16, dtype=torch.float64)), dict(inv_freq=torch.zeros(64, dtype=torch.float64)[::2]),
+          dict(q_out=torch.zeros(2, 4 * 64)), dict(q_out=torch.zeros(3, 4 * 64, dtype=BF16)), dict(q_out=torch.zeros(2, 5 * 64, dtype=BF16)),
+          dict(q_out=torch.zeros(4 * 64, 2, dtype=BF16).t()), dict(q_out=torch.zeros(1, 4 * 64, dtype=BF16).expand(2, -1)),
+          dict(qkv=torch.zeros(8 * 64, 2, dtype=BF16).t()), dict(block_table=torch.zeros(2, **I32)), dict(err=torch.zeros(1, dtype=torch.int64)),
+          dict(nkv=1, qkv=torch.zeros(2, 6 * 64, dtype=BF16)), dict(d=32, qkv=torch.zeros(2, 8 * 32, dtype=BF16)), dict(rotary_dim=65),
+          dict(rotary_dim=-64), dict(nq=-4, qkv=torch.zeros(2, 0, dtype=BF16))]
+DECODES = [dict(q=torch.zeros(2, 4 * 64)), dict(q=torch.zeros(2, 3 * 64, dtype=BF16)), dict(q=torch.zeros(1, 4 * 64, dtype=BF16)),
+           dict(q=torch.zeros(4 * 64, 2, dtype=BF16).t()), dict(out=torch.zeros(2, 8 * 64, dtype=BF16)[:, ::2]),
+           dict(q=torch.zeros(2, 4 * 64, dtype=torch.float16), out=torch.zeros(2, 4 * 64, dtype=torch.float16)),
+           dict(q_start=torch.zeros(2, **I32)), dict(seq_lens=torch.zeros(2, dtype=torch.int64)), dict(nd=3), dict(nd=-1), dict(ms=33), dict(ms=-1),
+           dict(mq=-1), dict(nkv=4), dict(nq=3), dict(nkv=0), dict(table=torch.zeros(1, 2, **I32)), dict(table=torch.zeros(2, 4, **I32)[:, ::2]),
+           dict(window=-1), dict(scale=math.nan), dict(scale=math.inf)]
+
+
+@pytest.mark.parametrize("over", WRITES)
+def test_a_write_that_does_not_fit_is_refused_on_the_gpu_too(over):
+    a = dict(qkv=torch.zeros(2, 8 * 64, dtype=BF16), positions=torch.arange(2, **I32), token_seq=torch.zeros(2, **I32),
+             inv_freq=torch.zeros(32, dtype=torch.float64), rotary_dim=64, block_table=torch.arange(2, **I32).view(1, 2), nq=4, nkv=2, d=64,
+             err=torch.zeros(1, **I32), q_out=None)
+    a.update(over)
+    a = {k: on_gpu(x) if k != "q_out" or x is None or x.stride(0) else x[:1].cuda().expand(2, -1) for k, x in a.items()}
+    cache = [torch.full((3, 2, 16) + tail, 9, dtype=torch.uint8, device="cuda") for tail in ((64,), (64,), (), ())]
+    with pytest.raises(ops.KernelError):
+        ops.rope_kv_write_e4m3(a["qkv"], a["positions"], a["token_seq"], a["inv_freq"], a["rotary_dim"], a["block_table"], cache[0].view(E4M3),
+                               cache[1].view(E4M3), cache[2].view(E8M0), cache[3].view(E8M0), a["nq"], a["nkv"], a["d"], a["err"], q_out=a["q_out"])
+    assert all((c == 9).all() for c in cache)
+
+
+@pytest.mark.parametrize("over", DECODES)
+def test_an_attention_of_single_tokens_that_does_not_fit_is_refused_on_the_gpu_too(over):
+    a = dict(q=torch.zeros(2, 4 * 64, dtype=BF16), out=torch.zeros(2, 4 * 64, dtype=BF16), table=torch.zeros(2, 2, **I32),
+             q_start=torch.arange(3, **I32), seq_lens=torch.full((2,), 20, **I32), nd=2, mq=1, ms=20, nq=4, nkv=2, window=0, scale=0.125,
+             err=torch.zeros(1, **I32))
+    a.update(over)
+    a = {k: on_gpu(x) for k, x in a.items()}
+    cache = [torch.zeros((3, 2, 16) + tail, dtype=torch.uint8, device="cuda") for tail in ((64,), (64,), (), ())]
+    with pytest.raises(ops.KernelError):
+        ops.attention_e4m3(a["q"], a["out"], cache[0].view(E4M3), cache[1].view(E4M3), cache[2].view(E8M0), cache[3].view(E8M0), a["table"],
+                           a["q_start"], a["seq_lens"], a["nd"], a["mq"], a["ms"], a["nq"], a["nkv"], a["window"], a["scale"], a["err"])
+
+
+def test_a_reading_that_does_not_fit_is_refused_on_the_gpu_too():
+    st = Step([2], [0], 4, 2, 64, 16, BF16)
+    good = dict(pos=st.positions, seq=st.token_seq, k=torch.zeros(2, 128, dtype=BF16, device="cuda"), v=torch.zeros(2, 128, dtype=BF16, device="cuda"))
+    for over in (dict(seq=st.token_seq[:1]), dict(pos=st.positions.long()), dict(k=good["k"][:1]), dict(v=good["v"].float()),
+                 dict(k=good["k"].half(), v=good["v"].half()), dict(k=torch.zeros(2, 256, dtype=BF16, device="cuda")[:, ::2]), dict(v=good["v"].cpu())):
+        a = {**good, **over}
+        with pytest.raises(ops.KernelError):
+            ops.kv_read_e4m3(a["pos"], a["seq"], st.table, st.k, st.v, st.ks, st.vs, a["k"], a["v"], st.err)
+    with pytest.raises(ops.KernelError):
+        ops.kv_read_e4m3(good["pos"], good["seq"], st.table, st.k, st.v, st.k, st.vs, good["k"], good["v"], st.err)
