@@ -716,7 +716,7 @@ RLLM_EXPORT int rllm_attention_e4m3_rows(const void* q, int q_stride, void* out,
   if (max_q_len <= 0 || seq_end <= seq_begin) return 0;
   if (const int rc = e4_check(q, out, kcache, vcache, kscale, vscale, block_table, max_blocks, q_start, seq_lens, seq_begin,
                               seq_end, nq, nkv, d, page_size, num_pages, window, scale, err)) return rc;
-  if (page_size % 16 || !(d == 64 || d == 128 || d == 256) || (((uintptr_t)kscale | (uintptr_t)vscale) & 15)) return RLLM_E_UNSUPPORTED;
+  if (page_size % 16 || !(d == 64 || d == 128 || d == 256) || (((uintptr_t)kscale | (uintptr_t)vscale | (uintptr_t)out) & 15)) return RLLM_E_UNSUPPORTED;
   if ((long long)num_pages * nkv * (page_size >> 4) > 0x7fffffffLL) return RLLM_E_UNSUPPORTED;      // tiles of 16 rows are counted in 32 bits
 #define E4_ROWS(DD, NBB, TT)                                                                                                   \
   return e4_rows_launch<DD, NBB, TT>(q, q_stride, out, kcache, vcache, kscale, vscale, block_table, max_blocks, q_start, \

@@ -65,6 +65,7 @@ _TABLE = {
     "rllm_kv_e4m3_widen": ("kv_e4m3", "pippiiipppppppiiiiip", "attention_e4m3"),
     "rllm_attention_dense_tcgen05": ("attention_tcgen05", "piippppippiiiiiiifp", "attention_e4m3"),
     "rllm_attention_e4m3_tcgen05": ("attention_e4m3_tcgen05", "pippppppippiiiiiiiiiifp", "attention_e4m3"),
+    "rllm_attention_e4m3_columns": ("attention_e4m3_columns", "pippppppippiiiiiiiiiifp", "attention_e4m3"),
     "rllm_attention_e4m3_rows": ("attention_e4m3", "pipppppipippiiiiiiiiiifp", "attention_e4m3"),
     "rllm_attention_e4m3_simt": ("attention_e4m3", "pipppppipippiiiiiiiiifp", "attention_e4m3"),
     "rllm_softcap": ("elementwise", "plf", "softcap_rows"),
@@ -2176,22 +2177,29 @@ def e4m3_dense_scratch(nkv: int, d: int, max_seq_len: int) -> int:
 
 def attention_e4m3_form(dtype: torch.dtype, nq: int, nkv: int, d: int, page_size: int, scale: float, max_q_len: int,
                         num_seqs: int, max_keys: int) -> str:
-    """Which kernel takes ``num_seqs`` sequences of up to ``max_q_len`` tokens whose queries see up to ``max_keys`` keys: "rows"
-    (mma.sync, up to 32 rows of a kv head at a time; a row is a token and a head of the kv head's group), "tcgen05" (128 rows,
-    keys and values widened inside), "dense" (tcgen05 over keys and values widened once for all tiles of rows), "simt".
+    """Which kernel takes ``num_seqs`` sequences of up to ``max_q_len`` tokens whose queries see up to ``max_keys`` keys: "columns"
+    (tcgen05, the cache's bytes as operands, up to 32 rows of a kv head at a time; a row is a token and a head of the kv head's
+    group), "rows" (mma.sync, 8 to 32 rows), "tcgen05" (128 rows, keys and values widened inside), "dense" (tcgen05 over keys and
+    values widened once for all tiles of rows), "simt".
 
-    Measured (microseconds; 8 kv heads with four heads each):
-      rows / tcgen05, heads of 64: 8 sequences of 16,000 keys, 32 rows 72 / 81, 48 rows 138 / 82; one of 4,000, 128 rows 15 / 18;
-        heads of 128: 8 of 16,000, 24 rows 95 / 101, 32 rows 181 / 101; one of 1,000, 64 rows 12 / 15, of 16,000, 128 rows 90 / 48;
+    Measured (microseconds in a row; 8 kv heads with four heads each):
+      rows / columns, heads of 64: one token each, one sequence of 511 keys 4.5 / 6.3, 2,047 6.1 / 6.8, 8,191 11.7 / 9.8; 8 of 511
+        5.8 / 7.0, 1,023 8.9 / 8.1, 8,191 23.4 / 17.8; 64 of 255 8.4 / 11.9, 511 12.9 / 14.1, 1,023 21.6 / 19.8, 8,191 118 / 100; 8 of
+        4,095, 16 rows 25 / 18.6, 32 rows 32 / 24; heads of 128: one sequence of 511 5.7 / 5.7, 8 of 1,023 10.9 / 8.6, 64 of 255
+        11.7 / 12.9, 8,191 221 / 161; 8 of 4,095, 16 rows 34 / 20.6, 32 rows 61 / 28;
+      columns / tcgen05, more rows: heads of 128, one of 4,095, 64 rows 18.0 / 20.2, 128 rows 19.0 / 22.8 (heads of 64, rows / tcgen05: 15.0 /
+        17.2 and 16.6 / 18.4); 8 of 4,095, 64 rows 44 / 38, 128 rows 86 / 45;
       tcgen05 / dense, heads of 64: 4 of 16,000, 4 tiles of 128 rows 182 / 240, 6 tiles 340 / 287, 16 tiles 682 / 518; heads of
         128: 216 / 353, 406 / 381, 798 / 666."""
     g, forced = nq // nkv, os.environ.get("RLLM_ATTENTION")
-    rows_take = d in (64, 128, 256) and page_size % 16 == 0 and forced != "simt" and -(-max_q_len * g // 8) * nkv <= 65535
-    if dtype is torch.bfloat16 and d in (64, 128) and g <= 128 and scale > 0 and forced not in ("simt", "mma"):
-        most = 32 if d == 64 else 24
-        tiles = -(-max_q_len * g // most)
-        few = tiles == 1 or (num_seqs * nkv * tiles <= 32 and (d == 64 or max_keys <= 2048))
-        if not (few and rows_take):
+    rows, in_16s = max_q_len * g, page_size % 16 == 0 and forced != "simt"
+    rows_take = in_16s and d in (64, 128, 256) and -(-rows // 8) * nkv <= 65535
+    if dtype is torch.bfloat16 and d in (64, 128) and forced not in ("simt", "mma"):
+        tiles = -(-rows // 32)
+        few = tiles == 1 or num_seqs * nkv * tiles <= 32
+        if few and in_16s and (tiles == 1 or d == 128) and max_keys >= 768 and num_seqs * nkv * tiles * max_keys * d >= 1 << 21:
+            return "columns"
+        if not (few and rows_take) and g <= 128 and scale > 0:
             return "tcgen05" if -(-max_q_len // (128 // g)) <= 4 else "dense"
     return "rows" if rows_take else "simt"
 
@@ -2209,7 +2217,7 @@ def attention_e4m3(q: torch.Tensor, out: torch.Tensor, kcache: torch.Tensor, vca
     ``err``, and its keys are left out."""
     if num_decode == seq_lens.numel() and max_q_len >= 0 and \
             _launch().e4m3_decode(_entries.rllm_attention_e4m3_rows, q, out, q_start, seq_lens, err, kcache, vcache, kscale, vscale,
-                                  block_table, max_seq_len, nq, nkv, window, scale):
+                                  block_table, max_seq_len, nq, nkv, window, scale, _entries.rllm_attention_e4m3_columns):
         return
     dt = dtype_code(q.dtype)
     S, d = seq_lens.numel(), kcache.shape[-1]
@@ -2234,10 +2242,15 @@ def attention_e4m3(q: torch.Tensor, out: torch.Tensor, kcache: torch.Tensor, vca
         if first == end or longest == 0:
             continue
         form = attention_e4m3_form(q.dtype, nq, nkv, d, page_size, scale, longest, end - first, keys)
-        if form in ("tcgen05", "dense") and (stride % 8 or (q.data_ptr() | out.data_ptr()) % 16):
+        if out.data_ptr() % 16:
+            form = "simt"
+        elif form in ("tcgen05", "dense") and (stride % 8 or q.data_ptr() % 16):
             form = "rows" if page_size % 16 == 0 else "simt"
         if form == "rows":
             _entries.rllm_attention_e4m3_rows(q, stride, out, *cache, first, end, longest, keys, *heads)
+        elif form == "columns":
+            _entries.rllm_attention_e4m3_columns(q, stride, out, kcache, vcache, kscale, vscale, block_table, blocks, q_start,
+                                                 seq_lens, first, end, longest, keys, *heads)
         elif form == "tcgen05":
             _entries.rllm_attention_e4m3_tcgen05(q, stride, out, kcache, vcache, kscale, vscale, block_table, blocks, q_start,
                                                  seq_lens, first, end, longest, keys, *heads)

@@ -402,41 +402,51 @@ PyObject* e4m3_read(PyObject*, PyObject* const* args, Py_ssize_t n) {
   });
 }
 
-// e4m3_decode(entry, q, out, q_start, seq_lens, err, kcache, vcache, kscale, vscale, block_table, max_seq_len, nq, nkv, window, scale):
-// every sequence brings one token, and the rows kernel takes it
+// e4m3_decode(rows entry, q, out, q_start, seq_lens, err, kcache, vcache, kscale, vscale, block_table, max_seq_len, nq, nkv, window,
+// scale, columns entry): every sequence brings one token, and one of the two kernels takes it, by the rule of attention_e4m3_form in
+// rllm_b200/kernels/ops.py
 PyObject* e4m3_decode(PyObject*, PyObject* const* args, Py_ssize_t n) {
-  if (n != 16 || Py_TYPE(args[0]) != &EntryType) return PyErr_Format(PyExc_TypeError, "e4m3_decode(entry, ... 15 arguments)");
+  if (n != 17 || Py_TYPE(args[0]) != &EntryType || Py_TYPE(args[16]) != &EntryType)
+    return PyErr_Format(PyExc_TypeError, "e4m3_decode(entry, ... 15 arguments, entry)");
   if (!cuda_tensors(args + 1, 10)) Py_RETURN_FALSE;
   return guarded([&]() -> PyObject* {
     bool bad = false;
     const long long most = whole(args[11], bad), nq = whole(args[12], bad), nkv = whole(args[13], bad), window = whole(args[14], bad);
     const float scale = bad ? 0.f : Arg<'f'>::get(args[15], bad);
     if (bad) return nullptr;
-    Entry* e = (Entry*)args[0];
-    if (!ready(e)) return nullptr;
     const at::Tensor &q = THPVariable_Unpack(args[1]), &out = THPVariable_Unpack(args[2]), &k = THPVariable_Unpack(args[6]),
                      &table = THPVariable_Unpack(args[10]);
     const int device = c10::cuda::current_device(), dt = float_code(q);
     if (dt < 0 || k.dim() != 4 || nq <= 0 || nkv <= 0 || nkv > 16383 || nq % nkv || std::getenv("RLLM_ATTENTION")) Py_RETURN_FALSE;
     const long long d = k.size(3), page = k.size(2), g = nq / nkv;
-    if (!(d == 64 || d == 128 || d == 256) || page % 16 || g > (dt == 1 && d != 256 ? (d == 64 ? 32 : 24) : 16) || !e4m3_cache(args + 6, nkv, d, device))
-      Py_RETURN_FALSE;
+    const bool both = dt == 1 && d != 256;
+    if (!(d == 64 || d == 128 || d == 256) || page % 16 || g > (both ? 32 : 16) || !e4m3_cache(args + 6, nkv, d, device)) Py_RETURN_FALSE;
     for (int i = 3; i < 6; ++i)
       if (!vector_of_ints(THPVariable_Unpack(args[i]), device)) Py_RETURN_FALSE;
     const long long S = THPVariable_Unpack(args[4]).numel();
     if (S == 0 || THPVariable_Unpack(args[3]).numel() != S + 1 || table.size(0) < S || most < 0 || most > table.size(1) * page || q.dim() != 2 ||
         out.dim() != 2 || out.scalar_type() != q.scalar_type() || q.stride(1) != 1 || out.size(1) != nq * d || q.size(1) < nq * d ||
-        q.size(0) < out.size(0) || out.size(0) == 0 || !out.is_contiguous() || q.get_device() != device || out.get_device() != device)
+        q.size(0) < out.size(0) || out.size(0) == 0 || !out.is_contiguous() || q.get_device() != device || out.get_device() != device ||
+        ((uintptr_t)out.data_ptr() & 15))
       Py_RETURN_FALSE;
     const long long keys = window > 0 && window + 1 < most ? window + 1 : most;
+    const bool columns = both && keys >= 768 && S * nkv * keys * d >= 1 << 21;
+    Entry* e = (Entry*)args[columns ? 16 : 0];
+    if (!ready(e)) return nullptr;
     auto at_ = [&](int i) { return THPVariable_Unpack(args[i]).data_ptr(); };
     const cudaStream_t stream = stream_now();
     int rc;
     Py_BEGIN_ALLOW_THREADS
-    rc = reinterpret_cast<int (*)(void*, int, void*, void*, void*, void*, void*, int, void*, int, void*, void*, int, int, int, int, int, int, int,
-                                  int, int, int, float, void*, cudaStream_t)>(e->fn)(
-        q.data_ptr(), (int)q.stride(0), out.data_ptr(), at_(6), at_(7), at_(8), at_(9), dt, table.data_ptr(), (int)table.size(1), at_(3), at_(4), 0,
-        (int)S, 1, (int)keys, (int)nq, (int)nkv, (int)d, (int)page, (int)k.size(0), (int)window, scale, at_(5), stream);
+    if (columns)
+      rc = reinterpret_cast<int (*)(void*, int, void*, void*, void*, void*, void*, void*, int, void*, void*, int, int, int, int, int, int, int, int,
+                                    int, int, float, void*, cudaStream_t)>(e->fn)(
+          q.data_ptr(), (int)q.stride(0), out.data_ptr(), at_(6), at_(7), at_(8), at_(9), table.data_ptr(), (int)table.size(1), at_(3), at_(4), 0,
+          (int)S, 1, (int)keys, (int)nq, (int)nkv, (int)d, (int)page, (int)k.size(0), (int)window, scale, at_(5), stream);
+    else
+      rc = reinterpret_cast<int (*)(void*, int, void*, void*, void*, void*, void*, int, void*, int, void*, void*, int, int, int, int, int, int, int,
+                                    int, int, int, float, void*, cudaStream_t)>(e->fn)(
+          q.data_ptr(), (int)q.stride(0), out.data_ptr(), at_(6), at_(7), at_(8), at_(9), dt, table.data_ptr(), (int)table.size(1), at_(3), at_(4),
+          0, (int)S, 1, (int)keys, (int)nq, (int)nkv, (int)d, (int)page, (int)k.size(0), (int)window, scale, at_(5), stream);
     Py_END_ALLOW_THREADS
     if (!finish(rc, e->what)) return nullptr;
     Py_RETURN_TRUE;

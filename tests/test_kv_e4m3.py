@@ -100,13 +100,17 @@ def test_the_tests_own_rounding():
 
 
 @pytest.mark.parametrize("dtype,nq,nkv,d,page,scale,q,seqs,keys,form", [
-    (BF16, 32, 8, 64, 16, 0.1, 1, 64, 9000, "rows"), (BF16, 32, 8, 64, 16, 0.1, 8, 64, 9000, "rows"), (BF16, 32, 8, 64, 16, 0.1, 9, 8, 9000, "tcgen05"),
-    (BF16, 32, 8, 64, 16, 0.1, 32, 1, 9000, "rows"), (BF16, 32, 8, 64, 16, 0.1, 33, 1, 9000, "tcgen05"), (BF16, 32, 8, 128, 16, 0.1, 6, 8, 9000, "rows"),
-    (BF16, 32, 8, 128, 16, 0.1, 7, 8, 9000, "tcgen05"), (BF16, 32, 8, 128, 16, 0.1, 12, 1, 2000, "rows"), (BF16, 32, 8, 128, 16, 0.1, 12, 1, 4000, "tcgen05"),
+    (BF16, 32, 8, 64, 16, 0.1, 1, 64, 9000, "columns"), (BF16, 32, 8, 64, 16, 0.1, 8, 64, 9000, "columns"), (BF16, 32, 8, 64, 16, 0.1, 9, 8, 9000, "tcgen05"),
+    (BF16, 32, 8, 64, 16, 0.1, 1, 64, 767, "rows"), (BF16, 32, 8, 64, 16, 0.1, 1, 64, 768, "columns"), (BF16, 32, 8, 64, 16, 0.1, 1, 1, 4095, "rows"),
+    (BF16, 32, 8, 64, 16, 0.1, 1, 1, 4096, "columns"), (BF16, 32, 8, 128, 16, 0.1, 1, 1, 2048, "columns"), (BF16, 32, 8, 128, 16, 0.1, 1, 1, 2047, "rows"),
+    (BF16, 32, 8, 64, 16, 0.1, 32, 1, 9000, "rows"), (BF16, 32, 8, 64, 16, 0.1, 33, 1, 9000, "tcgen05"), (BF16, 32, 8, 128, 16, 0.1, 6, 8, 9000, "columns"),
+    (BF16, 32, 8, 128, 16, 0.1, 8, 8, 9000, "columns"), (BF16, 32, 8, 128, 16, 0.1, 9, 8, 9000, "tcgen05"), (BF16, 32, 8, 128, 16, 0.1, 32, 1, 4000, "columns"),
+    (BF16, 32, 8, 128, 16, 0.1, 33, 1, 4000, "tcgen05"), (BF16, 32, 8, 128, 16, 0.1, 12, 1, 700, "rows"), (BF16, 32, 8, 128, 16, -0.1, 6, 8, 9000, "columns"),
     (BF16, 32, 8, 64, 16, 0.1, 128, 1, 128, "tcgen05"), (BF16, 32, 8, 64, 16, 0.1, 129, 1, 129, "dense"), (BF16, 8, 8, 128, 16, 0.1, 513, 2, 600, "dense"),
     (BF16, 32, 8, 64, 8, 0.1, 1, 1, 100, "tcgen05"), (BF16, 32, 8, 64, 16, -0.1, 200, 1, 200, "rows"), (BF16, 32, 8, 96, 16, 0.1, 1, 1, 100, "simt"),
-    (BF16, 200, 1, 64, 16, 0.1, 1, 1, 100, "rows"), (torch.float32, 32, 8, 64, 16, 0.1, 300, 1, 300, "rows"), (torch.float32, 32, 8, 64, 8, 0.1, 3, 1, 300, "simt"),
-    (BF16, 8, 1, 256, 32, 0.1, 300, 1, 300, "rows")])
+    (BF16, 32, 8, 64, 8, 0.1, 1, 64, 9000, "tcgen05"), (BF16, 200, 1, 64, 16, 0.1, 1, 1, 100, "rows"), (torch.float32, 32, 8, 64, 16, 0.1, 1, 64, 9000, "rows"),
+    (torch.float32, 32, 8, 64, 16, 0.1, 300, 1, 300, "rows"), (torch.float32, 32, 8, 64, 8, 0.1, 3, 1, 300, "simt"),
+    (BF16, 8, 1, 256, 32, 0.1, 300, 1, 300, "rows"), (BF16, 8, 1, 256, 32, 0.1, 1, 64, 9000, "rows")])
 def test_which_kernel_a_call_takes(dtype, nq, nkv, d, page, scale, q, seqs, keys, form, monkeypatch):
     assert ops.attention_e4m3_form(dtype, nq, nkv, d, page, scale, q, seqs, keys) == form
     monkeypatch.setenv("RLLM_ATTENTION", "mma")

@@ -168,7 +168,10 @@ SHAPES = [  # nq, nkv, d, page, lens, starts, window
     (16, 4, 64, 16, [1, 96], [1200, 500], 512), (8, 8, 128, 16, [33], [1000], 0), (24, 8, 128, 16, [130], [0], 0),
     (32, 4, 64, 32, [200, 1 + 64], [1000, 3], 0), (32, 8, 64, 16, [300], [77], 64), (4, 4, 64, 16, [257], [255], 1),
     (3, 3, 48, 4, [9, 2], [3, 30], 0), (5, 1, 80, 1, [1, 4], [44, 2], 7), (4, 2, 16, 16, [3, 20], [0, 300], 0),
-    (8, 4, 96, 8, [1, 11], [5, 50], 0), (2, 1, 128, 7, [1, 30], [100, 9], 0), (6, 2, 32, 16, [1, 40], [600, 0], 33)]
+    (8, 4, 96, 8, [1, 11], [5, 50], 0), (2, 1, 128, 7, [1, 30], [100, 9], 0), (6, 2, 32, 16, [1, 40], [600, 0], 33),
+    (32, 8, 64, 16, [1] * 6, [5000, 0, 255, 256, 257, 1023], 0), (24, 8, 128, 16, [1] * 5, [4999, 127, 128, 129, 3], 0), (32, 8, 64, 16, [5, 1, 6, 8], [4000, 1, 255, 2000], 0),
+    (32, 8, 128, 48, [5, 1, 6, 8], [4000, 1, 255, 2000], 0), (16, 2, 64, 32, [1] * 12, [100 * i for i in range(12)], 900), (64, 2, 128, 16, [1] * 9, [900] * 9, 0),
+    (20, 4, 128, 16, [6] * 6, [1500, 30, 0, 700, 122, 1], 1000), (8, 8, 128, 16, [1] * 20, [150 * i for i in range(20)], 0)]
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
@@ -236,7 +239,7 @@ def test_pages_that_are_not_held_are_left_out_and_reported(dtype, lens, starts):
         st.check(out)
 
 
-FORMS = ["rows", "tcgen05", "dense"]
+FORMS = ["rows", "columns", "tcgen05", "dense"]
 
 
 @pytest.mark.parametrize("form", FORMS)
@@ -299,6 +302,44 @@ def test_rows_that_are_zeros_in_every_form(form, monkeypatch):
     out = st.attend(ops, num_decode=0)
     st.check(out)
     assert (out[40:43] == 0).all()
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("what", [math.nan, math.inf])
+def test_a_query_that_is_not_finite_reaches_its_own_row_alone(form, d, what, monkeypatch):
+    monkeypatch.setattr(ops, "attention_e4m3_form", lambda *a: form)
+    st = Step([5, 3], [300, 40], 8, 2, d, 16, BF16, seed=3)
+    plain = st.attend(ops, num_decode=0)
+    st.q[2, 3 * d + 7] = what
+    out = st.attend(ops, num_decode=0)
+    assert torch.isnan(out[2, 3 * d:4 * d]).all() and int(st.err) == 0
+    out[2, 3 * d:4 * d] = plain[2, 3 * d:4 * d]
+    assert torch.equal(out, plain)
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("d", [64, 128])
+def test_queries_whose_numbers_lie_far_apart(form, d, monkeypatch):
+    """A few of a row's numbers 2^10 and more above the others, rows up to 2^30 apart."""
+    monkeypatch.setattr(ops, "attention_e4m3_form", lambda *a: form)
+    for size in (1.0, 2.0 ** -20):
+        st = Step([6, 1], [500, 900], 8, 2, d, 16, BF16, seed=11, spread=0.5)
+        g = torch.Generator().manual_seed(2)
+        st.q.mul_(torch.exp(2.5 * torch.randn(st.q.shape, generator=g)).to(BF16).cuda() * (0.02 * size))
+        st.check(st.attend(ops, scale=d ** -0.5 / size, num_decode=0), scale=d ** -0.5 / size)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("lens,starts", [([1, 1], [60, 2000]), ([5], [100]), ([140], [60])])
+def test_results_off_16_bytes(dtype, lens, starts):
+    """out anywhere in a buffer: kernels that store 16 bytes are not the ones that take it."""
+    st = Step(lens, starts, 8, 2, 64, 16, dtype, seed=4)
+    buffer = torch.full((sum(lens) * 8 * 64 + 3,), 7.0, dtype=dtype, device="cuda")
+    out = buffer[1:-2].view(sum(lens), -1)
+    st.attend(ops, out=out)
+    st.check(out)
+    assert int(st.err) == 0 and float(buffer[0]) == 7 and (buffer[-2:] == 7).all()
 
 
 def test_prompts_in_groups_of_what_the_scratch_holds(monkeypatch):
@@ -406,15 +447,17 @@ class TheLongWay:
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
-@pytest.mark.parametrize("nq,nkv,d,rd,page,window", [(8, 2, 64, 64, 16, 0), (6, 2, 128, 64, 32, 20), (5, 1, 256, 0, 16, 0), (4, 4, 48, 48, 7, 9),
-                                                     (64, 1, 64, 64, 16, 0), (32, 1, 64, 64, 16, 33)])
-def test_calls_checked_in_one_go_and_the_long_way_give_the_same_bits(dtype, nq, nkv, d, rd, page, window, monkeypatch):
+@pytest.mark.parametrize("nq,nkv,d,rd,page,window,start", [
+    (8, 2, 64, 64, 16, 0, 100), (6, 2, 128, 64, 32, 20, 100), (5, 1, 256, 0, 16, 0, 100), (4, 4, 48, 48, 7, 9, 100), (64, 1, 64, 64, 16, 0, 100),
+    (32, 1, 64, 64, 16, 33, 100), (32, 1, 128, 64, 16, 0, 100), (32, 8, 64, 64, 16, 0, 1364), (32, 8, 64, 64, 16, 0, 1365), (16, 16, 128, 128, 16, 0, 766),
+    (16, 16, 128, 128, 16, 0, 767), (16, 16, 128, 128, 16, 767, 2000), (16, 16, 128, 128, 16, 766, 2000), (32, 1, 128, 64, 48, 0, 6000), (12, 4, 256, 64, 16, 0, 3000)])
+def test_calls_checked_in_one_go_and_the_long_way_give_the_same_bits(dtype, nq, nkv, d, rd, page, window, start, monkeypatch):
     results = []
     for long_way in (False, True):
         if long_way:
             module = TheLongWay(ops._launch())
             monkeypatch.setattr(ops, "_launch", lambda: module)
-        st = Step([1, 1, 1], [37, 100, 15], nq, nkv, d, page, dtype, seed=d, more_rows=1, stride_pad=16)
+        st = Step([1, 1, 1], [37, start, 15], nq, nkv, d, page, dtype, seed=d, more_rows=1, stride_pad=16)
         g = torch.Generator().manual_seed(1)
         qkv = torch.randn(3, (nq + 2 * nkv) * d, generator=g).to(dtype).cuda()
         cache = (st.k, st.v, st.ks, st.vs)
