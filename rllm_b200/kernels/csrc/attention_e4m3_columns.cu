@@ -35,12 +35,16 @@
 #define EC_SCORES 34.0f              // a score may pass its reference by 2^40: it is only for the sum of the weights, which is float32
 #define EC_NONE -3.0e38f             // the reference of a row that has seen nothing
 
-template <int D, int NB> struct EcShape {
+template <int D, int NB, bool MANY> struct EcShape {
   static constexpr int R = 8 * NB, QN = 16 * NB;                       // rows; columns of S
   static constexpr int PC = 2 * NB, PN = 16 * PC;                      // planes of 16 of the weights' columns: two terms of eight rows each
   static constexpr int PAR = 128 / D, TN = 128 * PAR, ON = PN * PAR;   // keys a line and a tile; columns of O
   static constexpr int CTAS = NB <= 2 ? 2 : 1, THREADS = 128 * NB + 32 + EC_PRODUCERS;       // of an SM
-  static constexpr int STAGES = NB > 2 ? (D == 128 ? 5 : 4) : D == 128 && NB == 1 ? 3 : 2;
+  // Two CTAs of two stages leave 50 KB of an SM, and one of three or four as much: the next kernel's CTAs come in beside them on every
+  // SM alike.  Where none fit, they gather on the SMs that are free first (a layer's two products, write and attention, 8 sequences of
+  // 2,048 keys, heads of 128: 52 us with three stages, 34 with two, 37 with the mma.sync kernel).  MANY: more CTAs than have room at a
+  // time keep memory busier with three (64 of 8,191: 172 -> 160 us).
+  static constexpr int STAGES = MANY ? 3 : NB == 3 || (NB == 4 && D == 128) ? 4 : NB == 4 ? 3 : 2;
   static constexpr int TILE = 128 * 128, P_BYTES = ON * 128, SLOT = 2 * TN;                  // SLOT: a tile's scales
   static constexpr int COLUMNS = 2 * QN * PAR + ON;
   static constexpr int TMEM = COLUMNS <= 64 ? 64 : COLUMNS <= 128 ? 128 : COLUMNS <= 256 ? 256 : 512;
@@ -121,13 +125,13 @@ template <bool MAX> __device__ __forceinline__ float ec_fold(const float* v, int
   return join(x[0], __shfl_xor_sync(0xffffffffu, x[0], 16));
 }
 
-template <int D, int NB>
-__global__ void __launch_bounds__(EcShape<D, NB>::THREADS, EcShape<D, NB>::CTAS)
+template <int D, int NB, bool MANY>
+__global__ void __launch_bounds__(EcShape<D, NB, MANY>::THREADS, EcShape<D, NB, MANY>::CTAS)
 attention_e4m3_columns_kernel(const bf16* q, int q_stride, bf16* __restrict__ out, const unsigned char* kcache, const unsigned char* vcache,
                               const unsigned char* kscale, const unsigned char* vscale, const int* __restrict__ block_table, int max_blocks, const int* __restrict__ q_start,
                               const int* __restrict__ seq_lens, int seq_begin, int nq, int nkv, int page_size, int num_pages, int window,
                               float scale_log2, int q_wide, int* __restrict__ err) {
-  typedef EcShape<D, NB> X;
+  typedef EcShape<D, NB, MANY> X;
   constexpr int R = X::R, NS = X::STAGES, PAR = X::PAR, PLANE = 128 * 16, TN = X::TN, MMA = 4 * NB;      // MMA: that warp
   extern __shared__ __align__(1024) unsigned char ec_raw[];
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31, tid = threadIdx.x;
@@ -557,17 +561,21 @@ attention_e4m3_columns_kernel(const bf16* q, int q_stride, bf16* __restrict__ ou
   if (C > 1) cluster.sync();                               // nobody leaves while its shared memory is being read
 }
 
-template <int D, int NB>
+template <int D, int NB, bool MANY = false>
 static int ec_launch(const void* q, int q_stride, void* out, const void* kcache, const void* vcache, const void* kscale, const void* vscale,
                      const int* block_table, int max_blocks, const int* q_start, const int* seq_lens, int seq_begin, int num_seqs,
                      int max_q_len, int max_keys, int nq, int nkv, int page_size, int num_pages, int window, float scale, int* err,
                      cudaStream_t stream) {
-  typedef EcShape<D, NB> X;
-  auto* kernel = attention_e4m3_columns_kernel<D, NB>;
-  static SmemLimit limit;
-  if (const int e = limit.allow(kernel, X::SMEM)) return e;
+  typedef EcShape<D, NB, MANY> X;
   const long long tiles = ((long long)max_q_len * (nq / nkv) + X::R - 1) / X::R, units = tiles * nkv * num_seqs;
   if (tiles * nkv > 65535 || num_seqs > 65535) return RLLM_E_UNSUPPORTED;
+  if constexpr (D == 128 && NB == 1 && !MANY)
+    if (units > 148 * X::CTAS)
+      return ec_launch<D, NB, true>(q, q_stride, out, kcache, vcache, kscale, vscale, block_table, max_blocks, q_start, seq_lens, seq_begin,
+                                    num_seqs, max_q_len, max_keys, nq, nkv, page_size, num_pages, window, scale, err, stream);
+  auto* kernel = attention_e4m3_columns_kernel<D, NB, MANY>;
+  static SmemLimit limit;
+  if (const int e = limit.allow(kernel, X::SMEM)) return e;
   // CTAs a unit: to fill the GPU's places, of a tile at least; clusters of eight do not fill a GPC's SMs (16 of them, a CTA an SM,
   // took two rounds)
   int C = 1;

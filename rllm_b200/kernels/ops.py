@@ -2197,7 +2197,7 @@ def attention_e4m3_form(dtype: torch.dtype, nq: int, nkv: int, d: int, page_size
     if dtype is torch.bfloat16 and d in (64, 128) and forced not in ("simt", "mma"):
         tiles = -(-rows // 32)
         few = tiles == 1 or num_seqs * nkv * tiles <= 32
-        if few and in_16s and (tiles == 1 or d == 128) and max_keys >= 768 and num_seqs * nkv * tiles * max_keys * d >= 1 << 21:
+        if few and in_16s and (tiles == 1 or d == 128) and max_keys >= 768 and num_seqs * nkv * tiles * max_keys >= (1 << 16 if d == 64 else 1 << 14):
             return "columns"
         if not (few and rows_take) and g <= 128 and scale > 0:
             return "tcgen05" if -(-max_q_len // (128 // g)) <= 4 else "dense"

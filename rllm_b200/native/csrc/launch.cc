@@ -430,7 +430,7 @@ PyObject* e4m3_decode(PyObject*, PyObject* const* args, Py_ssize_t n) {
         ((uintptr_t)out.data_ptr() & 15))
       Py_RETURN_FALSE;
     const long long keys = window > 0 && window + 1 < most ? window + 1 : most;
-    const bool columns = both && keys >= 768 && S * nkv * keys * d >= 1 << 21;
+    const bool columns = both && keys >= 768 && S * nkv * keys >= (d == 64 ? 1 << 16 : 1 << 14);
     Entry* e = (Entry*)args[columns ? 16 : 0];
     if (!ready(e)) return nullptr;
     auto at_ = [&](int i) { return THPVariable_Unpack(args[i]).data_ptr(); };

@@ -101,8 +101,8 @@ def test_the_tests_own_rounding():
 
 @pytest.mark.parametrize("dtype,nq,nkv,d,page,scale,q,seqs,keys,form", [
     (BF16, 32, 8, 64, 16, 0.1, 1, 64, 9000, "columns"), (BF16, 32, 8, 64, 16, 0.1, 8, 64, 9000, "columns"), (BF16, 32, 8, 64, 16, 0.1, 9, 8, 9000, "tcgen05"),
-    (BF16, 32, 8, 64, 16, 0.1, 1, 64, 767, "rows"), (BF16, 32, 8, 64, 16, 0.1, 1, 64, 768, "columns"), (BF16, 32, 8, 64, 16, 0.1, 1, 1, 4095, "rows"),
-    (BF16, 32, 8, 64, 16, 0.1, 1, 1, 4096, "columns"), (BF16, 32, 8, 128, 16, 0.1, 1, 1, 2048, "columns"), (BF16, 32, 8, 128, 16, 0.1, 1, 1, 2047, "rows"),
+    (BF16, 32, 8, 64, 16, 0.1, 1, 64, 767, "rows"), (BF16, 32, 8, 64, 16, 0.1, 1, 64, 768, "columns"), (BF16, 32, 8, 64, 16, 0.1, 1, 1, 8191, "rows"),
+    (BF16, 32, 8, 64, 16, 0.1, 1, 1, 8192, "columns"), (BF16, 32, 8, 128, 16, 0.1, 1, 1, 2048, "columns"), (BF16, 32, 8, 128, 16, 0.1, 1, 1, 2047, "rows"),
     (BF16, 32, 8, 64, 16, 0.1, 32, 1, 9000, "rows"), (BF16, 32, 8, 64, 16, 0.1, 33, 1, 9000, "tcgen05"), (BF16, 32, 8, 128, 16, 0.1, 6, 8, 9000, "columns"),
     (BF16, 32, 8, 128, 16, 0.1, 8, 8, 9000, "columns"), (BF16, 32, 8, 128, 16, 0.1, 9, 8, 9000, "tcgen05"), (BF16, 32, 8, 128, 16, 0.1, 32, 1, 4000, "columns"),
     (BF16, 32, 8, 128, 16, 0.1, 33, 1, 4000, "tcgen05"), (BF16, 32, 8, 128, 16, 0.1, 12, 1, 700, "rows"), (BF16, 32, 8, 128, 16, -0.1, 6, 8, 9000, "columns"),
