@@ -9,8 +9,10 @@
 // A page that the sequence does not hold sets bit 4 of the error word, and its keys are left out.
 //
 //   rows kernel   tensor cores (mma.sync m16n8k16, f16 operands): one (sequence, kv head) and up to 8 NB rows (a row is a
-//                 (token, head of the group) pair) a cluster of CTAs; see below.
-//   simt kernel   CUDA cores, one warp a (token, head): head sizes and pages that the rows kernel does not take.
+//                 (token, head of the group) pair) a cluster of CTAs; see below.  Few rows over few keys, float32, heads of 256.
+//   simt kernel   CUDA cores, one warp a (token, head): head sizes and pages that no other takes.
+// Few rows over many keys: attention_e4m3_columns.cu; more rows: attention_e4m3_tcgen05.cu; prompts: the widening kernel of
+// kv_e4m3.cu and attention_tcgen05.cu's DENSE form.
 #include "kv_e4m3.cuh"
 #include <cooperative_groups.h>
 #include <math.h>
@@ -144,7 +146,9 @@ static int e4_check(const void* q, const void* out, const void* kcache, const vo
 // 2^-31 of a weight of 1).  The denominator sums the weights themselves.
 // Queries are put into halves after a division by a power of two of the row's own (bfloat16: exact down to 2^-27 of the
 // row's largest; float32: two halves, 22 bits, and P likewise, with which the path is as good as float32 products).
-// What bounds it is memory: 16 keys of 128 dims are 4 KB a warp and 170 instructions, and warps load a tile ahead.
+// What bounds it: over few keys the start (780 instructions a warp beside its keys: queries, merge) and the latency of one or two
+// tiles, 4.5 us for 511 keys of 8 heads of 64; over many the instructions, 286 for 16 keys of 128 dims (4 KB), a third of them
+// conversions to halves at half the ALU's rate: 64 sequences of 8,191 keys, 8 heads of 128, 221 us, 4.9 TB/s.
 //
 // A cluster of C CTAs of 4 warps shares one (sequence, kv head, tile of rows): key tiles go round over the warps of the
 // cluster, partial results are merged in shared memory, first the CTA's, then, each CTA a slice, the cluster's (distributed

@@ -24,7 +24,12 @@
 // even keys (the lines' first 64 bytes) and the odd ones, and O too, of all 128 "dims" of a line, of which the halves that mix the
 // two are left where they are (the tensor core has time).
 // A cluster shares the keys of a (sequence, kv head, tile of rows); parts are merged in shared memory as in attention_e4m3.cu.
-#include "tcgen05.cuh"
+//
+// What bounds it: memory for heads of 128 (64 sequences of 8,191 keys, 8 kv heads of four rows: 159 us, 6.8 TB/s; the mma.sync kernel
+// 221).  For heads of 64 a key has half the bytes and the same work for a thread, 40 cycles of exponentials, conversions and
+// additions a (key, row) pair over four warps: 99 us, 5.4 TB/s (118), and 24 us for 32 rows of 8 sequences of 4,095 (32).  Over few keys
+// the way to the first tile's result, 6 us, is longer than the mma.sync kernel's.
+#include "attention_tcgen05.cuh"
 #include "kv_e4m3.cuh"
 #include <cooperative_groups.h>
 #include <math.h>
@@ -53,10 +58,10 @@ template <int D, int NB, bool MANY> struct EcShape {
   static_assert(PAR * R * D * 4 <= 2 * STAGES * TILE, "the parts lie where keys and values were");
 };
 
-__device__ __forceinline__ float ec_ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
+__device__ __forceinline__ unsigned long long ec_mul2(unsigned long long a, unsigned long long b) {
+  unsigned long long d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
 }
 __device__ __forceinline__ unsigned ec_e4m3(unsigned halves) {          // two halves as e4m3, the low one in the low byte
   unsigned short r;
@@ -158,8 +163,9 @@ attention_e4m3_columns_kernel(const bf16* q, int q_stride, bf16* __restrict__ ou
   unsigned long long *s_full = bars + 32, *p_full = bars + 34, *pv_full = bars + 36, *q_full = bars + 38;  // [2] each, q_full one
   unsigned* tmem_slot = (unsigned*)(bars + 39);
   unsigned* held = (unsigned*)(bars + 40);                 // [2 NS]: a bit for every 16 keys that were brought
-  float4* info = (float4*)((unsigned char*)bars + 448);    // [R]: a row's factor, its scores' reference m, its weights', m + EC_SCORES
-  float2* moved = (float2*)(info + R);                     // [R]: what the row's sum and its output are multiplied by
+  // every eight rows' factors f, and, negative, their scores' references m, their weights' t, and m + EC_SCORES: [NB][4][8]
+  float* info = (float*)((unsigned char*)bars + 448);
+  float2* moved = (float2*)(info + 4 * R);                     // [R]: what the row's sum and its output are multiplied by
   int2* sight = (int2*)(moved + R);                        // [R]: the first key it sees, and the one behind its last
   float2* tops = (float2*)(sight + R);                     // [4][R]: the warps' largest score and weight; at the end their sums
   float* cM = (float*)(tops + 4 * R);                      // [3][R]: the CTA's references and sum
@@ -186,7 +192,12 @@ attention_e4m3_columns_kernel(const bf16* q, int q_stride, bf16* __restrict__ ou
 
   if (warp < MMA) {
     const int group = warp >> 2, quarter = warp & 3, line = tid & 127;
-    float l[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    typedef unsigned long long pair;                       // two rows' numbers, for instructions that take two
+    pair l[4] = {0ull, 0ull, 0ull, 0ull};
+    auto notes = [&](int what, pair (&x)[4]) {             // 0: f, 1: -m, 2: -t, 3: -(m + EC_SCORES)
+      *(ulonglong2*)&x[0] = *(const ulonglong2*)(info + what * 8);
+      *(ulonglong2*)&x[2] = *(const ulonglong2*)(info + what * 8 + 4);
+    };
     pdl_wait_on(q);
     pdl_launch();
     // queries: L lanes a row, 16 numbers each
@@ -237,7 +248,9 @@ attention_e4m3_columns_kernel(const bf16* q, int q_stride, bf16* __restrict__ ou
           *(uint4*)(sQ + col * D + ((D == 128 ? c ^ (col & 7) : c ^ (col >> 1 & 3)) << 4)) = make_uint4(w[term][0], w[term][1], w[term][2], w[term][3]);
         }
         if (c == 0) {
-          info[r] = make_float4(__uint_as_float((unsigned)(127 - 7 + e) << 23) * scale_log2 + odd, EC_NONE, EC_NONE, EC_NONE);
+          float* note = info + (r >> 3) * 32 + (r & 7);
+          note[0] = __uint_as_float((unsigned)(127 - 7 + e) << 23) * scale_log2 + odd;
+          note[8] = note[16] = note[24] = -EC_NONE;
           const int hi = pos0 + min(at, rows - 1) / g + 1;
           sight[r] = make_int2(window > 0 ? hi - window : 0, hi);
         }
@@ -248,7 +261,7 @@ attention_e4m3_columns_kernel(const bf16* q, int q_stride, bf16* __restrict__ ou
     if (lane == 0) mbar_arrive(q_full);
     asm volatile("bar.sync 5, %0;" ::"n"(128 * NB) : "memory");         // (the rows' notes, of all warps)
 
-    info += group * 8; moved += group * 8; sight += group * 8; tops += group * 32;
+    info += group * 32; moved += group * 8; sight += group * 8; tops += group * 32;
     const unsigned lane_sel = (unsigned)(quarter * 32) << 16;
     // this thread's half of O: even or odd keys' sums, and its rows' columns
     const unsigned my_o = tmem_o + lane_sel + (PAR == 2 ? (quarter >> 1) * X::PN : 0) + group * 32;
@@ -257,7 +270,8 @@ attention_e4m3_columns_kernel(const bf16* q, int q_stride, bf16* __restrict__ ou
       // (the tile's scores are there, so its keys and scales are, and the products issued before: the weights' place is free)
       ok = ok && __all_sync(0xffffffffu, mbar_wait(&s_full[buf], (it >> 1) & 1, err));
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      float sc[PAR][8], kf[PAR], ev[PAR];
+      pair sc[PAR][4], ev[PAR];
+      float kf[PAR];
       {
         float x[PAR][16];
 #pragma unroll
@@ -266,7 +280,8 @@ attention_e4m3_columns_kernel(const bf16* q, int q_stride, bf16* __restrict__ ou
 #pragma unroll
         for (int u = 0; u < PAR; ++u)
 #pragma unroll
-          for (int r = 0; r < 8; ++r) sc[u][r] = fmaf(x[u][8 + r], 1.0f / 32, x[u][r]);
+          for (int i = 0; i < 4; ++i)
+            sc[u][i] = at_fma2(at_pack2(x[u][8 + 2 * i], x[u][9 + 2 * i]), at_pack2(1.0f / 32, 1.0f / 32), at_pack2(x[u][2 * i], x[u][2 * i + 1]));
       }
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       const bool brought = held[slot] >> (line * PAR >> 4) & 1u;
@@ -276,59 +291,78 @@ attention_e4m3_columns_kernel(const bf16* q, int q_stride, bf16* __restrict__ ou
         const int kb = sS[slot * X::SLOT + line * PAR + u], vb = sS[slot * X::SLOT + TN + line * PAR + u];
         // 2^ek (255: infinity, which makes NaN of the row's zeros), NaN where the value is NaN; ev
         kf[u] = vb == KV8_NAN_SCALE ? __uint_as_float(0x7FC00000u) : __uint_as_float((unsigned)kb << 23);
-        ev[u] = (float)(vb - 127);
+        ev[u] = at_pack2((float)(vb - 127), (float)(vb - 127));
         readable[u] = brought && j + u >= kmin && j + u < kend;
         all_readable = all_readable && readable[u];
       }
       all_readable = __all_sync(0xffffffffu, all_readable);
+      {
+        pair f[4];
+        notes(0, f);
 #pragma unroll
-      for (int r = 0; r < 8; ++r) {
-        const float f = info[r].x;
+        for (int u = 0; u < PAR; ++u)
 #pragma unroll
-        for (int u = 0; u < PAR; ++u) sc[u][r] = sc[u][r] * f * kf[u];
+          for (int i = 0; i < 4; ++i) sc[u][i] = ec_mul2(ec_mul2(sc[u][i], f[i]), at_pack2(kf[u], kf[u]));
       }
       if (!(j0 >= lo_last && j0 + TN <= hi_first && all_readable)) {
 #pragma unroll
-        for (int r = 0; r < 8; ++r) {
-          const int2 see = sight[r];
+        for (int i = 0; i < 4; ++i) {
+          const int2 s0 = sight[2 * i], s1 = sight[2 * i + 1];
 #pragma unroll
-          for (int u = 0; u < PAR; ++u)
-            if (!(readable[u] && j + u >= see.x && j + u < see.y)) sc[u][r] = -INFINITY;
+          for (int u = 0; u < PAR; ++u) {
+            float a, b;
+            at_unpack2(sc[u][i], a, b);
+            sc[u][i] = at_pack2(readable[u] && j + u >= s0.x && j + u < s0.y ? a : -INFINITY, readable[u] && j + u >= s1.x && j + u < s1.y ? b : -INFINITY);
+          }
         }
       }
-      float over = EC_NONE;                                // how far a score or a weight passes its reference
+      float over = EC_NONE, over2 = EC_NONE;               // how far a score or a weight passes its reference
+      {
+        pair t[4], lim[4];
+        notes(2, t);
+        notes(3, lim);
 #pragma unroll
-      for (int r = 0; r < 8; ++r) {
-        const float4 f = info[r];
+        for (int u = 0; u < PAR; ++u)
 #pragma unroll
-        for (int u = 0; u < PAR; ++u) over = fmaxf(over, fmaxf(sc[u][r] - f.w, sc[u][r] + ev[u] - f.z));
+          for (int i = 0; i < 4; ++i) {
+            float a, b, c, d;
+            at_unpack2(at_add2(sc[u][i], lim[i]), a, b);
+            at_unpack2(at_add2(sc[u][i], at_add2(ev[u], t[i])), c, d);
+            over = at_max3(over, a, b);
+            over2 = at_max3(over2, c, d);
+          }
       }
-      if (ec_any(group, over > EC_SLACK)) {
+      if (ec_any(group, fmaxf(over, over2) > EC_SLACK)) {
         float top[8], wt[8];
 #pragma unroll
-        for (int r = 0; r < 8; ++r) {
-          top[r] = sc[0][r];
-          wt[r] = sc[0][r] + ev[0];
-          if (PAR == 2) { top[r] = fmaxf(top[r], sc[PAR - 1][r]); wt[r] = fmaxf(wt[r], sc[PAR - 1][r] + ev[PAR - 1]); }
+        for (int i = 0; i < 4; ++i) {
+          at_unpack2(sc[0][i], top[2 * i], top[2 * i + 1]);
+          at_unpack2(at_add2(sc[0][i], ev[0]), wt[2 * i], wt[2 * i + 1]);
+          if (PAR == 2) {
+            float a, b, c, d;
+            at_unpack2(sc[PAR - 1][i], a, b);
+            at_unpack2(at_add2(sc[PAR - 1][i], ev[PAR - 1]), c, d);
+            top[2 * i] = fmaxf(top[2 * i], a); top[2 * i + 1] = fmaxf(top[2 * i + 1], b);
+            wt[2 * i] = fmaxf(wt[2 * i], c); wt[2 * i + 1] = fmaxf(wt[2 * i + 1], d);
+          }
         }
         int at;
         const float a = ec_fold<true>(top, lane, &at), b = ec_fold<true>(wt, lane, &at);
         if (lane < 8) tops[quarter * 8 + at] = make_float2(a, b);
         ec_sync(group);
         if (line < 8) {
-          float4 f = info[line];
           float2 t = tops[line];
 #pragma unroll
           for (int w = 1; w < 4; ++w) { t.x = fmaxf(t.x, tops[w * 8 + line].x); t.y = fmaxf(t.y, tops[w * 8 + line].y); }
           float2 by = make_float2(1.f, 1.f);
-          if (t.x > f.w + EC_SLACK) { by.x = ec_ex2(f.y - t.x); f.y = t.x; f.w = t.x + EC_SCORES; }
-          if (t.y > f.z + EC_SLACK) { by.y = ec_ex2(f.z - t.y); f.z = t.y; }
-          info[line] = f;
+          float* note = info + line;
+          if (t.x + note[24] > EC_SLACK) { by.x = at_ex2(-note[8] - t.x); note[8] = -t.x; note[24] = -(t.x + EC_SCORES); }
+          if (t.y + note[16] > EC_SLACK) { by.y = at_ex2(-note[16] - t.y); note[16] = -t.y; }
           moved[line] = by;
         }
         ec_sync(group);
 #pragma unroll
-        for (int r = 0; r < 8; ++r) l[r] *= moved[r].x;
+        for (int i = 0; i < 4; ++i) l[i] = ec_mul2(l[i], at_pack2(moved[2 * i].x, moved[2 * i + 1].x));
         if (it > 0) {                                      // the product of the tile before has to be through: it writes what is rescaled
           ok = ok && __all_sync(0xffffffffu, mbar_wait(&pv_full[buf ^ 1], ((it - 1) >> 1) & 1, err));
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -345,23 +379,24 @@ attention_e4m3_columns_kernel(const bf16* q, int q_stride, bf16* __restrict__ ou
           asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
         }
       }
+      pair m[4], t_[4];
+      notes(1, m);
+      notes(2, t_);
 #pragma unroll
       for (int u = 0; u < PAR; ++u) {
         unsigned terms[4][4];
+        const pair up = at_add2(ev[u], at_pack2(EC_SHIFT, EC_SHIFT));
 #pragma unroll
-        for (int r = 0; r < 8; r += 2) {
-          float w[2];
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            const float4 f = info[r + k];
-            l[r + k] += ec_ex2(sc[u][r + k] - f.y);
-            w[k] = ec_ex2(sc[u][r + k] + (ev[u] - f.z + EC_SHIFT));
-          }
-          __half2 h = __floats2half2_rn(w[0], w[1]);
+        for (int i = 0; i < 4; ++i) {
+          float a, b, c, d;
+          at_unpack2(at_add2(sc[u][i], m[i]), a, b);
+          at_unpack2(at_add2(sc[u][i], at_add2(up, t_[i])), c, d);
+          l[i] = at_add2(l[i], at_pack2(at_ex2(a), at_ex2(b)));
+          __half2 h = __floats2half2_rn(at_ex2(c), at_ex2(d));
 #pragma unroll
           for (int t = 0; t < 4; ++t) {
-            terms[t][r / 2] = ec_e4m3(*(const unsigned*)&h);
-            const unsigned b = kv8_halves((unsigned short)terms[t][r / 2]);
+            terms[t][i] = ec_e4m3(*(const unsigned*)&h);
+            const unsigned b = kv8_halves((unsigned short)terms[t][i]);
             h = __hmul2(__hsub2(h, *(const __half2*)&b), __float2half2_rn(32.f));
           }
         }
@@ -386,15 +421,18 @@ attention_e4m3_columns_kernel(const bf16* q, int q_stride, bf16* __restrict__ ou
     if (n > 0) ok = ok && __all_sync(0xffffffffu, mbar_wait(&pv_full[(n - 1) & 1], ((n - 1) >> 1) & 1, err));
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     int at;
-    const float sum = ec_fold<false>(l, lane, &at);
+    float sums[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) at_unpack2(l[i], sums[2 * i], sums[2 * i + 1]);
+    const float sum = ec_fold<false>(sums, lane, &at);
     if (lane < 8) tops[quarter * 8 + at].x = sum;
     ec_sync(group);
     if (line < 8) {
       float all = 0.f;
 #pragma unroll
       for (int w = 0; w < 4; ++w) all += tops[w * 8 + line].x;
-      cM[group * 8 + line] = info[line].y;
-      cM[R + group * 8 + line] = info[line].z;
+      cM[group * 8 + line] = -info[8 + line];
+      cM[R + group * 8 + line] = -info[16 + line];
       cM[2 * R + group * 8 + line] = all;
     }
     // O, its terms added up, as float32 rows [PAR][R][D] where keys and values were (all of them have been read)
@@ -549,11 +587,11 @@ attention_e4m3_columns_kernel(const bf16* q, int q_stride, bf16* __restrict__ ou
       }
       for (int c = 0; c < C; ++c) {
         const float* m = cluster.map_shared_rank(cM, c);
-        sum = fmaf(m[2 * R + r], ec_ex2(m[r] - top), sum);
-        add(cluster.map_shared_rank((const float*)ec_raw, c), ec_ex2(m[R + r] - high));
+        sum = fmaf(m[2 * R + r], at_ex2(m[r] - top), sum);
+        add(cluster.map_shared_rank((const float*)ec_raw, c), at_ex2(m[R + r] - high));
       }
     }
-    const float inv = sum == 0.f ? 0.f : 1.0f / sum, by = ec_ex2(high - top - EC_SHIFT);      // NaN stays NaN
+    const float inv = sum == 0.f ? 0.f : 1.0f / sum, by = at_ex2(high - top - EC_SHIFT);      // NaN stays NaN
     const int tok = at / g;
     const __nv_bfloat162 lo = __floats2bfloat162_rn(x.x * inv * by, x.y * inv * by), hi = __floats2bfloat162_rn(x.z * inv * by, x.w * inv * by);
     *(uint2*)(out + ((size_t)(qs + tok) * nq + kvh * g + at - tok * g) * D + col) = make_uint2(*(const unsigned*)&lo, *(const unsigned*)&hi);

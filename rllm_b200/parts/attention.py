@@ -52,7 +52,7 @@ reads, q'_h = [sum over the heads g of kv head 0 of talk[h, g] q_g | ... | of th
 mixed score (``kernels/csrc/talking_heads.cu``); the pages keep that row and the values of all kv heads side by side.
 
 Where the engine keeps its cache in 8 bits (``KVCacheView.k_scale``), the Llama's form goes through the kernels of
-``kernels/csrc/kv_e4m3.cu`` and ``attention_e4m3.cu``: one writes the tokens' rows, the attention reads them back from there.  The
+``kernels/csrc/kv_e4m3.cu`` and ``attention_e4m3*.cu``: one writes the tokens' rows, the attention reads them back from there.  The
 other options have no such form (``no_8_bit_cache``).
 
 A position part that rotates pairs (2i, 2i + 1) is served by the same kernels, which rotate halves: the rows of
