@@ -2164,6 +2164,7 @@ def kv_read_e4m3(positions: torch.Tensor, token_seq: torch.Tensor, block_table: 
                                dt, T, nkv, d, page_size, pages, err)
 
 
+E4M3_FORMS = None                   # two names in place of attention_e4m3_form's: for single tokens, for the others
 E4M3_DENSE_SCRATCH = 512 << 20      # bytes of widened keys and values at a time; more only where one sequence needs more
 
 
@@ -2191,17 +2192,7 @@ def attention_e4m3_form(dtype: torch.dtype, nq: int, nkv: int, d: int, page_size
         17.2 and 16.6 / 18.4); 8 of 4,095, 64 rows 44 / 38, 128 rows 86 / 45;
       tcgen05 / dense, heads of 64: 4 of 16,000, 4 tiles of 128 rows 182 / 240, 6 tiles 340 / 287, 16 tiles 682 / 518; heads of
         128: 216 / 353, 406 / 381, 798 / 666."""
-    g, forced = nq // nkv, os.environ.get("RLLM_ATTENTION")
-    rows, in_16s = max_q_len * g, page_size % 16 == 0 and forced != "simt"
-    rows_take = in_16s and d in (64, 128, 256) and -(-rows // 8) * nkv <= 65535
-    if dtype is torch.bfloat16 and d in (64, 128) and forced not in ("simt", "mma"):
-        tiles = -(-rows // 32)
-        few = tiles == 1 or num_seqs * nkv * tiles <= 32
-        if few and in_16s and (tiles == 1 or d == 128) and max_keys >= 768 and num_seqs * nkv * tiles * max_keys >= (1 << 16 if d == 64 else 1 << 14):
-            return "columns"
-        if not (few and rows_take) and g <= 128 and scale > 0:
-            return "tcgen05" if -(-max_q_len // (128 // g)) <= 4 else "dense"
-    return "rows" if rows_take else "simt"
+    return _launch().e4m3_form(dtype is torch.bfloat16, nq, nkv, d, page_size, scale, max_q_len, num_seqs, max_keys)
 
 
 def attention_e4m3(q: torch.Tensor, out: torch.Tensor, kcache: torch.Tensor, vcache: torch.Tensor, kscale: torch.Tensor,
@@ -2215,57 +2206,18 @@ def attention_e4m3(q: torch.Tensor, out: torch.Tensor, kcache: torch.Tensor, vca
     the first ``num_decode`` sequences bring one token each.  ``max_q_len`` and ``max_seq_len`` bound every sequence's tokens
     in this step and in the cache.  Rows behind the last sequence's stay as they are.  A page that is not held sets bit 4 of
     ``err``, and its keys are left out."""
-    if num_decode == seq_lens.numel() and max_q_len >= 0 and \
-            _launch().e4m3_decode(_entries.rllm_attention_e4m3_rows, q, out, q_start, seq_lens, err, kcache, vcache, kscale, vscale,
-                                  block_table, max_seq_len, nq, nkv, window, scale, _entries.rllm_attention_e4m3_columns):
+    entries = (_entries.rllm_attention_e4m3_rows, _entries.rllm_attention_e4m3_columns, _entries.rllm_attention_e4m3_tcgen05,
+               _entries.rllm_attention_e4m3_simt, _entries.rllm_kv_e4m3_widen, _entries.rllm_attention_dense_tcgen05)
+    if _launch().e4m3_attention(entries, q, out, q_start, seq_lens, err, kcache, vcache, kscale, vscale, block_table, num_decode, max_q_len,
+                                max_seq_len, nq, nkv, window, scale, E4M3_DENSE_SCRATCH, E4M3_FORMS):
         return
-    dt = dtype_code(q.dtype)
+    dtype_code(q.dtype)
     S, d = seq_lens.numel(), kcache.shape[-1]
     if q.dim() != 2 or out.dim() != 2 or out.dtype is not q.dtype:
         raise KernelError("attention_e4m3: q must be [T, >= nq d] and out [T, nq d] of one type")
-    (T, width), stride = out.shape, q.stride(0)
-    if q.stride(1) != 1 or width != nq * d or q.shape[1] < width or q.shape[0] < T or not out.is_contiguous():
+    if q.stride(1) != 1 or out.shape[1] != nq * d or q.shape[1] < nq * d or q.shape[0] < out.shape[0] or not out.is_contiguous():
         raise KernelError("attention_e4m3: q must be [T, >= nq d] and out [T, nq d] of one type, their rows contiguous")
     _e4m3_cache(kcache, vcache, kscale, vscale, block_table, nkv, d, q_start, seq_lens, err)
     _beside(kcache, q, out)
-    pages, _, page_size, _ = kcache.shape
-    seqs, blocks = block_table.shape
-    if q_start.numel() != S + 1 or not 0 <= num_decode <= S or seqs < S or max_q_len < 0 or not 0 <= max_seq_len <= blocks * page_size:
-        raise KernelError("attention_e4m3: q_start [S + 1] and seq_lens [S], num_decode of them with one token, a row of block_table "
-                          "each, that can hold max_seq_len tokens")
-    if T == 0 or S == 0:
-        return
-    cache = (kcache, vcache, kscale, vscale, dt, block_table, blocks, q_start, seq_lens)
-    heads = (nq, nkv, d, page_size, pages, window, scale, err)
-    keys = max_seq_len if window <= 0 else min(max_seq_len, window + max_q_len)
-    for first, end, longest in ((0, num_decode, 1), (num_decode, S, max_q_len)):
-        if first == end or longest == 0:
-            continue
-        form = attention_e4m3_form(q.dtype, nq, nkv, d, page_size, scale, longest, end - first, keys)
-        if out.data_ptr() % 16:
-            form = "simt"
-        elif form in ("tcgen05", "dense") and (stride % 8 or q.data_ptr() % 16):
-            form = "rows" if page_size % 16 == 0 else "simt"
-        if form == "rows":
-            _entries.rllm_attention_e4m3_rows(q, stride, out, *cache, first, end, longest, keys, *heads)
-        elif form == "columns":
-            _entries.rllm_attention_e4m3_columns(q, stride, out, kcache, vcache, kscale, vscale, block_table, blocks, q_start,
-                                                 seq_lens, first, end, longest, keys, *heads)
-        elif form == "tcgen05":
-            _entries.rllm_attention_e4m3_tcgen05(q, stride, out, kcache, vcache, kscale, vscale, block_table, blocks, q_start,
-                                                 seq_lens, first, end, longest, keys, *heads)
-        elif form == "simt":
-            _entries.rllm_attention_e4m3_simt(q, stride, out, *cache, first, end, min(T, (end - first) * longest), *heads)
-        else:
-            bn = 8192 // d
-            tiles = keys // bn + 2
-            a_sequence = 2 * tiles * nkv * bn * d
-            group = max(1, min(end - first, E4M3_DENSE_SCRATCH // (2 * a_sequence), 65535))
-            dense = torch.empty((2, group * a_sequence // 2), dtype=torch.bfloat16, device=q.device)
-            marks = torch.empty(group * tiles * nkv * 8, dtype=torch.int32, device=q.device)
-            for s in range(first, end, group):
-                n = min(group, end - s)
-                _entries.rllm_kv_e4m3_widen(block_table, blocks, q_start, seq_lens, s, n, tiles, kcache, vcache, kscale, vscale,
-                                            dense[0], dense[1], marks, nkv, d, page_size, pages, window, err)
-                _entries.rllm_attention_dense_tcgen05(q, stride, q.shape[0], out, dense[0], dense[1], marks, tiles, q_start,
-                                                      seq_lens, s, n, min(T, n * longest), nq, nkv, d, window, scale, err)
+    raise KernelError("attention_e4m3: nq a multiple of nkv, q_start [S + 1] and seq_lens [S], num_decode of them with one token, a row of "
+                      "block_table each, that can hold max_seq_len tokens")

@@ -17,6 +17,7 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
 #include <cstdlib>
 #include <cstring>
 #include <tuple>
@@ -322,8 +323,8 @@ PyObject* e4m3_ready(PyObject*, PyObject* const* args, Py_ssize_t n) {
   });
 }
 
-// The three operators' common calls, checked and launched in one go: True, or False where Python's own way has to look (and
-// refuse, or take the call another way).  Each is given its entry point first.
+// The operators' calls, checked and launched in one go: True, or False where Python has to look (and refuse, or take the call its
+// own way).  Each is given its entry points first.
 int float_code(const at::Tensor& t) { return t.scalar_type() == at::kBFloat16 ? 1 : t.scalar_type() == at::kFloat ? 0 : -1; }
 
 // e4m3_write(entry, qkv, q_out or None, positions, token_seq, err, kcache, vcache, kscale, vscale, block_table, inv_freq or None, rotary_dim,
@@ -402,53 +403,156 @@ PyObject* e4m3_read(PyObject*, PyObject* const* args, Py_ssize_t n) {
   });
 }
 
-// e4m3_decode(rows entry, q, out, q_start, seq_lens, err, kcache, vcache, kscale, vscale, block_table, max_seq_len, nq, nkv, window,
-// scale, columns entry): every sequence brings one token, and one of the two kernels takes it, by the rule of attention_e4m3_form in
-// rllm_b200/kernels/ops.py
-PyObject* e4m3_decode(PyObject*, PyObject* const* args, Py_ssize_t n) {
-  if (n != 17 || Py_TYPE(args[0]) != &EntryType || Py_TYPE(args[16]) != &EntryType)
-    return PyErr_Format(PyExc_TypeError, "e4m3_decode(entry, ... 15 arguments, entry)");
+// Which kernel takes an attention over such a cache: the rule of ops.attention_e4m3_form, whose text has both sides of every limit
+// as measured.
+enum Form { kRows, kColumns, kTcgen05, kDense, kSimt, kForms };
+const char* const kFormNames[kForms] = {"rows", "columns", "tcgen05", "dense", "simt"};
+
+Form e4m3_rule(bool bf16, long long nq, long long nkv, long long d, long long page, double scale, long long max_q_len, long long seqs,
+               long long keys) {
+  const char* forced = std::getenv("RLLM_ATTENTION");
+  const long long g = nq / nkv, rows = max_q_len * g;
+  const bool simt = is(forced, "simt"), in_16s = page % 16 == 0 && !simt, heads = d == 64 || d == 128;
+  const bool rows_take = in_16s && (heads || d == 256) && (rows + 7) / 8 * nkv <= 65535;
+  if (bf16 && heads && !simt && !is(forced, "mma")) {
+    const long long tiles = (rows + 31) / 32;
+    const bool few = tiles == 1 || seqs * nkv * tiles <= 32;
+    if (few && in_16s && (tiles == 1 || d == 128) && tiles * nkv <= 65535 && keys >= 768 && seqs * nkv * tiles * keys >= (d == 64 ? 1 << 16 : 1 << 14))
+      return kColumns;
+    if (!(few && rows_take) && g <= 128 && scale > 0) {
+      const long long tokens = 128 / g;                    // of a tile of 128 rows
+      return (max_q_len + tokens - 1) / tokens <= 4 ? kTcgen05 : kDense;
+    }
+  }
+  return rows_take ? kRows : kSimt;
+}
+
+// e4m3_form(bfloat16, nq, nkv, d, page_size, scale, max_q_len, num_seqs, max_keys)
+PyObject* e4m3_form(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (n != 9) return PyErr_Format(PyExc_TypeError, "e4m3_form(bfloat16, nq, nkv, d, page_size, scale, max_q_len, num_seqs, max_keys)");
+  bool bad = false;
+  long long v[9];
+  for (int i = 0; i < 9; ++i) v[i] = i == 5 || bad ? 0 : whole(args[i], bad);
+  const double scale = bad ? 0. : PyFloat_AsDouble(args[5]);
+  if (bad || PyErr_Occurred()) return nullptr;
+  if (v[1] <= 0 || v[2] <= 0 || v[1] % v[2]) return PyErr_Format(g_error, "%lld query heads over %lld kv heads", v[1], v[2]);
+  return PyUnicode_FromString(kFormNames[e4m3_rule(v[0] != 0, v[1], v[2], v[3], v[4], scale, v[6], v[7], v[8])]);
+}
+
+// e4m3_attention(entries, q, out, q_start, seq_lens, err, kcache, vcache, kscale, vscale, block_table, num_decode, max_q_len,
+//                max_seq_len, nq, nkv, window, scale, scratch, forms): checked and launched.  entries: (rows, columns, tcgen05, simt, widen,
+// dense); scratch: bytes of widened keys and values at a time; forms: None, or two names (for the single tokens, for the others) in
+// place of the rule's.  False: a call that has to be refused, ops.attention_e4m3 says why.
+PyObject* e4m3_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  enum { kEntries = 6 };
+  if (n != 20 || !PyTuple_Check(args[0]) || PyTuple_GET_SIZE(args[0]) != kEntries)
+    return PyErr_Format(PyExc_TypeError, "e4m3_attention((entries), ... 19 arguments)");
+  Entry* e[kEntries];
+  for (int i = 0; i < kEntries; ++i) {
+    PyObject* x = PyTuple_GET_ITEM(args[0], i);
+    if (Py_TYPE(x) != &EntryType) return PyErr_Format(PyExc_TypeError, "entries are wanted first");
+    e[i] = (Entry*)x;
+  }
+  int named[2] = {-1, -1};
+  if (args[19] != Py_None) {
+    if (!PyTuple_Check(args[19]) || PyTuple_GET_SIZE(args[19]) != 2) return PyErr_Format(PyExc_TypeError, "forms: None or two names");
+    for (int i = 0; i < 2; ++i) {
+      const char* text = PyUnicode_Check(PyTuple_GET_ITEM(args[19], i)) ? PyUnicode_AsUTF8(PyTuple_GET_ITEM(args[19], i)) : nullptr;
+      for (int f = 0; text && f < kForms; ++f)
+        if (!std::strcmp(text, kFormNames[f])) named[i] = f;
+      if (named[i] < 0) return PyErr_Occurred() ? nullptr : PyErr_Format(g_error, "no form of that name");
+    }
+  }
   if (!cuda_tensors(args + 1, 10)) Py_RETURN_FALSE;
   return guarded([&]() -> PyObject* {
     bool bad = false;
-    const long long most = whole(args[11], bad), nq = whole(args[12], bad), nkv = whole(args[13], bad), window = whole(args[14], bad);
-    const float scale = bad ? 0.f : Arg<'f'>::get(args[15], bad);
-    if (bad) return nullptr;
+    long long v[8];                                        // num_decode, max_q_len, max_seq_len, nq, nkv, window, -, scratch
+    for (int i = 0; i < 8 && !bad; ++i) v[i] = i == 6 ? 0 : whole(args[11 + i], bad);
+    const double scale = bad ? 0. : PyFloat_AsDouble(args[17]);
+    if (bad || PyErr_Occurred()) return nullptr;
+    const long long decode = v[0], max_q = v[1], most = v[2], nq = v[3], nkv = v[4], window = v[5], scratch = v[7];
     const at::Tensor &q = THPVariable_Unpack(args[1]), &out = THPVariable_Unpack(args[2]), &k = THPVariable_Unpack(args[6]),
                      &table = THPVariable_Unpack(args[10]);
     const int device = c10::cuda::current_device(), dt = float_code(q);
-    if (dt < 0 || k.dim() != 4 || nq <= 0 || nkv <= 0 || nkv > 16383 || nq % nkv || std::getenv("RLLM_ATTENTION")) Py_RETURN_FALSE;
-    const long long d = k.size(3), page = k.size(2), g = nq / nkv;
-    const bool both = dt == 1 && d != 256;
-    if (!(d == 64 || d == 128 || d == 256) || page % 16 || g > (both ? 32 : 16) || !e4m3_cache(args + 6, nkv, d, device)) Py_RETURN_FALSE;
+    if (dt < 0 || k.dim() != 4 || nq <= 0 || nkv <= 0 || nq % nkv) Py_RETURN_FALSE;
+    const long long d = k.size(3), page = k.size(2), pages = k.size(0);
+    if (!e4m3_cache(args + 6, nkv, d, device)) Py_RETURN_FALSE;
     for (int i = 3; i < 6; ++i)
       if (!vector_of_ints(THPVariable_Unpack(args[i]), device)) Py_RETURN_FALSE;
-    const long long S = THPVariable_Unpack(args[4]).numel();
-    if (S == 0 || THPVariable_Unpack(args[3]).numel() != S + 1 || table.size(0) < S || most < 0 || most > table.size(1) * page || q.dim() != 2 ||
-        out.dim() != 2 || out.scalar_type() != q.scalar_type() || q.stride(1) != 1 || out.size(1) != nq * d || q.size(1) < nq * d ||
-        q.size(0) < out.size(0) || out.size(0) == 0 || !out.is_contiguous() || q.get_device() != device || out.get_device() != device ||
-        ((uintptr_t)out.data_ptr() & 15))
+    const long long S = THPVariable_Unpack(args[4]).numel(), blocks = table.size(1);
+    if (THPVariable_Unpack(args[3]).numel() != S + 1 || decode < 0 || decode > S || table.size(0) < S || max_q < 0 || most < 0 ||
+        most > blocks * page || q.dim() != 2 || out.dim() != 2 || out.scalar_type() != q.scalar_type() || q.stride(1) != 1 ||
+        out.size(1) != nq * d || q.size(1) < nq * d || q.size(0) < out.size(0) || !out.is_contiguous() || q.get_device() != device ||
+        out.get_device() != device)
       Py_RETURN_FALSE;
-    const long long keys = window > 0 && window + 1 < most ? window + 1 : most;
-    const bool columns = both && keys >= 768 && S * nkv * keys >= (d == 64 ? 1 << 16 : 1 << 14);
-    Entry* e = (Entry*)args[columns ? 16 : 0];
-    if (!ready(e)) return nullptr;
-    auto at_ = [&](int i) { return THPVariable_Unpack(args[i]).data_ptr(); };
+    const long long T = out.size(0), stride = q.stride(0);
+    if (T == 0 || S == 0) Py_RETURN_TRUE;
+    const long long keys = window > 0 && window + max_q < most ? window + max_q : most;
+    void *pq = q.data_ptr(), *po = out.data_ptr(), *pqs = THPVariable_Unpack(args[3]).data_ptr(), *psl = THPVariable_Unpack(args[4]).data_ptr(),
+         *pe = THPVariable_Unpack(args[5]).data_ptr(), *pk = k.data_ptr(), *pv = THPVariable_Unpack(args[7]).data_ptr(),
+         *pks = THPVariable_Unpack(args[8]).data_ptr(), *pvs = THPVariable_Unpack(args[9]).data_ptr(), *pt = table.data_ptr();
     const cudaStream_t stream = stream_now();
-    int rc;
-    Py_BEGIN_ALLOW_THREADS
-    if (columns)
-      rc = reinterpret_cast<int (*)(void*, int, void*, void*, void*, void*, void*, void*, int, void*, void*, int, int, int, int, int, int, int, int,
-                                    int, int, float, void*, cudaStream_t)>(e->fn)(
-          q.data_ptr(), (int)q.stride(0), out.data_ptr(), at_(6), at_(7), at_(8), at_(9), table.data_ptr(), (int)table.size(1), at_(3), at_(4), 0,
-          (int)S, 1, (int)keys, (int)nq, (int)nkv, (int)d, (int)page, (int)k.size(0), (int)window, scale, at_(5), stream);
-    else
-      rc = reinterpret_cast<int (*)(void*, int, void*, void*, void*, void*, void*, int, void*, int, void*, void*, int, int, int, int, int, int, int,
-                                    int, int, int, float, void*, cudaStream_t)>(e->fn)(
-          q.data_ptr(), (int)q.stride(0), out.data_ptr(), at_(6), at_(7), at_(8), at_(9), dt, table.data_ptr(), (int)table.size(1), at_(3), at_(4),
-          0, (int)S, 1, (int)keys, (int)nq, (int)nkv, (int)d, (int)page, (int)k.size(0), (int)window, scale, at_(5), stream);
-    Py_END_ALLOW_THREADS
-    if (!finish(rc, e->what)) return nullptr;
+    for (int group = 0; group < 2; ++group) {
+      const long long first = group ? decode : 0, end = group ? S : decode, longest = group ? max_q : 1;
+      if (first == end || longest == 0) continue;
+      int form = named[group] >= 0 ? named[group] : e4m3_rule(dt == 1, nq, nkv, d, page, scale, longest, end - first, keys);
+      // results off 16 bytes: the kernel that stores single numbers; queries off 16 bytes: one that reads them one by one
+      if ((uintptr_t)po & 15) form = kSimt;
+      else if ((form == kTcgen05 || form == kDense) && (stride % 8 || ((uintptr_t)pq & 15))) form = page % 16 ? kSimt : kRows;
+      Entry* at_ = e[form == kRows ? 0 : form == kColumns ? 1 : form == kTcgen05 ? 2 : form == kSimt ? 3 : 5];
+      if (!ready(at_)) return nullptr;
+      int rc = 0;
+      if (form == kColumns || form == kTcgen05) {
+        Py_BEGIN_ALLOW_THREADS
+        rc = reinterpret_cast<int (*)(void*, int, void*, void*, void*, void*, void*, void*, int, void*, void*, int, int, int, int, int, int, int,
+                                      int, int, int, float, void*, cudaStream_t)>(at_->fn)(
+            pq, (int)stride, po, pk, pv, pks, pvs, pt, (int)blocks, pqs, psl, (int)first, (int)end, (int)longest, (int)keys, (int)nq, (int)nkv,
+            (int)d, (int)page, (int)pages, (int)window, (float)scale, pe, stream);
+        Py_END_ALLOW_THREADS
+      } else if (form == kRows) {
+        Py_BEGIN_ALLOW_THREADS
+        rc = reinterpret_cast<int (*)(void*, int, void*, void*, void*, void*, void*, int, void*, int, void*, void*, int, int, int, int, int, int,
+                                      int, int, int, int, float, void*, cudaStream_t)>(at_->fn)(
+            pq, (int)stride, po, pk, pv, pks, pvs, dt, pt, (int)blocks, pqs, psl, (int)first, (int)end, (int)longest, (int)keys, (int)nq, (int)nkv,
+            (int)d, (int)page, (int)pages, (int)window, (float)scale, pe, stream);
+        Py_END_ALLOW_THREADS
+      } else if (form == kSimt) {
+        const long long tokens = std::min(T, (end - first) * longest);
+        Py_BEGIN_ALLOW_THREADS
+        rc = reinterpret_cast<int (*)(void*, int, void*, void*, void*, void*, void*, int, void*, int, void*, void*, int, int, int, int, int, int,
+                                      int, int, int, float, void*, cudaStream_t)>(at_->fn)(
+            pq, (int)stride, po, pk, pv, pks, pvs, dt, pt, (int)blocks, pqs, psl, (int)first, (int)end, (int)tokens, (int)nq, (int)nkv, (int)d,
+            (int)page, (int)pages, (int)window, (float)scale, pe, stream);
+        Py_END_ALLOW_THREADS
+      } else {
+        const long long bn = 8192 / d, tiles = keys / bn + 2, a_sequence = 2 * tiles * nkv * bn * d;      // bytes
+        const long long together = std::max(1LL, std::min(std::min(end - first, scratch / (2 * a_sequence)), 65535LL));
+        const at::Tensor dense = at::empty({2 * together * a_sequence}, k.options().dtype(at::kByte));
+        const at::Tensor marks = at::empty({together * tiles * nkv * 8}, table.options());
+        char* const pd = (char*)dense.data_ptr();
+        void* const pm = marks.data_ptr();
+        if (!ready(e[4])) return nullptr;
+        for (long long s = first; s < end; s += together) {
+          const long long m = std::min(together, end - s);
+          Py_BEGIN_ALLOW_THREADS
+          rc = reinterpret_cast<int (*)(void*, int, void*, void*, int, int, int, void*, void*, void*, void*, void*, void*, void*, int, int, int, int,
+                                        int, void*, cudaStream_t)>(e[4]->fn)(
+              pt, (int)blocks, pqs, psl, (int)s, (int)m, (int)tiles, pk, pv, pks, pvs, pd, pd + together * a_sequence, pm, (int)nkv, (int)d,
+              (int)page, (int)pages, (int)window, pe, stream);
+          Py_END_ALLOW_THREADS
+          if (!finish(rc, at_->what)) return nullptr;
+          Py_BEGIN_ALLOW_THREADS
+          rc = reinterpret_cast<int (*)(void*, int, int, void*, void*, void*, void*, int, void*, void*, int, int, int, int, int, int, int, float,
+                                        void*, cudaStream_t)>(at_->fn)(
+              pq, (int)stride, (int)q.size(0), po, pd, pd + together * a_sequence, pm, (int)tiles, pqs, psl, (int)s, (int)m,
+              (int)std::min(T, m * longest), (int)nq, (int)nkv, (int)d, (int)window, (float)scale, pe, stream);
+          Py_END_ALLOW_THREADS
+          if (!finish(rc, at_->what)) return nullptr;
+        }
+        continue;
+      }
+      if (!finish(rc, at_->what)) return nullptr;
+    }
     Py_RETURN_TRUE;
   });
 }
@@ -469,7 +573,8 @@ PyMethodDef kMethods[] = {{"setup", (PyCFunction)(void*)setup, METH_FASTCALL, nu
                           {"e4m3_ready", (PyCFunction)(void*)e4m3_ready, METH_FASTCALL, nullptr},
                           {"e4m3_write", (PyCFunction)(void*)e4m3_write, METH_FASTCALL, nullptr},
                           {"e4m3_read", (PyCFunction)(void*)e4m3_read, METH_FASTCALL, nullptr},
-                          {"e4m3_decode", (PyCFunction)(void*)e4m3_decode, METH_FASTCALL, nullptr},
+                          {"e4m3_form", (PyCFunction)(void*)e4m3_form, METH_FASTCALL, nullptr},
+                          {"e4m3_attention", (PyCFunction)(void*)e4m3_attention, METH_FASTCALL, nullptr},
                           {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "launch", nullptr, -1, kMethods};
 

@@ -248,7 +248,7 @@ FORMS = ["rows", "columns", "tcgen05", "dense"]
     (8, 8, 128, 32, [127, 129], [1, 63], 0), (24, 8, 128, 16, [43, 42], [64, 65], 0), (32, 1, 64, 16, [9], [500], 70), (16, 2, 128, 64, [100], [300], 1),
     (8, 1, 128, 16, [20, 50], [1000, 10], 128), (40, 8, 64, 16, [30], [90], 0), (5, 1, 128, 48, [28], [200], 33), (128, 1, 64, 16, [2], [200], 0)])
 def test_every_form_of_the_attention(form, nq, nkv, d, page, lens, starts, window, monkeypatch):
-    monkeypatch.setattr(ops, "attention_e4m3_form", lambda *a: form)
+    monkeypatch.setattr(ops, "E4M3_FORMS", (form, form))
     for spread, qscale in ((1.0, 1.0), (3.0, 0.3)):
         st = Step(lens, starts, nq, nkv, d, page, BF16, seed=nq + d, more_rows=2, stride_pad=16, spread=spread, qscale=qscale)
         out = st.attend(ops, window, num_decode=0)
@@ -260,7 +260,7 @@ def test_every_form_of_the_attention(form, nq, nkv, d, page, lens, starts, windo
 @pytest.mark.parametrize("d", [64, 128])
 @pytest.mark.parametrize("lens,starts", [([5], [100]), ([3, 150], [40, 30]), ([70, 2], [200, 1000])])
 def test_keys_that_are_nan_missing_or_out_of_sight_in_every_form(form, d, lens, starts, monkeypatch):
-    monkeypatch.setattr(ops, "attention_e4m3_form", lambda *a: form)
+    monkeypatch.setattr(ops, "E4M3_FORMS", (form, form))
     s, n = len(lens) - 1, lens[-1]
     for where in (0, 1):                                          # a key, a value that is NaN, of a token of the step
         st = Step(lens, starts, 8, 2, d, 16, BF16, seed=4)
@@ -293,7 +293,7 @@ def test_keys_that_are_nan_missing_or_out_of_sight_in_every_form(form, d, lens, 
 @pytest.mark.parametrize("form", FORMS)
 def test_rows_that_are_zeros_in_every_form(form, monkeypatch):
     """Queries, keys and values of zeros (the least scales of all), alone and beside others."""
-    monkeypatch.setattr(ops, "attention_e4m3_form", lambda *a: form)
+    monkeypatch.setattr(ops, "E4M3_FORMS", (form, form))
     st = Step([40, 3], [100, 200], 8, 2, 64, 16, BF16, seed=7)
     st.q[::3] = 0
     for t in (st.k, st.v, st.ks, st.vs):
@@ -308,7 +308,7 @@ def test_rows_that_are_zeros_in_every_form(form, monkeypatch):
 @pytest.mark.parametrize("d", [64, 128])
 @pytest.mark.parametrize("what", [math.nan, math.inf])
 def test_a_query_that_is_not_finite_reaches_its_own_row_alone(form, d, what, monkeypatch):
-    monkeypatch.setattr(ops, "attention_e4m3_form", lambda *a: form)
+    monkeypatch.setattr(ops, "E4M3_FORMS", (form, form))
     st = Step([5, 3], [300, 40], 8, 2, d, 16, BF16, seed=3)
     plain = st.attend(ops, num_decode=0)
     st.q[2, 3 * d + 7] = what
@@ -322,7 +322,7 @@ def test_a_query_that_is_not_finite_reaches_its_own_row_alone(form, d, what, mon
 @pytest.mark.parametrize("d", [64, 128])
 def test_queries_whose_numbers_lie_far_apart(form, d, monkeypatch):
     """A few of a row's numbers 2^10 and more above the others, rows up to 2^30 apart."""
-    monkeypatch.setattr(ops, "attention_e4m3_form", lambda *a: form)
+    monkeypatch.setattr(ops, "E4M3_FORMS", (form, form))
     for size in (1.0, 2.0 ** -20):
         st = Step([6, 1], [500, 900], 8, 2, d, 16, BF16, seed=11, spread=0.5)
         g = torch.Generator().manual_seed(2)
@@ -343,7 +343,7 @@ def test_results_off_16_bytes(dtype, lens, starts):
 
 
 def test_prompts_in_groups_of_what_the_scratch_holds(monkeypatch):
-    monkeypatch.setattr(ops, "attention_e4m3_form", lambda *a: "dense")
+    monkeypatch.setattr(ops, "E4M3_FORMS", ("dense", "dense"))
     st = Step([40, 3, 70, 9], [100, 200, 0, 30], 8, 2, 64, 16, BF16, seed=7)
     whole = st.attend(ops, num_decode=0)
     monkeypatch.setattr(ops, "E4M3_DENSE_SCRATCH", 1)              # a sequence at a time
@@ -443,7 +443,7 @@ class TheLongWay:
         self.module = module
 
     def __getattr__(self, name):
-        return (lambda *args: False) if name in ("e4m3_write", "e4m3_read", "e4m3_decode") else getattr(self.module, name)
+        return (lambda *args: False) if name in ("e4m3_write", "e4m3_read") else getattr(self.module, name)
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
