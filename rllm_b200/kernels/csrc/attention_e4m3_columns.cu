@@ -25,10 +25,10 @@
 // two are left where they are (the tensor core has time).
 // A cluster shares the keys of a (sequence, kv head, tile of rows); parts are merged in shared memory as in attention_e4m3.cu.
 //
-// What bounds it: memory for heads of 128 (64 sequences of 8,191 keys, 8 kv heads of four rows: 159 us, 6.8 TB/s; the mma.sync kernel
-// 221).  For heads of 64 a key has half the bytes and the same work for a thread, 40 cycles of exponentials, conversions and
-// additions a (key, row) pair over four warps: 99 us, 5.4 TB/s (118), and 24 us for 32 rows of 8 sequences of 4,095 (32).  Over few keys
-// the way to the first tile's result, 6 us, is longer than the mma.sync kernel's.
+// What bounds it: memory for heads of 128 (64 sequences of 8,191 keys, 8 kv heads of four rows: 157 us, 6.9 TB/s; the mma.sync kernel
+// 221).  For heads of 64 a key has half the bytes and the same work for a thread (two exponentials and nine conversions for every two
+// rows, seven of them at half and a quarter of the ALU's rate): 96 us, 5.7 TB/s (118), and 20 us for 24 rows of 8 sequences of 4,095 (29).
+// Over few keys the way to the first tile's result, 6 us, is longer than the mma.sync kernel's.
 #include "attention_tcgen05.cuh"
 #include "kv_e4m3.cuh"
 #include <cooperative_groups.h>

@@ -2184,12 +2184,12 @@ def attention_e4m3_form(dtype: torch.dtype, nq: int, nkv: int, d: int, page_size
     values widened once for all tiles of rows), "simt".
 
     Measured (microseconds in a row; 8 kv heads with four heads each):
-      rows / columns, heads of 64: one token each, one sequence of 511 keys 4.5 / 6.3, 2,047 6.1 / 6.8, 8,191 11.7 / 9.8; 8 of 511
-        5.8 / 7.0, 1,023 8.9 / 8.1, 8,191 23.4 / 17.8; 64 of 255 8.4 / 11.9, 511 12.9 / 14.1, 1,023 21.6 / 19.8, 8,191 118 / 100; 8 of
-        4,095, 16 rows 25 / 18.6, 32 rows 32 / 24; heads of 128: one sequence of 511 5.7 / 5.7, 8 of 1,023 10.9 / 8.6, 64 of 255
-        11.7 / 12.9, 8,191 221 / 161; 8 of 4,095, 16 rows 34 / 20.6, 32 rows 61 / 28;
-      columns / tcgen05, more rows: heads of 128, one of 4,095, 64 rows 18.0 / 20.2, 128 rows 19.0 / 22.8 (heads of 64, rows / tcgen05: 15.0 /
-        17.2 and 16.6 / 18.4); 8 of 4,095, 64 rows 44 / 38, 128 rows 86 / 45;
+      rows / columns, heads of 64: one token each, one sequence of 511 keys 4.6 / 6.0, 2,047 6.1 / 6.6, 8,191 11.7 / 9.5; 8 of 1,023
+        8.9 / 7.8, 8,191 23.4 / 16.4; 64 of 255 8.3 / 11.5, 511 12.7 / 13.6, 1,023 21.6 / 18.5, 8,191 118 / 96; 8 of 4,095, 16 rows
+        25 / 16.9, 24 rows 29 / 19.6; heads of 128: one sequence of 511 5.9 / 5.7, 8 of 1,023 10.9 / 8.6, 64 of 255 11.6 / 12.5,
+        8,191 221 / 157; 8 of 4,095, 16 rows 34 / 19.3, 24 rows 43 / 22.8;
+      columns / tcgen05, more rows: heads of 128, one of 4,095, 64 rows 16.8 / 20.0, 128 rows 17.8 / 22.5 (heads of 64, rows / tcgen05:
+        15.0 / 17.1 and 16.5 / 18.4); 8 of 4,095, 64 rows 40 / 38, 128 rows 78 / 45;
       tcgen05 / dense, heads of 64: 4 of 16,000, 4 tiles of 128 rows 182 / 240, 6 tiles 340 / 287, 16 tiles 682 / 518; heads of
         128: 216 / 353, 406 / 381, 798 / 666."""
     return _launch().e4m3_form(dtype is torch.bfloat16, nq, nkv, d, page_size, scale, max_q_len, num_seqs, max_keys)
