@@ -14,9 +14,9 @@
 //   warp 8      allocates TMEM and issues the products: S = Q K^T (128 x 64 x D), O += P V (128 x D x 64, P in TMEM, V as the
 //               MN-major operand, straight from its rows).
 // Halves, not bfloat16: e4m3 numbers become halves in one instruction a pair, and a weight keeps 11 bits.  Powers of two:
-//   K  a row's numbers are multiplied by 2^(ek - EK), EK the largest ek of the tile, and the tile's scores by 2^EK: exact down to
-//      2^-24 of the tile's largest power;
-//   V  by 2^(ev - EV'), EV' the tile's largest, but at least 2^-30 of a running reference that moves when passed by 2^4, and the
+//   K  a row's numbers are multiplied by 2^(ek - EK + 6), EK the largest ek of the tile, and the tile's scores by 2^(EK - 6): exact for
+//      powers down to 2^-21 of the tile's largest, to a step of 2^-30 of that below;
+//   V  by 2^(ev - EV' + 6), EV' the tile's largest, but at least 2^-30 of a running reference that moves when passed by 2^4, and the
 //      tile's weights by 2^(EV' - reference), which rides in the exponent's argument; 2^7 more, as in the mma.sync kernel;
 //   Q  a row by a power of two of its own, exact for bfloat16 down to 2^-27 of the row's largest.
 // A token whose key or value is NaN has a NaN key and zeros for a value: rows that see it become NaN by the score, and the others'
@@ -31,6 +31,7 @@
 #define E8_AHEAD 8                   // tiles whose rows and factors are known at a time
 #define E8_SLACK 4.0f
 #define E8_SHIFT 7
+#define E8_LIFT 6                    // log2 of what keys and values are multiplied by beside: 448 2^6 is a half, and so is the factor 2^(6 - 30)
 
 // Q, the widened stages of K and of V (two each for heads of 64, one for 128: two CTAs fit one SM), two tiles of K and of V as
 // they come, barriers and the tiles' notes
@@ -134,7 +135,7 @@ attention_e4m3_tcgen05_kernel(const bf16* q, int q_stride, bf16* __restrict__ ou
         *(uint4*)(dst + ((((c & 3) * 2) ^ (r & 7)) << 4)) = w[0];
         *(uint4*)(dst + ((((c & 3) * 2 + 1) ^ (r & 7)) << 4)) = w[1];
         // the row's factor waits in the V ring for the softmax warps (they read it before the first value is widened)
-        if (c == 0) ((float*)sV)[r] = __uint_as_float((unsigned)(127 - 13 + e) << 23) * scale_log2;
+        if (c == 0) ((float*)sV)[r] = __uint_as_float((unsigned)(127 - 13 - E8_LIFT + e) << 23) * scale_log2;
       }
     }
   }
@@ -273,7 +274,7 @@ attention_e4m3_tcgen05_kernel(const bf16* q, int q_stride, bf16* __restrict__ ou
     if (ok) ok = __all_sync(0xffffffffu, mbar_wait(pv_full, (ntiles - 1) & 1, err));
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     // the result, without the values' powers' reference
-    const float fe = ref < 0 ? 0.f : kv8_power(ref) * (1.0f / (1 << E8_SHIFT));
+    const float fe = ref < 0 ? 0.f : kv8_power(ref) * (1.0f / (1 << (E8_SHIFT + E8_LIFT)));
     if (splits == 1) {
       const float inv = (l == 0.f ? 0.f : 1.0f / l) * fe;  // NaN stays NaN
       bf16* orow = out + ((size_t)(qs + t0 + tl) * nq + kvh * g + (r - tl * g)) * D;
@@ -453,8 +454,8 @@ attention_e4m3_tcgen05_kernel(const bf16* q, int q_stride, bf16* __restrict__ ou
         page[h] = page_of(it + 1, h);
       }
     };
-    auto factor = [&](int b, int top) {                    // 2^(b - top) twice, as halves
-      const __half2 p = __float2half2_rn(b - top < -30 ? 0.f : __uint_as_float((unsigned)(127 + b - top) << 23));
+    auto factor = [&](int b, int top) {                    // 2^(b - top + E8_LIFT) twice, as halves
+      const __half2 p = __float2half2_rn(b - top < -30 ? 0.f : __uint_as_float((unsigned)(127 + E8_LIFT + b - top) << 23));
       return *(const unsigned*)&p;
     };
     rows_of(0);

@@ -375,9 +375,11 @@ def test_sequences_without_tokens_and_calls_without_any():
     assert st.attend(ops, out=empty).numel() == 0
 
 
-def test_the_operators_in_a_row_on_another_stream_and_captured():
+@pytest.mark.parametrize("form,d", [(None, 64), ("columns", 64), ("columns", 128), ("tcgen05", 64), ("dense", 128)])
+def test_the_operators_in_a_row_on_another_stream_and_captured(form, d, monkeypatch):
     """Tokens written step by step, attended to and read back, eagerly and in a captured graph that is replayed with other inputs."""
-    nq, nkv, d, page = 8, 2, 64, 16
+    monkeypatch.setattr(ops, "E4M3_FORMS", form and (form, form))
+    nq, nkv, page = 8, 2, 16
     st = Step([1, 1, 1], [37, 100, 15], nq, nkv, d, page, BF16)
     inv = freqs(d)
     side = torch.cuda.Stream()
@@ -535,3 +537,42 @@ def test_a_reading_that_does_not_fit_is_refused_on_the_gpu_too():
             ops.kv_read_e4m3(a["pos"], a["seq"], st.table, st.k, st.v, st.ks, st.vs, a["k"], a["v"], st.err)
     with pytest.raises(ops.KernelError):
         ops.kv_read_e4m3(good["pos"], good["seq"], st.table, st.k, st.v, st.k, st.vs, good["k"], good["v"], st.err)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("nq,nkv", [(8, 2), (32, 2), (16, 8)])
+def test_the_same_bits_again_and_again_beside_other_work(d, nq, nkv, monkeypatch):
+    """Calls whose warps hand tiles to one another, repeated, two streams at a time, each over a cache of its own: no result depends
+    on who was first."""
+    monkeypatch.setattr(ops, "E4M3_FORMS", ("columns", "columns"))
+    steps = [Step(lens, starts, nq, nkv, d, 16, BF16, seed=i, spread=2.0) for i, (lens, starts) in enumerate(
+        [([1] * 7, [3000, 5, 777, 128, 255, 2000, 1]), ([1, 1, 2, 1 + 3 % nkv], [1500, 900, 640, 64]), ([1], [9000])])]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    first = [st.attend(ops) for st in steps]
+    torch.cuda.synchronize()
+    for st, out in zip(steps, first):
+        st.check(out)
+    outs = []
+    for i in range(40):
+        with torch.cuda.stream(streams[i % 2]):
+            outs.append((i % 3, steps[i % 3].attend(ops)))
+    torch.cuda.synchronize()
+    assert all(torch.equal(first[which], out) for which, out in outs) and all(int(st.err) == 0 for st in steps)
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("gap", [10, 22, 25, 27])
+def test_a_small_value_that_has_all_the_weight(form, d, gap, monkeypatch):
+    """One key that every row looks at, whose value lies 2^gap below those that weigh nothing."""
+    monkeypatch.setattr(ops, "E4M3_FORMS", (form, form))
+    st = Step([1, 2], [46, 600], 8, 2, d, 16, BF16, seed=5, spread=0.3)
+    for s, j in ((0, 1), (1, 333)):
+        page, slot = int(st.table[s, j // 16]), j % 16
+        k = (st.k[page, :, slot].float() * 2.0 ** (st.ks.view(torch.uint8)[page, :, slot].float() - 127)[:, None])     # [nkv, d]
+        first, last = int(st.q_start[s]), int(st.q_start[s + 1])
+        st.q[first:last] = (k * 60 / k.square().sum(-1, keepdim=True) * d ** 0.5).repeat_interleave(4, 0).reshape(-1).to(BF16)
+        st.vs.view(torch.uint8)[page, :, slot] -= gap
+    out = st.attend(ops, num_decode=0)
+    st.check(out)
+    assert (out[:3] != 0).any(-1).all()
