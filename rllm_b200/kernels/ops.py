@@ -2205,7 +2205,8 @@ def attention_e4m3(q: torch.Tensor, out: torch.Tensor, kcache: torch.Tensor, vca
     i's result.  Sequence s owns the tokens q_start[s] .. q_start[s + 1] - 1, the last ones of its seq_lens[s] in the cache;
     the first ``num_decode`` sequences bring one token each.  ``max_q_len`` and ``max_seq_len`` bound every sequence's tokens
     in this step and in the cache.  Rows behind the last sequence's stay as they are.  A page that is not held sets bit 4 of
-    ``err``, and its keys are left out."""
+    ``err``, and its keys are left out.  Single tokens and the others are two launches, but where no fewer sequences bring
+    several tokens and all of them few."""
     entries = (_entries.rllm_attention_e4m3_rows, _entries.rllm_attention_e4m3_columns, _entries.rllm_attention_e4m3_tcgen05,
                _entries.rllm_attention_e4m3_simt, _entries.rllm_kv_e4m3_widen, _entries.rllm_attention_dense_tcgen05)
     if _launch().e4m3_attention(entries, q, out, q_start, seq_lens, err, kcache, vcache, kscale, vscale, block_table, num_decode, max_q_len,

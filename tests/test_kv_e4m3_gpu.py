@@ -171,6 +171,7 @@ SHAPES = [  # nq, nkv, d, page, lens, starts, window
     (8, 4, 96, 8, [1, 11], [5, 50], 0), (2, 1, 128, 7, [1, 30], [100, 9], 0), (6, 2, 32, 16, [1, 40], [600, 0], 33),
     (32, 8, 64, 16, [1] * 6, [5000, 0, 255, 256, 257, 1023], 0), (24, 8, 128, 16, [1] * 5, [4999, 127, 128, 129, 3], 0), (32, 8, 64, 16, [5, 1, 6, 8], [4000, 1, 255, 2000], 0),
     (32, 8, 128, 48, [5, 1, 6, 8], [4000, 1, 255, 2000], 0), (16, 2, 64, 32, [1] * 12, [100 * i for i in range(12)], 900), (64, 2, 128, 16, [1] * 9, [900] * 9, 0),
+    (32, 8, 64, 16, [1, 1, 1, 5, 2, 8], [4000, 0, 700, 30, 2500, 0], 0), (32, 8, 128, 16, [1, 4, 2], [40, 0, 700], 100), (32, 8, 128, 16, [1, 1, 1, 1, 2], [900] * 5, 0),
     (20, 4, 128, 16, [6] * 6, [1500, 30, 0, 700, 122, 1], 1000), (8, 8, 128, 16, [1] * 20, [150 * i for i in range(20)], 0)]
 
 
