@@ -62,11 +62,11 @@ def _check(code: int, what: str) -> None:
 _TABLE = {
     "rllm_kv_e4m3_write": ("kv_e4m3", "piplpppipiippppiiiiiip", "rope_kv_write_e4m3"),
     "rllm_kv_e4m3_read": ("kv_e4m3", "pppiippppppiiiiiip", "kv_read_e4m3"),
-    "rllm_kv_e4m3_widen": ("kv_e4m3", "pippiiipppppppiiiiip", "attention_e4m3"),
+    "rllm_kv_e4m3_widen": ("kv_e4m3", "pippiiipppppppiiiiiip", "attention_e4m3"),
     "rllm_attention_dense_tcgen05": ("attention_tcgen05", "piippppippiiiiiiifp", "attention_e4m3"),
-    "rllm_attention_e4m3_tcgen05": ("attention_e4m3_tcgen05", "pippppppippiiiiiiiiiifp", "attention_e4m3"),
-    "rllm_attention_e4m3_columns": ("attention_e4m3_columns", "pippppppippiiiiiiiiiifp", "attention_e4m3"),
-    "rllm_attention_e4m3_rows": ("attention_e4m3", "pipppppipippiiiiiiiiiifp", "attention_e4m3"),
+    "rllm_attention_e4m3_tcgen05": ("attention_e4m3_tcgen05", "pippppppippiiiiiiiiiifip", "attention_e4m3"),
+    "rllm_attention_e4m3_columns": ("attention_e4m3_columns", "pippppppippiiiiiiiiiifip", "attention_e4m3"),
+    "rllm_attention_e4m3_rows": ("attention_e4m3", "pipppppipippiiiiiiiiiifip", "attention_e4m3"),
     "rllm_attention_e4m3_simt": ("attention_e4m3", "pipppppipippiiiiiiiiifp", "attention_e4m3"),
     "rllm_softcap": ("elementwise", "plf", "softcap_rows"),
     "rllm_shared_key_attention_mma": ("shared_key_attention", "pppppippiiiiiiiiiiifiipp", "shared_key_attention_mma"),

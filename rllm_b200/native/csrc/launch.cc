@@ -100,7 +100,7 @@ const Row kSignatures[] = {
     ROW("piiipppppppi"), ROW("piippifpppfippppiiiiiippip"), ROW("piippippppiiipiiip"),
     ROW("piippppifpippiiiiiiipiiippififiip"), ROW("piippppippiiiiiiiiifiifppiipp"), ROW("piippppippiiiiiiiiifpi"),
     ROW("piipppppipipppippiiiiiiiiipp"), ROW("piplpppipiippppiiiiiip"), ROW("pppiippppppiiiiiip"), ROW("pipppppipippiiiiiiiiifp"),
-    ROW("pipppppipippiiiiiiiiiifp"), ROW("pippiiipppppppiiiiip"), ROW("pippppppippiiiiiiiiiifp"), ROW("piippppippiiiiiiifp"), ROW("piippppppppiiiiff"), ROW("piiipppppppppiiipiiiip"), ROW("pipifpipiiiiifff"),
+    ROW("pipppppipippiiiiiiiiiifip"), ROW("pippiiipppppppiiiiiip"), ROW("pippppppippiiiiiiiiiifip"), ROW("piippppippiiiiiiifp"), ROW("piippppppppiiiiff"), ROW("piiipppppppppiiipiiiip"), ROW("pipifpipiiiiifff"),
     ROW("pipipiiii"), ROW("pipipiiiiifff"), ROW("pipipiiiiifffp"), ROW("pipipippipippiii"), ROW("pippifpppfipppppiiiiiiipp"),
     ROW("pippiiipppiiiiiiiifpp"), ROW("pippippppipppppppiiiiiiiiiiiiifffip"), ROW("pipppipippiiiiiiifp"),
     ROW("pipppipippiiiiiiiifiifppiipiip"), ROW("pipppipippiiiiiiip"), ROW("pipppippiiiiiiiiifpp"),
@@ -497,29 +497,34 @@ PyObject* e4m3_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
     // and 16 of 8 behind 2,000, more tiles of 32 rows than SMs, would be 30 -> 35).
     const long long few = max_q * (nq / nkv);
     const bool together_all = args[19] == Py_None && decode > 0 && S - decode >= decode && (few <= 16 || (few <= 32 && S * nkv <= 148));
+    int before = -1;                                       // the form of the call's first launch
     for (int group = together_all ? 1 : 0; group < 2; ++group) {
       const long long first = group && !together_all ? decode : 0, end = group ? S : decode, longest = group ? max_q : 1;
       if (first == end || longest == 0) continue;
+      // behind the single tokens' kernel, of which it reads nothing and overwrites nothing (widened tiles come from memory that the first's
+      // widened tiles may just have left)
+      const int late = group && before >= 0 && before != kDense;
       int form = named[group] >= 0 ? named[group] : e4m3_rule(dt == 1, nq, nkv, d, page, scale, longest, end - first, keys);
       // results off 16 bytes: the kernel that stores single numbers; queries off 16 bytes: one that reads them one by one
       if ((uintptr_t)po & 15) form = kSimt;
       else if ((form == kTcgen05 || form == kDense) && (stride % 8 || ((uintptr_t)pq & 15))) form = page % 16 ? kSimt : kRows;
+      before = form;
       Entry* at_ = e[form == kRows ? 0 : form == kColumns ? 1 : form == kTcgen05 ? 2 : form == kSimt ? 3 : 5];
       if (!ready(at_)) return nullptr;
       int rc = 0;
       if (form == kColumns || form == kTcgen05) {
         Py_BEGIN_ALLOW_THREADS
         rc = reinterpret_cast<int (*)(void*, int, void*, void*, void*, void*, void*, void*, int, void*, void*, int, int, int, int, int, int, int,
-                                      int, int, int, float, void*, cudaStream_t)>(at_->fn)(
+                                      int, int, int, float, int, void*, cudaStream_t)>(at_->fn)(
             pq, (int)stride, po, pk, pv, pks, pvs, pt, (int)blocks, pqs, psl, (int)first, (int)end, (int)longest, (int)keys, (int)nq, (int)nkv,
-            (int)d, (int)page, (int)pages, (int)window, (float)scale, pe, stream);
+            (int)d, (int)page, (int)pages, (int)window, (float)scale, late, pe, stream);
         Py_END_ALLOW_THREADS
       } else if (form == kRows) {
         Py_BEGIN_ALLOW_THREADS
         rc = reinterpret_cast<int (*)(void*, int, void*, void*, void*, void*, void*, int, void*, int, void*, void*, int, int, int, int, int, int,
-                                      int, int, int, int, float, void*, cudaStream_t)>(at_->fn)(
+                                      int, int, int, int, float, int, void*, cudaStream_t)>(at_->fn)(
             pq, (int)stride, po, pk, pv, pks, pvs, dt, pt, (int)blocks, pqs, psl, (int)first, (int)end, (int)longest, (int)keys, (int)nq, (int)nkv,
-            (int)d, (int)page, (int)pages, (int)window, (float)scale, pe, stream);
+            (int)d, (int)page, (int)pages, (int)window, (float)scale, late, pe, stream);
         Py_END_ALLOW_THREADS
       } else if (form == kSimt) {
         const long long tokens = std::min(T, (end - first) * longest);
@@ -541,9 +546,9 @@ PyObject* e4m3_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
           const long long m = std::min(together, end - s);
           Py_BEGIN_ALLOW_THREADS
           rc = reinterpret_cast<int (*)(void*, int, void*, void*, int, int, int, void*, void*, void*, void*, void*, void*, void*, int, int, int, int,
-                                        int, void*, cudaStream_t)>(e[4]->fn)(
+                                        int, int, void*, cudaStream_t)>(e[4]->fn)(
               pt, (int)blocks, pqs, psl, (int)s, (int)m, (int)tiles, pk, pv, pks, pvs, pd, pd + together * a_sequence, pm, (int)nkv, (int)d,
-              (int)page, (int)pages, (int)window, pe, stream);
+              (int)page, (int)pages, (int)window, late && s == first, pe, stream);
           Py_END_ALLOW_THREADS
           if (!finish(rc, at_->what)) return nullptr;
           Py_BEGIN_ALLOW_THREADS

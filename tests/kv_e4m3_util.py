@@ -157,9 +157,9 @@ class Step:
 
     def check(self, out, window=0, scale=None):
         from rllm_b200.kernels import ops
-        form = ops.E4M3_FORMS[1] if ops.E4M3_FORMS else ops.attention_e4m3_form(
-            self.dtype, self.nq, self.nkv, self.d, self.page, 1.0, max(self.lens), len(self.lens) - self.num_decode, max(self.totals))
-        prompts = form == "dense"
+        forms = ops.E4M3_FORMS or (ops.attention_e4m3_form(
+            self.dtype, self.nq, self.nkv, self.d, self.page, 1.0, max(self.lens), len(self.lens) - self.num_decode, max(self.totals)),)
+        prompts = "dense" in forms
         want, bound = self.expected(window, scale, prompts)
         got = out[:want.shape[0]].to(F64)
         assert torch.equal(torch.isnan(got), torch.isnan(want)), "NaN where none belongs, or none where one does"

@@ -577,3 +577,43 @@ def test_a_small_value_that_has_all_the_weight(form, d, gap, monkeypatch):
     out = st.attend(ops, num_decode=0)
     st.check(out)
     assert (out[:3] != 0).any(-1).all()
+
+
+@pytest.mark.parametrize("dtype,forms", [(BF16, None), (F32, None)] + [(BF16, (a, b)) for a in FORMS for b in FORMS])
+def test_single_tokens_and_portions_side_by_side(dtype, forms, monkeypatch):
+    """The portions' kernel does not wait for the single tokens' one, but for the write ahead of both, and what comes behind waits for
+    both: written, attended to and overwritten many times without a stop in between, each result that of its own inputs."""
+    monkeypatch.setattr(ops, "E4M3_FORMS", forms)
+    nq, nkv, d, page = 8, 2, 64, 16
+    lens, starts = [1] * 6 + [40, 200, 3], [3000, 5, 900, 2000, 0, 77, 500, 0, 64]
+    st = Step(lens, starts, nq, nkv, d, page, dtype, seed=3)
+    T, inv = sum(lens), freqs(d)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    inputs = [torch.randn(T, (nq + 2 * nkv) * d, device="cuda", generator=g).to(dtype) for _ in range(24)]
+    cache = [st.k, st.v, st.ks, st.vs]
+
+    def step(x, out, q):
+        ops.rope_kv_write_e4m3(x, st.positions, st.token_seq, inv, d, st.table, *cache, nq, nkv, d, st.err, q_out=q)
+        ops.attention_e4m3(q, out, *cache, st.table, st.q_start, st.seq_lens, 6, 200, max(st.totals), nq, nkv, 0, d ** -0.5, st.err)
+
+    apart = []
+    q = torch.empty(T, nq * d, dtype=dtype, device="cuda")
+    for x in inputs:
+        out = torch.empty(T, nq * d, dtype=dtype, device="cuda")
+        step(x, out, q)
+        torch.cuda.synchronize()
+        apart.append(out)
+    st.q = q.clone()
+    st.check(apart[-1])
+    outs = [torch.empty(T, nq * d, dtype=dtype, device="cuda") for _ in inputs]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        kept = []
+        for x, out in zip(inputs, outs):
+            step(x, out, q)
+            kept.append(out.clone())
+            out.zero_()
+    for _ in range(3):
+        graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(apart, kept)) and int(st.err) == 0
