@@ -37,7 +37,7 @@
 // without any of it.
 // Every mbarrier wait is bounded (bit 16 of the error word, then wind-down).
 // No cluster, no multicast.
-// The DENSE form reads keys and values that a kernel has widened from a cache kept in 8 bits (attention_e4m3.cu) into bfloat16
+// The DENSE form reads keys and values that a kernel has widened from a cache kept in 8 bits (kv_e4m3.cu) into bfloat16
 // tiles of BN keys, [sequence][tile][kv head][BN][D], a tile a box; a mark beside a tile says whether it has keys that are NaN
 // (the polynomial for exponentials knows none: the sums of the rows that see one are made NaN by themselves) or that are missing
 // (then they are masked one by one).

@@ -20,15 +20,15 @@
 #define KV8_NAN_SCALE 255
 
 // A call's second kernel, which reads nothing of its first (the portions' attention behind the single tokens'), does not wait for
-// it before it begins but before it ends (`late`): what was written ahead of both is there when it starts, for the first has let it
+// it before it begins but before it ends (`beside`): what was written ahead of both is there when it starts, for the first has let it
 // in behind its own wait, and whoever comes after it finds both complete.  It lets nobody in itself.
 template <typename... P>
-__device__ __forceinline__ void kv8_begin(int late, P&... ptrs) {
-  if (!late) pdl_wait();
+__device__ __forceinline__ void kv8_begin(int beside, P&... ptrs) {
+  if (!beside) pdl_wait();
   (pdl_fresh_in_place(ptrs), ...);
 }
-__device__ __forceinline__ void kv8_let_in(int late) { if (!late) pdl_launch(); }
-__device__ __forceinline__ void kv8_end(int late) { if (late) pdl_wait(); }
+__device__ __forceinline__ void kv8_let_in(int beside) { if (!beside) pdl_launch(); }
+__device__ __forceinline__ void kv8_end(int beside) { if (beside) pdl_wait(); }
 
 // the scale byte of a row whose largest magnitude is `top` (finite): (bits + 0x1FFFFF) >> 23 is top's biased exponent, one
 // more where its mantissa lies above 1.75 = 448 / 256

@@ -503,7 +503,7 @@ PyObject* e4m3_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
       if (first == end || longest == 0) continue;
       // behind the single tokens' kernel, of which it reads nothing and overwrites nothing (widened tiles come from memory that the first's
       // widened tiles may just have left)
-      const int late = group && before >= 0 && before != kDense;
+      const int beside = group && before >= 0 && before != kDense;
       int form = named[group] >= 0 ? named[group] : e4m3_rule(dt == 1, nq, nkv, d, page, scale, longest, end - first, keys);
       // results off 16 bytes: the kernel that stores single numbers; queries off 16 bytes: one that reads them one by one
       if ((uintptr_t)po & 15) form = kSimt;
@@ -517,14 +517,14 @@ PyObject* e4m3_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
         rc = reinterpret_cast<int (*)(void*, int, void*, void*, void*, void*, void*, void*, int, void*, void*, int, int, int, int, int, int, int,
                                       int, int, int, float, int, void*, cudaStream_t)>(at_->fn)(
             pq, (int)stride, po, pk, pv, pks, pvs, pt, (int)blocks, pqs, psl, (int)first, (int)end, (int)longest, (int)keys, (int)nq, (int)nkv,
-            (int)d, (int)page, (int)pages, (int)window, (float)scale, late, pe, stream);
+            (int)d, (int)page, (int)pages, (int)window, (float)scale, beside, pe, stream);
         Py_END_ALLOW_THREADS
       } else if (form == kRows) {
         Py_BEGIN_ALLOW_THREADS
         rc = reinterpret_cast<int (*)(void*, int, void*, void*, void*, void*, void*, int, void*, int, void*, void*, int, int, int, int, int, int,
                                       int, int, int, int, float, int, void*, cudaStream_t)>(at_->fn)(
             pq, (int)stride, po, pk, pv, pks, pvs, dt, pt, (int)blocks, pqs, psl, (int)first, (int)end, (int)longest, (int)keys, (int)nq, (int)nkv,
-            (int)d, (int)page, (int)pages, (int)window, (float)scale, late, pe, stream);
+            (int)d, (int)page, (int)pages, (int)window, (float)scale, beside, pe, stream);
         Py_END_ALLOW_THREADS
       } else if (form == kSimt) {
         const long long tokens = std::min(T, (end - first) * longest);
@@ -548,7 +548,7 @@ PyObject* e4m3_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
           rc = reinterpret_cast<int (*)(void*, int, void*, void*, int, int, int, void*, void*, void*, void*, void*, void*, void*, int, int, int, int,
                                         int, int, void*, cudaStream_t)>(e[4]->fn)(
               pt, (int)blocks, pqs, psl, (int)s, (int)m, (int)tiles, pk, pv, pks, pvs, pd, pd + together * a_sequence, pm, (int)nkv, (int)d,
-              (int)page, (int)pages, (int)window, late && s == first, pe, stream);
+              (int)page, (int)pages, (int)window, beside && s == first, pe, stream);
           Py_END_ALLOW_THREADS
           if (!finish(rc, at_->what)) return nullptr;
           Py_BEGIN_ALLOW_THREADS
