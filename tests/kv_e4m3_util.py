@@ -96,7 +96,7 @@ class Step:
         x = values(codes[at], scale[at]).transpose(0, 1).reshape(self.nkv, -1, self.d)[:, :n]
         return x, held.repeat_interleave(self.page)[:n]
 
-    def expected(self, window=0, scale=None, prompts=False):
+    def expected(self, window=0, scale=None, prompts=False, columns=False):
         """(result, bound of the error) float64 [T, nq d].
 
         The bound, from the kernels' arithmetic.  A score's sum of d products in float32 is off by at most (d + 4) 2^-24 of
@@ -105,7 +105,12 @@ class Step:
         2^-24, counted with 2^-17) and by the rounding of p to a half (2^-11), or to two of them (2^-22); the sums over the keys
         add n 2^-24; the result is rounded once to its type.  A half's step does not fall below 2^-24, so a weight, held as
         p 2^ev 2^7 over a power of two that is at most the largest 2^ev in sight, is off by 2^-32 of that at least: over n keys
-        with numbers of at most 448, n 448 2^-32 max 2^ev, p being 1 at the row's reference and the weights' sum 1 at least."""
+        with numbers of at most 448, n 448 2^-32 max 2^ev, p being 1 at the row's reference and the weights' sum 1 at least.
+
+        ``columns``: there a weight is p 2^ev over a reference that is at most the row's largest p 2^ev, times 2^2; a half is off by
+        2^-25 at least, and the last of the four terms it is taken apart into, of a step of 2^-9 over 2^15, by as much: by 2^-24 over
+        2^2 of the row's largest p 2^ev together, n 448 2^-26 max p 2^ev over n keys.  (Its products' sums are off by 2^-21 of the
+        absolute sum, which the score's (d + 4) 2^-24 and the weights' 2^-17 cover.)"""
         scale = self.d ** -0.5 if scale is None else scale
         # prompts on tcgen05: the weights are bfloat16 (2^-8), some exponentials a polynomial's (4e-5)
         half = 2.0 ** -8 + 4e-5 if prompts else 2.0 ** -11 if self.dtype is torch.bfloat16 else 2.0 ** -22
@@ -141,6 +146,8 @@ class Step:
                 outs.append(out)
                 power = torch.where(seen.any(0)[:, None], vz.abs(), torch.zeros_like(vz)).amax() / 224        # 2^ev <= max|v| / 224
                 floor = key.numel() * 448 * 2.0 ** -32 * power
+                if columns:
+                    floor = floor + key.numel() * 448 * 2.0 ** -26 * (p * (vz.abs().amax(-1) / 224)[None]).amax(-1, keepdim=True)
                 bounds.append(rel * (w @ vz.abs()) + floor + torch.finfo(self.dtype).eps / 2 * out.abs() + 1e-30)
         T = sum(self.lens)
         place = []
@@ -159,8 +166,7 @@ class Step:
         from rllm_b200.kernels import ops
         forms = ops.E4M3_FORMS or (ops.attention_e4m3_form(
             self.dtype, self.nq, self.nkv, self.d, self.page, 1.0, max(self.lens), len(self.lens) - self.num_decode, max(self.totals)),)
-        prompts = "dense" in forms
-        want, bound = self.expected(window, scale, prompts)
+        want, bound = self.expected(window, scale, "dense" in forms, "columns" in forms)
         got = out[:want.shape[0]].to(F64)
         assert torch.equal(torch.isnan(got), torch.isnan(want)), "NaN where none belongs, or none where one does"
         fine = ~torch.isnan(want)
