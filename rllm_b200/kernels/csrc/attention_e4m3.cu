@@ -40,7 +40,7 @@ attention_e4m3_simt_kernel(const T* q, int q_stride, T* __restrict__ out, const 
                            int num_tokens, int nq, int nkv, int d, int page_size, int num_pages, int window, float scale,
                            int* __restrict__ err) {
   extern __shared__ float qs[];      // [E4_SIMT_WARPS][d]
-  pdl_wait_on(q, kcache, vcache, kscale, vscale);
+  pdl_wait_on(q, kcache, vcache, kscale, vscale, block_table, q_start, seq_lens);
   pdl_launch();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const long long gw = (long long)blockIdx.x * E4_SIMT_WARPS + warp;
@@ -204,10 +204,11 @@ attention_e4m3_rows_kernel(const T* q, int q_stride, T* __restrict__ out, const 
                            const unsigned char* __restrict__ vcache, const unsigned char* __restrict__ kscale,
                            const unsigned char* __restrict__ vscale, const int* __restrict__ block_table, int max_blocks,
                            const int* __restrict__ q_start, const int* __restrict__ seq_lens, int seq_begin, int nq, int nkv,
-                           int page_size, int num_pages, int window, float scale_log2, int q_wide, int beside, int* __restrict__ err) {
+                           int page_size, int num_pages, int window, float scale_log2, int q_wide, int known, int* __restrict__ err) {
   constexpr int R = 8 * NB, TERMS = sizeof(T) == 4 ? 2 : 1, KC = D / 64, VW = D / 32, TB = e4_tile_bytes<D>();
   extern __shared__ __align__(16) float e4_smem[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, gid = lane >> 2, tig = lane & 3;
+  kv8_inputs(known, block_table, q_start, seq_lens);
   const int C = gridDim.x, rank = blockIdx.x;      // the cluster is the grid's x
   const int kvh = blockIdx.y % nkv, s = seq_begin + blockIdx.z;
   const int g = nq / nkv;
@@ -245,8 +246,8 @@ attention_e4m3_rows_kernel(const T* q, int q_stride, T* __restrict__ out, const 
   };
   auto place_of = [&](int i, int u) { return __shfl_sync(0xffffffffu, (i & 16) ? places1 : places0, (2 * i + u) & 31); };
   look_up(0);
-  kv8_begin(beside, q, kcache, vcache, kscale, vscale);
-  kv8_let_in(beside);
+  kv8_begin(known, q, kcache, vcache, kscale, vscale);
+  kv8_let_in(known);
   // A warp's pair lies behind the queries: for each tile [pieces][32 lanes] of 16 bytes of K, then of V, and its scales.  A lane
   // reads back what it copied itself (the scales apart), each of its accesses 16 bytes beside its neighbour's.  There is one
   // place for K and one for V: the next pair's keys are asked for when this pair's scores are made, its values behind this
@@ -648,7 +649,7 @@ attention_e4m3_rows_kernel(const T* q, int q_stride, T* __restrict__ out, const 
     if (C == 1) store(r, c, x, cL[r]);
     else *(float4*)(part + r * LD + c) = x;
   }
-  if (C == 1) { kv8_end(beside); return; }
+  if (C == 1) { kv8_end(known); return; }
   namespace cg = cooperative_groups;
   cg::cluster_group cluster = cg::this_cluster();
   cluster.sync();
@@ -666,14 +667,14 @@ attention_e4m3_rows_kernel(const T* q, int q_stride, T* __restrict__ out, const 
     store(r, i - r * D, x, sum);
   }
   cluster.sync();                                    // nobody leaves while its shared memory is being read
-  kv8_end(beside);
+  kv8_end(known);
 }
 
 template <int D, int NB, typename T>
 static int e4_rows_launch(const void* q, int q_stride, void* out, const void* kcache, const void* vcache, const void* kscale,
                           const void* vscale, const int* block_table, int max_blocks, const int* q_start, const int* seq_lens,
                           int seq_begin, int num_seqs, int max_q_len, int max_keys, int nq, int nkv, int page_size,
-                          int num_pages, int window, float scale, int beside, int* err, cudaStream_t stream) {
+                          int num_pages, int window, float scale, int known, int* err, cudaStream_t stream) {
   constexpr int R = 8 * NB;
   auto* kernel = attention_e4m3_rows_kernel<D, NB, T>;
   const size_t stage = sizeof(float) * R * (D + 4), merge = sizeof(float) * (E4_WARPS * R * (D + 6) + 2 * R);
@@ -705,19 +706,19 @@ static int e4_rows_launch(const void* q, int q_stride, void* out, const void* kc
                                            (const unsigned char*)vcache, (const unsigned char*)kscale, (const unsigned char*)vscale,
                                            block_table, max_blocks, q_start, seq_lens, seq_begin, nq, nkv, page_size, num_pages,
                                            window, scale * 1.4426950408889634f,
-                                           (((uintptr_t)q | ((uintptr_t)q_stride * sizeof(T))) & 15) == 0 ? 1 : 0, beside, err);
+                                           (((uintptr_t)q | ((uintptr_t)q_stride * sizeof(T))) & 15) == 0 ? 1 : 0, known, err);
   if (e != cudaSuccess) { cudaGetLastError(); return (int)e; }
   RLLM_LAUNCH_CHECK();
   return 0;
 }
 
-// Sequences seq_begin .. seq_end - 1, of at most max_q_len tokens each; no query sees more than max_keys keys; beside: see kv8_begin.  Heads of 64,
+// Sequences seq_begin .. seq_end - 1, of at most max_q_len tokens each; no query sees more than max_keys keys; known: see kv8_inputs.  Heads of 64,
 // 128 or 256, pages of a multiple of 16 keys.
 RLLM_EXPORT int rllm_attention_e4m3_rows(const void* q, int q_stride, void* out, const void* kcache, const void* vcache,
                                          const void* kscale, const void* vscale, int dtype, const int* block_table,
                                          int max_blocks, const int* q_start, const int* seq_lens, int seq_begin, int seq_end,
                                          int max_q_len, int max_keys, int nq, int nkv, int d, int page_size, int num_pages,
-                                         int window, float scale, int beside, int* err, cudaStream_t stream) {
+                                         int window, float scale, int known, int* err, cudaStream_t stream) {
   if (max_q_len <= 0 || seq_end <= seq_begin) return 0;
   if (const int rc = e4_check(q, out, kcache, vcache, kscale, vscale, block_table, max_blocks, q_start, seq_lens, seq_begin,
                               seq_end, nq, nkv, d, page_size, num_pages, window, scale, err)) return rc;
@@ -726,7 +727,7 @@ RLLM_EXPORT int rllm_attention_e4m3_rows(const void* q, int q_stride, void* out,
 #define E4_ROWS(DD, NBB, TT)                                                                                                   \
   return e4_rows_launch<DD, NBB, TT>(q, q_stride, out, kcache, vcache, kscale, vscale, block_table, max_blocks, q_start, \
                                           seq_lens, seq_begin, seq_end - seq_begin, max_q_len, max_keys, nq, nkv, page_size,  \
-                                          num_pages, window, scale, beside, err, stream)
+                                          num_pages, window, scale, known, err, stream)
   // tiles of as many rows as the sequences bring, where registers hold them: every tile reads all keys again
   const long long rows = (long long)max_q_len * (nq / nkv);
   if (dtype == RLLM_DT_BF16) {

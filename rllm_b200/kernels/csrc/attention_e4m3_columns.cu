@@ -135,10 +135,11 @@ __global__ void __launch_bounds__(EcShape<D, NB, MANY>::THREADS, EcShape<D, NB, 
 attention_e4m3_columns_kernel(const bf16* q, int q_stride, bf16* __restrict__ out, const unsigned char* kcache, const unsigned char* vcache,
                               const unsigned char* kscale, const unsigned char* vscale, const int* __restrict__ block_table, int max_blocks, const int* __restrict__ q_start,
                               const int* __restrict__ seq_lens, int seq_begin, int nq, int nkv, int page_size, int num_pages, int window,
-                              float scale_log2, int q_wide, int beside, int* __restrict__ err) {
+                              float scale_log2, int q_wide, int known, int* __restrict__ err) {
   typedef EcShape<D, NB, MANY> X;
   constexpr int R = X::R, NS = X::STAGES, PAR = X::PAR, PLANE = 128 * 16, TN = X::TN, MMA = 4 * NB;      // MMA: that warp
   extern __shared__ __align__(1024) unsigned char ec_raw[];
+  kv8_inputs(known, block_table, q_start, seq_lens);
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31, tid = threadIdx.x;
   const int C = gridDim.x, rank = blockIdx.x;              // the cluster is the grid's x
   const int kvh = blockIdx.y % nkv, s = seq_begin + blockIdx.z, g = nq / nkv;
@@ -198,8 +199,8 @@ attention_e4m3_columns_kernel(const bf16* q, int q_stride, bf16* __restrict__ ou
       *(ulonglong2*)&x[0] = *(const ulonglong2*)(info + what * 8);
       *(ulonglong2*)&x[2] = *(const ulonglong2*)(info + what * 8 + 4);
     };
-    kv8_begin(beside, q);
-    kv8_let_in(beside);
+    kv8_begin(known, q);
+    kv8_let_in(known);
     // queries: L lanes a row, 16 numbers each
     constexpr int L = D / 16;
     {
@@ -451,7 +452,7 @@ attention_e4m3_columns_kernel(const bf16* q, int q_stride, bf16* __restrict__ ou
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   } else if (warp == MMA) {
     // ---- products ----
-    kv8_begin(beside);
+    kv8_begin(known);
     const unsigned id_s = (1u << 4) | (unsigned)(X::QN >> 3) << 17 | (128u >> 4) << 24;
     const unsigned id_o = (1u << 4) | 3u << 15 | (unsigned)(X::ON >> 3) << 17 | (128u >> 4) << 24;
     auto wait = [&](unsigned long long* bar, int phase) {
@@ -519,7 +520,7 @@ attention_e4m3_columns_kernel(const bf16* q, int q_stride, bf16* __restrict__ ou
       return there ? (page * nkv + kvh) * page_size + in_page(j) : -1;
     };
     int ahead = pages_of(0), place = -1;
-    kv8_begin(beside, kcache, vcache, kscale, vscale);
+    kv8_begin(known, kcache, vcache, kscale, vscale);
     const unsigned to = line * 128 + ((c16 ^ line) << 4);
     auto bring = [&](const unsigned char* stage, const unsigned char* cache, int it) {
       const unsigned dst = tg_smem(stage) + to;
@@ -597,13 +598,13 @@ attention_e4m3_columns_kernel(const bf16* q, int q_stride, bf16* __restrict__ ou
     *(uint2*)(out + ((size_t)(qs + tok) * nq + kvh * g + at - tok * g) * D + col) = make_uint2(*(const unsigned*)&lo, *(const unsigned*)&hi);
   }
   if (C > 1) cluster.sync();                               // nobody leaves while its shared memory is being read
-  kv8_end(beside);
+  kv8_end(known);
 }
 
 template <int D, int NB, bool MANY = false>
 static int ec_launch(const void* q, int q_stride, void* out, const void* kcache, const void* vcache, const void* kscale, const void* vscale,
                      const int* block_table, int max_blocks, const int* q_start, const int* seq_lens, int seq_begin, int num_seqs,
-                     int max_q_len, int max_keys, int nq, int nkv, int page_size, int num_pages, int window, float scale, int beside, int* err,
+                     int max_q_len, int max_keys, int nq, int nkv, int page_size, int num_pages, int window, float scale, int known, int* err,
                      cudaStream_t stream) {
   typedef EcShape<D, NB, MANY> X;
   const long long tiles = ((long long)max_q_len * (nq / nkv) + X::R - 1) / X::R, units = tiles * nkv * num_seqs;
@@ -611,7 +612,7 @@ static int ec_launch(const void* q, int q_stride, void* out, const void* kcache,
   if constexpr (D == 128 && NB == 1 && !MANY)
     if (units > 148 * X::CTAS)
       return ec_launch<D, NB, true>(q, q_stride, out, kcache, vcache, kscale, vscale, block_table, max_blocks, q_start, seq_lens, seq_begin,
-                                    num_seqs, max_q_len, max_keys, nq, nkv, page_size, num_pages, window, scale, beside, err, stream);
+                                    num_seqs, max_q_len, max_keys, nq, nkv, page_size, num_pages, window, scale, known, err, stream);
   auto* kernel = attention_e4m3_columns_kernel<D, NB, MANY>;
   static SmemLimit limit;
   if (const int e = limit.allow(kernel, X::SMEM)) return e;
@@ -636,18 +637,18 @@ static int ec_launch(const void* q, int q_stride, void* out, const void* kcache,
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, (const bf16*)q, q_stride, (bf16*)out, (const unsigned char*)kcache,
                                            (const unsigned char*)vcache, (const unsigned char*)kscale, (const unsigned char*)vscale, block_table, max_blocks, q_start, seq_lens, seq_begin, nq, nkv,
                                            page_size, num_pages, window, scale * 1.4426950408889634f,
-                                           (((uintptr_t)q | ((uintptr_t)q_stride * 2)) & 15) == 0 ? 1 : 0, beside, err);
+                                           (((uintptr_t)q | ((uintptr_t)q_stride * 2)) & 15) == 0 ? 1 : 0, known, err);
   if (e != cudaSuccess) { cudaGetLastError(); return (int)e; }
   return 0;
 }
 
 // Sequences seq_begin .. seq_end - 1 of bfloat16 queries, of at most max_q_len tokens each; no query sees more than max_keys
-// keys; beside: see kv8_begin.  Heads of 64 or 128, pages of a multiple of 16 keys.
+// keys; known: see kv8_inputs.  Heads of 64 or 128, pages of a multiple of 16 keys.
 RLLM_EXPORT int rllm_attention_e4m3_columns(const void* q, int q_stride, void* out, const void* kcache, const void* vcache,
                                             const void* kscale, const void* vscale, const int* block_table, int max_blocks,
                                             const int* q_start, const int* seq_lens, int seq_begin, int seq_end, int max_q_len,
                                             int max_keys, int nq, int nkv, int d, int page_size, int num_pages, int window,
-                                            float scale, int beside, int* err, cudaStream_t stream) {
+                                            float scale, int known, int* err, cudaStream_t stream) {
   if (max_q_len <= 0 || seq_end <= seq_begin) return 0;
   if (!q || !out || !kcache || !vcache || !kscale || !vscale || !block_table || !q_start || !seq_lens || !err || max_blocks <= 0 ||
       seq_begin < 0 || nq <= 0 || nkv <= 0 || nq % nkv || page_size <= 0 || num_pages <= 0 || window < 0 || !(scale == scale) ||
@@ -659,7 +660,7 @@ RLLM_EXPORT int rllm_attention_e4m3_columns(const void* q, int q_stride, void* o
   const long long rows = (long long)max_q_len * (nq / nkv);
 #define EC_LAUNCH(DD, NBB)                                                                                                             \
   return ec_launch<DD, NBB>(q, q_stride, out, kcache, vcache, kscale, vscale, block_table, max_blocks, q_start, seq_lens, seq_begin,   \
-                            seq_end - seq_begin, max_q_len, max_keys, nq, nkv, page_size, num_pages, window, scale, beside, err, stream)
+                            seq_end - seq_begin, max_q_len, max_keys, nq, nkv, page_size, num_pages, window, scale, known, err, stream)
   if (d == 64) { if (rows <= 8) EC_LAUNCH(64, 1); if (rows <= 16) EC_LAUNCH(64, 2); if (rows <= 24) EC_LAUNCH(64, 3); EC_LAUNCH(64, 4); }
   if (rows <= 8) EC_LAUNCH(128, 1);
   if (rows <= 16) EC_LAUNCH(128, 2);

@@ -56,9 +56,10 @@ attention_e4m3_tcgen05_kernel(const bf16* q, int q_stride, bf16* __restrict__ ou
                               const unsigned char* __restrict__ vcache, const unsigned char* __restrict__ kscale,
                               const unsigned char* __restrict__ vscale, const int* __restrict__ block_table, int max_blocks,
                               const int* __restrict__ q_start, const int* __restrict__ seq_lens, int seq_begin, int nq, int nkv,
-                              int page_size, int num_pages, int window, float scale_log2, int beside, int* __restrict__ err) {
+                              int page_size, int num_pages, int window, float scale_log2, int known, int* __restrict__ err) {
   constexpr int DP = D / 64, QPANEL = E8_BM * 128, KPANEL = E8_BN * 128, STAGE = E8_BN * D * 2, NS = e8_stages<D>();
   extern __shared__ __align__(1024) unsigned char e8_raw[];
+  kv8_inputs(known, block_table, q_start, seq_lens);
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int splits = gridDim.x, rank = blockIdx.x;       // the cluster is the grid's x
   const int kvh = blockIdx.y % nkv, s = seq_begin + blockIdx.z;
@@ -99,7 +100,7 @@ attention_e4m3_tcgen05_kernel(const bf16* q, int q_stride, bf16* __restrict__ ou
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tg_smem(tmem_slot)), "r"(256) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
-  kv8_begin(beside, q, kcache, vcache, kscale, vscale);
+  kv8_begin(known, q, kcache, vcache, kscale, vscale);
 
   // Queries as halves: a row by 2^(13 - e) with 2^e its largest's power; eight lanes a row (four for heads of 64)
   float my_factor = 0.f;
@@ -145,7 +146,7 @@ attention_e4m3_tcgen05_kernel(const bf16* q, int q_stride, bf16* __restrict__ ou
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   if (warp < 4) my_factor = ((float*)sV)[threadIdx.x];
   __syncthreads();
-  kv8_let_in(beside);                                        // behind the allocation: see pdl_launch
+  kv8_let_in(known);                                         // behind the allocation: see pdl_launch
   const unsigned tmem_s = __shfl_sync(0xffffffffu, *tmem_slot, 0), tmem_o = tmem_s + 2 * E8_BN;      // two tiles' scores: 128 + D <= 256 columns
 
   float m_ref = -INFINITY, l = 0.f;
@@ -537,7 +538,7 @@ attention_e4m3_tcgen05_kernel(const bf16* q, int q_stride, bf16* __restrict__ ou
   if (warp == 8) {
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_s), "r"(256) : "memory");
   }
-  if (splits == 1) { kv8_end(beside); return; }
+  if (splits == 1) { kv8_end(known); return; }
   namespace cg = cooperative_groups;
   cg::cluster_group cluster = cg::this_cluster();
   cluster.sync();
@@ -561,14 +562,14 @@ attention_e4m3_tcgen05_kernel(const bf16* q, int q_stride, bf16* __restrict__ ou
     *(uint2*)(out + ((size_t)(qs + t0 + tok) * nq + kvh * g + row - tok * g) * D + c) = make_uint2(*(const unsigned*)&lo, *(const unsigned*)&hi);
   }
   cluster.sync();                                          // nobody leaves while its shared memory is being read
-  kv8_end(beside);
+  kv8_end(known);
 }
 
 template <int D>
 static int e8_launch(const void* q, int q_stride, void* out, const void* kcache, const void* vcache, const void* kscale,
                      const void* vscale, const int* block_table, int max_blocks, const int* q_start, const int* seq_lens,
                      int seq_begin, int num_seqs, int max_q_len, int max_keys, int nq, int nkv, int page_size, int num_pages,
-                     int window, float scale, int beside, int* err, cudaStream_t stream) {
+                     int window, float scale, int known, int* err, cudaStream_t stream) {
   auto* kernel = attention_e4m3_tcgen05_kernel<D>;
   static SmemLimit limit;
   if (const int e = limit.allow(kernel, e8_smem_bytes<D>())) return e;
@@ -595,18 +596,18 @@ static int e8_launch(const void* q, int q_stride, void* out, const void* kcache,
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, (const bf16*)q, q_stride, (bf16*)out, (const unsigned char*)kcache,
                                            (const unsigned char*)vcache, (const unsigned char*)kscale, (const unsigned char*)vscale,
                                            block_table, max_blocks, q_start, seq_lens, seq_begin, nq, nkv, page_size, num_pages, window,
-                                           scale * 1.4426950408889634f, beside, err);
+                                           scale * 1.4426950408889634f, known, err);
   if (e != cudaSuccess) { cudaGetLastError(); return (int)e; }
   return 0;
 }
 
 // Sequences seq_begin .. seq_end - 1 of bfloat16 queries, of at most max_q_len tokens each; no query sees more than max_keys
-// keys; beside: see kv8_begin.  Heads of 64 or 128, up to 128 of them a kv head, pages of any size.
+// keys; known: see kv8_inputs.  Heads of 64 or 128, up to 128 of them a kv head, pages of any size.
 RLLM_EXPORT int rllm_attention_e4m3_tcgen05(const void* q, int q_stride, void* out, const void* kcache, const void* vcache,
                                             const void* kscale, const void* vscale, const int* block_table, int max_blocks,
                                             const int* q_start, const int* seq_lens, int seq_begin, int seq_end, int max_q_len,
                                             int max_keys, int nq, int nkv, int d, int page_size, int num_pages, int window,
-                                            float scale, int beside, int* err, cudaStream_t stream) {
+                                            float scale, int known, int* err, cudaStream_t stream) {
   if (max_q_len <= 0 || seq_end <= seq_begin) return 0;
   if (!q || !out || !kcache || !vcache || !kscale || !vscale || !block_table || !q_start || !seq_lens || !err || max_blocks <= 0 ||
       seq_begin < 0 || nq <= 0 || nkv <= 0 || nq % nkv || page_size <= 0 || num_pages <= 0 || window < 0 || !(scale > 0.f) || scale > 3e38f)
@@ -616,7 +617,7 @@ RLLM_EXPORT int rllm_attention_e4m3_tcgen05(const void* q, int q_stride, void* o
     return RLLM_E_UNSUPPORTED;
   if ((long long)num_pages * nkv * page_size > 0x7fffffffLL) return RLLM_E_UNSUPPORTED;      // cache rows are counted in 32 bits
 #define E8_LAUNCH(DD) return e8_launch<DD>(q, q_stride, out, kcache, vcache, kscale, vscale, block_table, max_blocks, q_start, seq_lens, \
-      seq_begin, seq_end - seq_begin, max_q_len, max_keys, nq, nkv, page_size, num_pages, window, scale, beside, err, stream)
+      seq_begin, seq_end - seq_begin, max_q_len, max_keys, nq, nkv, page_size, num_pages, window, scale, known, err, stream)
   if (d == 64) E8_LAUNCH(64);
   E8_LAUNCH(128);
 }

@@ -308,9 +308,10 @@ kv_e4m3_widen_kernel(const int* __restrict__ block_table, int max_blocks, const 
                      const int* __restrict__ seq_lens, int seq_begin, const unsigned char* __restrict__ kcache,
                      const unsigned char* __restrict__ vcache, const unsigned char* __restrict__ kscale,
                      const unsigned char* __restrict__ vscale, bf16* __restrict__ kdense, bf16* __restrict__ vdense,
-                     unsigned* __restrict__ marks, int nkv, int page_size, int num_pages, int window, int beside, int* __restrict__ err) {
+                     unsigned* __restrict__ marks, int nkv, int page_size, int num_pages, int window, int known, int* __restrict__ err) {
   constexpr int BN = 8192 / D, PIECES = D / 16;      // BN * PIECES = 512: a thread has 16 numbers of a key and of a value
   __shared__ unsigned mark[AT_MARK];
+  kv8_inputs(known, block_table, q_start, seq_lens);
   const int page_shift = (page_size & (page_size - 1)) == 0 ? __ffs(page_size) - 1 : -1;
   const int s = seq_begin + blockIdx.z, kvh = blockIdx.y;
   const int len = seq_lens[s], pos0 = len - (q_start[s + 1] - q_start[s]);
@@ -331,9 +332,9 @@ kv_e4m3_widen_kernel(const int* __restrict__ block_table, int max_blocks, const 
       atomicOr(&mark[0], AT_MARK_MISSING);
     }
   }
-  kv8_begin(beside, kcache, vcache, kscale, vscale, kdense, vdense, marks);
-  kv8_let_in(beside);
-  if (empty) { kv8_end(beside); return; }            // (the whole block)
+  kv8_begin(known, kcache, vcache, kscale, vscale, kdense, vdense, marks);
+  kv8_let_in(known);
+  if (empty) { kv8_end(known); return; }            // (the whole block)
   const bool held = row >= 0;
   const uint4 kx = held ? *(const uint4*)(kcache + row * D + c) : make_uint4(0u, 0u, 0u, 0u);
   const uint4 vx = held ? *(const uint4*)(vcache + row * D + c) : make_uint4(0u, 0u, 0u, 0u);
@@ -355,16 +356,16 @@ kv_e4m3_widen_kernel(const int* __restrict__ block_table, int max_blocks, const 
   }
   __syncthreads();
   if (threadIdx.x < AT_MARK) marks[(((size_t)blockIdx.z * gridDim.x + blockIdx.x) * nkv + kvh) * AT_MARK + threadIdx.x] = mark[threadIdx.x];
-  kv8_end(beside);
+  kv8_end(known);
 }
 
 // Sequences seq_begin .. seq_begin + num_seqs - 1, each from the tile of its portion's oldest visible key on, dense_tiles
-// tiles at most: kdense, vdense [num_seqs][dense_tiles][nkv][8192 / d][d], marks [num_seqs][dense_tiles][nkv][AT_MARK].  beside: see
-// kv8_begin.
+// tiles at most: kdense, vdense [num_seqs][dense_tiles][nkv][8192 / d][d], marks [num_seqs][dense_tiles][nkv][AT_MARK].  known: see
+// kv8_inputs.
 RLLM_EXPORT int rllm_kv_e4m3_widen(const int* block_table, int max_blocks, const int* q_start, const int* seq_lens, int seq_begin,
                                    int num_seqs, int dense_tiles, const void* kcache, const void* vcache, const void* kscale,
                                    const void* vscale, void* kdense, void* vdense, void* marks, int nkv, int d, int page_size,
-                                   int num_pages, int window, int beside, int* err, cudaStream_t stream) {
+                                   int num_pages, int window, int known, int* err, cudaStream_t stream) {
   if (num_seqs <= 0) return 0;
   if (!block_table || !q_start || !seq_lens || !kcache || !vcache || !kscale || !vscale || !kdense || !vdense || !marks || !err ||
       seq_begin < 0 || dense_tiles <= 0 || nkv <= 0 || page_size <= 0 || num_pages <= 0 || max_blocks <= 0 || window < 0)
@@ -374,7 +375,7 @@ RLLM_EXPORT int rllm_kv_e4m3_widen(const int* block_table, int max_blocks, const
     return RLLM_E_UNSUPPORTED;
 #define KV8_WIDEN(DD) rllm_launch_pdl(kv_e4m3_widen_kernel<DD>, dim3(dense_tiles, nkv, num_seqs), dim3(512), (size_t)0, stream, block_table, \
       max_blocks, q_start, seq_lens, seq_begin, (const unsigned char*)kcache, (const unsigned char*)vcache, (const unsigned char*)kscale,  \
-      (const unsigned char*)vscale, (bf16*)kdense, (bf16*)vdense, (unsigned*)marks, nkv, page_size, num_pages, window, beside, err)
+      (const unsigned char*)vscale, (bf16*)kdense, (bf16*)vdense, (unsigned*)marks, nkv, page_size, num_pages, window, known, err)
   if (d == 64) KV8_WIDEN(64);
   else KV8_WIDEN(128);
   RLLM_LAUNCH_CHECK();

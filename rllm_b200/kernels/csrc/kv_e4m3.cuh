@@ -19,16 +19,32 @@
 
 #define KV8_NAN_SCALE 255
 
-// A call's second kernel, which reads nothing of its first (the portions' attention behind the single tokens'), does not wait for
-// it before it begins but before it ends (`beside`): what was written ahead of both is there when it starts, for the first has let it
-// in behind its own wait, and whoever comes after it finds both complete.  It lets nobody in itself.
+// What a kernel of the attention may take for granted of the kernel ahead of it in the stream (`known`):
+//   KV8_ANY      nothing.  The kernel ahead may be the one that makes the step's lengths, row ranges and block table (decode_advance lets
+//                the next kernel in and then counts the lengths up), so they too are read behind the wait for it (kv8_inputs).
+//   KV8_LENGTHS  it leaves those alone: every kernel but the one directly ahead is complete when this one starts, so they are read, and
+//                tiles looked up, while that one ends.
+//   KV8_BESIDE   it is the first kernel of the same call, of which this one reads nothing (the portions' attention behind the single
+//                tokens').  This one does not wait before it begins but before it ends: what was written ahead of both is there when it
+//                starts, for the first has let it in behind its own wait, and whoever comes after it finds both complete.  It lets
+//                nobody in itself.
+#define KV8_ANY 0
+#define KV8_BESIDE 1
+#define KV8_LENGTHS 2
 template <typename... P>
-__device__ __forceinline__ void kv8_begin(int beside, P&... ptrs) {
-  if (!beside) pdl_wait();
+__device__ __forceinline__ void kv8_inputs(int known, P&... ptrs) {
+  if (known == KV8_ANY) {
+    pdl_wait();
+    (pdl_fresh_in_place(ptrs), ...);
+  }
+}
+template <typename... P>
+__device__ __forceinline__ void kv8_begin(int known, P&... ptrs) {
+  if (known != KV8_BESIDE) pdl_wait();
   (pdl_fresh_in_place(ptrs), ...);
 }
-__device__ __forceinline__ void kv8_let_in(int beside) { if (!beside) pdl_launch(); }
-__device__ __forceinline__ void kv8_end(int beside) { if (beside) pdl_wait(); }
+__device__ __forceinline__ void kv8_let_in(int known) { if (known != KV8_BESIDE) pdl_launch(); }
+__device__ __forceinline__ void kv8_end(int known) { if (known == KV8_BESIDE) pdl_wait(); }
 
 // the scale byte of a row whose largest magnitude is `top` (finite): (bits + 0x1FFFFF) >> 23 is top's biased exponent, one
 // more where its mantissa lies above 1.75 = 448 / 256

@@ -2198,7 +2198,7 @@ def attention_e4m3_form(dtype: torch.dtype, nq: int, nkv: int, d: int, page_size
 def attention_e4m3(q: torch.Tensor, out: torch.Tensor, kcache: torch.Tensor, vcache: torch.Tensor, kscale: torch.Tensor,
                    vscale: torch.Tensor, block_table: torch.Tensor, q_start: torch.Tensor, seq_lens: torch.Tensor,
                    num_decode: int, max_q_len: int, max_seq_len: int, nq: int, nkv: int, window: int, scale: float,
-                   err: torch.Tensor) -> None:
+                   err: torch.Tensor, lengths_ready: bool = False) -> None:
     """Causal attention of a step's tokens over a cache kept in 8 bits, their own keys and values (written before) among it.
 
     q [T, >= nq d], rotated; a row's first nq d numbers are read (rows may lie apart).  Row i of ``out`` [T, nq d] gets token
@@ -2206,11 +2206,14 @@ def attention_e4m3(q: torch.Tensor, out: torch.Tensor, kcache: torch.Tensor, vca
     the first ``num_decode`` sequences bring one token each.  ``max_q_len`` and ``max_seq_len`` bound every sequence's tokens
     in this step and in the cache.  Rows behind the last sequence's stay as they are.  A page that is not held sets bit 4 of
     ``err``, and its keys are left out.  Single tokens and the others are two launches, but where no fewer sequences bring
-    several tokens and all of them few."""
+    several tokens and all of them few.
+
+    ``lengths_ready``: the caller knows that the kernel directly ahead in the stream writes neither ``q_start`` nor ``seq_lens`` nor
+    ``block_table`` (in a layer it is the cache's write); they are then read, and tiles looked up, while that kernel ends."""
     entries = (_entries.rllm_attention_e4m3_rows, _entries.rllm_attention_e4m3_columns, _entries.rllm_attention_e4m3_tcgen05,
                _entries.rllm_attention_e4m3_simt, _entries.rllm_kv_e4m3_widen, _entries.rllm_attention_dense_tcgen05)
     if _launch().e4m3_attention(entries, q, out, q_start, seq_lens, err, kcache, vcache, kscale, vscale, block_table, num_decode, max_q_len,
-                                max_seq_len, nq, nkv, window, scale, E4M3_DENSE_SCRATCH, E4M3_FORMS):
+                                max_seq_len, nq, nkv, window, scale, E4M3_DENSE_SCRATCH, E4M3_FORMS, bool(lengths_ready)):
         return
     dtype_code(q.dtype)
     S, d = seq_lens.numel(), kcache.shape[-1]

@@ -440,13 +440,14 @@ PyObject* e4m3_form(PyObject*, PyObject* const* args, Py_ssize_t n) {
 }
 
 // e4m3_attention(entries, q, out, q_start, seq_lens, err, kcache, vcache, kscale, vscale, block_table, num_decode, max_q_len,
-//                max_seq_len, nq, nkv, window, scale, scratch, forms): checked and launched.  entries: (rows, columns, tcgen05, simt, widen,
-// dense); scratch: bytes of widened keys and values at a time; forms: None, or two names (for the single tokens, for the others) in
-// place of the rule's.  False: a call that has to be refused, ops.attention_e4m3 says why.
+//                max_seq_len, nq, nkv, window, scale, scratch, forms, lengths_ready): checked and launched.  entries: (rows, columns,
+// tcgen05, simt, widen, dense); scratch: bytes of widened keys and values at a time; forms: None, or two names (for the single tokens, for
+// the others) in place of the rule's.  False: a call that has to be refused, ops.attention_e4m3 says why.
+enum Known { kAny = 0, kBeside = 1, kLengths = 2 };        // what the kernels are told of the one ahead: kernels/csrc/kv_e4m3.cuh
 PyObject* e4m3_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
   enum { kEntries = 6 };
-  if (n != 20 || !PyTuple_Check(args[0]) || PyTuple_GET_SIZE(args[0]) != kEntries)
-    return PyErr_Format(PyExc_TypeError, "e4m3_attention((entries), ... 19 arguments)");
+  if (n != 21 || !PyTuple_Check(args[0]) || PyTuple_GET_SIZE(args[0]) != kEntries || !PyBool_Check(args[20]))
+    return PyErr_Format(PyExc_TypeError, "e4m3_attention((entries), ... 20 arguments)");
   Entry* e[kEntries];
   for (int i = 0; i < kEntries; ++i) {
     PyObject* x = PyTuple_GET_ITEM(args[0], i);
@@ -497,13 +498,14 @@ PyObject* e4m3_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
     // and 16 of 8 behind 2,000, more tiles of 32 rows than SMs, would be 30 -> 35).
     const long long few = max_q * (nq / nkv);
     const bool together_all = args[19] == Py_None && decode > 0 && S - decode >= decode && (few <= 16 || (few <= 32 && S * nkv <= 148));
+    const int ahead = args[20] == Py_True ? kLengths : kAny;
     int before = -1;                                       // the form of the call's first launch
     for (int group = together_all ? 1 : 0; group < 2; ++group) {
       const long long first = group && !together_all ? decode : 0, end = group ? S : decode, longest = group ? max_q : 1;
       if (first == end || longest == 0) continue;
       // behind the single tokens' kernel, of which it reads nothing and overwrites nothing (widened tiles come from memory that the first's
       // widened tiles may just have left)
-      const int beside = group && before >= 0 && before != kDense;
+      const int known = group && before >= 0 && before != kDense ? kBeside : ahead;
       int form = named[group] >= 0 ? named[group] : e4m3_rule(dt == 1, nq, nkv, d, page, scale, longest, end - first, keys);
       // results off 16 bytes: the kernel that stores single numbers; queries off 16 bytes: one that reads them one by one
       if ((uintptr_t)po & 15) form = kSimt;
@@ -517,14 +519,14 @@ PyObject* e4m3_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
         rc = reinterpret_cast<int (*)(void*, int, void*, void*, void*, void*, void*, void*, int, void*, void*, int, int, int, int, int, int, int,
                                       int, int, int, float, int, void*, cudaStream_t)>(at_->fn)(
             pq, (int)stride, po, pk, pv, pks, pvs, pt, (int)blocks, pqs, psl, (int)first, (int)end, (int)longest, (int)keys, (int)nq, (int)nkv,
-            (int)d, (int)page, (int)pages, (int)window, (float)scale, beside, pe, stream);
+            (int)d, (int)page, (int)pages, (int)window, (float)scale, known, pe, stream);
         Py_END_ALLOW_THREADS
       } else if (form == kRows) {
         Py_BEGIN_ALLOW_THREADS
         rc = reinterpret_cast<int (*)(void*, int, void*, void*, void*, void*, void*, int, void*, int, void*, void*, int, int, int, int, int, int,
                                       int, int, int, int, float, int, void*, cudaStream_t)>(at_->fn)(
             pq, (int)stride, po, pk, pv, pks, pvs, dt, pt, (int)blocks, pqs, psl, (int)first, (int)end, (int)longest, (int)keys, (int)nq, (int)nkv,
-            (int)d, (int)page, (int)pages, (int)window, (float)scale, beside, pe, stream);
+            (int)d, (int)page, (int)pages, (int)window, (float)scale, known, pe, stream);
         Py_END_ALLOW_THREADS
       } else if (form == kSimt) {
         const long long tokens = std::min(T, (end - first) * longest);
@@ -548,7 +550,7 @@ PyObject* e4m3_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
           rc = reinterpret_cast<int (*)(void*, int, void*, void*, int, int, int, void*, void*, void*, void*, void*, void*, void*, int, int, int, int,
                                         int, int, void*, cudaStream_t)>(e[4]->fn)(
               pt, (int)blocks, pqs, psl, (int)s, (int)m, (int)tiles, pk, pv, pks, pvs, pd, pd + together * a_sequence, pm, (int)nkv, (int)d,
-              (int)page, (int)pages, (int)window, beside && s == first, pe, stream);
+              (int)page, (int)pages, (int)window, s == first ? known : kLengths, pe, stream);
           Py_END_ALLOW_THREADS
           if (!finish(rc, at_->what)) return nullptr;
           Py_BEGIN_ALLOW_THREADS

@@ -458,8 +458,9 @@ class PagedAttention(Mixer):
             elif rd:
                 ops.rope_kv_write(qkv, ctx.positions, ctx.token_seq, inv_freq, rd, None, None, None, self.nq, nkv_here,
                                   self.d, ctx.err, write_kv=False)
+            # (the kernel directly ahead is the write, a rotation or the projection)
             ops.attention_e4m3(qkv, out, *pages, table, ctx.q_start, ctx.seq_lens, ctx.num_decode, ctx.max_q_len,
-                               ctx.max_seq_len, self.nq, self.nkv, int(self.window or 0), self.scale, ctx.err)
+                               ctx.max_seq_len, self.nq, self.nkv, int(self.window or 0), self.scale, ctx.err, lengths_ready=True)
             return out
         window = int(self.window or 0)
         stride = qkv.shape[1]
