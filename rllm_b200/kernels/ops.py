@@ -2223,5 +2223,7 @@ def attention_e4m3(q: torch.Tensor, out: torch.Tensor, kcache: torch.Tensor, vca
         raise KernelError("attention_e4m3: q must be [T, >= nq d] and out [T, nq d] of one type, their rows contiguous")
     _e4m3_cache(kcache, vcache, kscale, vscale, block_table, nkv, d, q_start, seq_lens, err)
     _beside(kcache, q, out)
-    raise KernelError("attention_e4m3: nq a multiple of nkv, q_start [S + 1] and seq_lens [S], num_decode of them with one token, a row of "
-                      "block_table each, that can hold max_seq_len tokens")
+    if q.shape[0] > 1 and q.stride(0) > 0x7FFFFFFF:
+        raise KernelError("attention_e4m3: rows of q that lie 2^31 numbers apart or more")
+    raise KernelError("attention_e4m3: nq a multiple of nkv, window >= 0, q_start [S + 1] and seq_lens [S], num_decode of them with one token, "
+                      "a row of block_table each, that can hold max_seq_len tokens")

@@ -292,7 +292,7 @@ bool e4m3_cache(PyObject* const* args, long long nkv, long long d, int device) {
   if (k.scalar_type() != at::kFloat8_e4m3fn || v.scalar_type() != at::kFloat8_e4m3fn || ks.scalar_type() != at::kFloat8_e8m0fnu ||
       vs.scalar_type() != at::kFloat8_e8m0fnu || table.scalar_type() != at::kInt)
     return false;
-  if (k.dim() != 4 || k.size(1) != nkv || k.size(3) != d || v.sizes() != k.sizes() || ks.sizes() != k.sizes().slice(0, 3) ||
+  if (k.dim() != 4 || k.size(1) != nkv || k.size(3) != d || k.size(2) > 0x7fffffffLL || v.sizes() != k.sizes() || ks.sizes() != k.sizes().slice(0, 3) ||
       vs.sizes() != ks.sizes() || table.dim() != 2)
     return false;
   for (int i = 0; i < 5; ++i) {
@@ -301,6 +301,9 @@ bool e4m3_cache(PyObject* const* args, long long nkv, long long d, int device) {
   }
   return true;
 }
+
+// The entry points count in 32 bits: a bound that is larger than what it bounds can be becomes the largest such number, never its low bits.
+long long in_32_bits(long long x) { return std::min(x, 0x7fffffffLL); }
 
 // all of args[0 .. n - 1] are tensors on CUDA devices (asked before CUDA is asked for its current one)
 bool cuda_tensors(PyObject* const* args, Py_ssize_t n) {
@@ -364,7 +367,7 @@ PyObject* e4m3_write(PyObject*, PyObject* const* args, Py_ssize_t n) {
     rc = reinterpret_cast<int (*)(void*, int, void*, long long, void*, void*, void*, int, void*, int, int, void*, void*, void*, void*, int, int,
                                   int, int, int, int, void*, cudaStream_t)>(e->fn)(
         qkv.data_ptr(), dt, q.data_ptr(), stride, at_(3), at_(4), freq, (int)rot, table.data_ptr(), (int)table.size(1), (int)table.size(0),
-        at_(6), at_(7), at_(8), at_(9), (int)T, (int)nq, (int)nkv, (int)d, (int)k.size(2), (int)k.size(0), at_(5), stream);
+        at_(6), at_(7), at_(8), at_(9), (int)T, (int)nq, (int)nkv, (int)d, (int)k.size(2), (int)in_32_bits(k.size(0)), at_(5), stream);
     Py_END_ALLOW_THREADS
     if (!finish(rc, e->what)) return nullptr;
     Py_RETURN_TRUE;
@@ -396,7 +399,7 @@ PyObject* e4m3_read(PyObject*, PyObject* const* args, Py_ssize_t n) {
     rc = reinterpret_cast<int (*)(void*, void*, void*, int, int, void*, void*, void*, void*, void*, void*, int, int, int, int, int, int, void*,
                                   cudaStream_t)>(e->fn)(
         at_(3), at_(4), table.data_ptr(), (int)table.size(1), (int)table.size(0), at_(6), at_(7), at_(8), at_(9), ok.data_ptr(), ov.data_ptr(), dt,
-        (int)T, (int)k.size(1), (int)k.size(3), (int)k.size(2), (int)k.size(0), at_(5), stream);
+        (int)T, (int)k.size(1), (int)k.size(3), (int)k.size(2), (int)in_32_bits(k.size(0)), at_(5), stream);
     Py_END_ALLOW_THREADS
     if (!finish(rc, e->what)) return nullptr;
     Py_RETURN_TRUE;
@@ -471,22 +474,24 @@ PyObject* e4m3_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
     for (int i = 0; i < 8 && !bad; ++i) v[i] = i == 6 ? 0 : whole(args[11 + i], bad);
     const double scale = bad ? 0. : PyFloat_AsDouble(args[17]);
     if (bad || PyErr_Occurred()) return nullptr;
-    const long long decode = v[0], max_q = v[1], most = v[2], nq = v[3], nkv = v[4], window = v[5], scratch = v[7];
+    const long long decode = v[0], nq = v[3], nkv = v[4], window = in_32_bits(v[5]), scratch = v[7];
     const at::Tensor &q = THPVariable_Unpack(args[1]), &out = THPVariable_Unpack(args[2]), &k = THPVariable_Unpack(args[6]),
                      &table = THPVariable_Unpack(args[10]);
     const int device = c10::cuda::current_device(), dt = float_code(q);
-    if (dt < 0 || k.dim() != 4 || nq <= 0 || nkv <= 0 || nq % nkv) Py_RETURN_FALSE;
-    const long long d = k.size(3), page = k.size(2), pages = k.size(0);
+    if (dt < 0 || k.dim() != 4 || nq <= 0 || nkv <= 0 || nq % nkv || nq > 0x7fffffffLL || window < 0) Py_RETURN_FALSE;
+    const long long d = k.size(3), page = k.size(2), pages = in_32_bits(k.size(0));
     if (!e4m3_cache(args + 6, nkv, d, device)) Py_RETURN_FALSE;
     for (int i = 3; i < 6; ++i)
       if (!vector_of_ints(THPVariable_Unpack(args[i]), device)) Py_RETURN_FALSE;
     const long long S = THPVariable_Unpack(args[4]).numel(), blocks = table.size(1);
-    if (THPVariable_Unpack(args[3]).numel() != S + 1 || decode < 0 || decode > S || table.size(0) < S || max_q < 0 || most < 0 ||
-        most > blocks * page || q.dim() != 2 || out.dim() != 2 || out.scalar_type() != q.scalar_type() || q.stride(1) != 1 ||
+    if (THPVariable_Unpack(args[3]).numel() != S + 1 || decode < 0 || decode > S || table.size(0) < S || v[1] < 0 || v[2] < 0 ||
+        v[2] > blocks * page || q.dim() != 2 || out.dim() != 2 || out.scalar_type() != q.scalar_type() || q.stride(1) != 1 ||
         out.size(1) != nq * d || q.size(1) < nq * d || q.size(0) < out.size(0) || !out.is_contiguous() || q.get_device() != device ||
         out.get_device() != device)
       Py_RETURN_FALSE;
-    const long long T = out.size(0), stride = q.stride(0);
+    // a single row may have any stride; no sequence has more tokens than out has rows, nor more keys than its length, an int, says
+    const long long T = in_32_bits(out.size(0)), stride = q.size(0) > 1 ? q.stride(0) : nq * d, max_q = std::min(v[1], T), most = in_32_bits(v[2]);
+    if (stride > 0x7fffffffLL) Py_RETURN_FALSE;
     if (T == 0 || S == 0) Py_RETURN_TRUE;
     const long long keys = window > 0 && window + max_q < most ? window + max_q : most;
     void *pq = q.data_ptr(), *po = out.data_ptr(), *pqs = THPVariable_Unpack(args[3]).data_ptr(), *psl = THPVariable_Unpack(args[4]).data_ptr(),
