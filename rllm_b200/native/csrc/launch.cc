@@ -430,6 +430,19 @@ Form e4m3_rule(bool bf16, long long nq, long long nkv, long long d, long long pa
   return rows_take ? kRows : kSimt;
 }
 
+// Whether a kernel takes a call at all: its grid's places, and what it reads or stores 16 bytes at a time.  The CUDA-core one takes every call.
+bool e4m3_takes(Form form, long long nq, long long nkv, long long d, long long page, long long max_q_len, long long seqs, bool scales_on_16,
+                bool queries_on_16, bool results_on_16) {
+  if (form == kSimt) return true;
+  const long long g = nq / nkv, places = 65535;
+  if (!results_on_16 || (form != kDense && seqs > places)) return false;
+  const long long rows = max_q_len * g, tile = form == kColumns ? std::min((rows + 7) / 8 * 8, 32LL) : 8;
+  if (form == kRows || form == kColumns) return scales_on_16 && page % 16 == 0 && (rows + tile - 1) / tile * nkv <= places;
+  if (!queries_on_16 || g > 128) return false;
+  const long long tokens = 128 / g;
+  return form == kDense ? nkv <= places : (max_q_len + tokens - 1) / tokens * nkv <= places;
+}
+
 // e4m3_form(bfloat16, nq, nkv, d, page_size, scale, max_q_len, num_seqs, max_keys)
 PyObject* e4m3_form(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (n != 9) return PyErr_Format(PyExc_TypeError, "e4m3_form(bfloat16, nq, nkv, d, page_size, scale, max_q_len, num_seqs, max_keys)");
@@ -511,10 +524,13 @@ PyObject* e4m3_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
       // behind the single tokens' kernel, of which it reads nothing and overwrites nothing (widened tiles come from memory that the first's
       // widened tiles may just have left)
       const int known = group && before >= 0 && before != kDense ? kBeside : ahead;
-      int form = named[group] >= 0 ? named[group] : e4m3_rule(dt == 1, nq, nkv, d, page, scale, longest, end - first, keys);
-      // results off 16 bytes: the kernel that stores single numbers; queries off 16 bytes: one that reads them one by one
-      if ((uintptr_t)po & 15) form = kSimt;
-      else if ((form == kTcgen05 || form == kDense) && (stride % 8 || ((uintptr_t)pq & 15))) form = page % 16 ? kSimt : kRows;
+      Form form = named[group] >= 0 ? (Form)named[group] : e4m3_rule(dt == 1, nq, nkv, d, page, (float)scale, longest, end - first, keys);
+      // off 16 bytes, or too many for its grid: the kernel that reads queries one by one, or the one that takes everything
+      auto takes = [&](Form f) {
+        return e4m3_takes(f, nq, nkv, d, page, longest, end - first, (((uintptr_t)pks | (uintptr_t)pvs) & 15) == 0,
+                          (((uintptr_t)pq | (uintptr_t)stride * 2) & 15) == 0, ((uintptr_t)po & 15) == 0);
+      };
+      if (!takes(form)) form = form != kRows && (d == 64 || d == 128) && takes(kRows) ? kRows : kSimt;
       before = form;
       Entry* at_ = e[form == kRows ? 0 : form == kColumns ? 1 : form == kTcgen05 ? 2 : form == kSimt ? 3 : 5];
       if (!ready(at_)) return nullptr;
