@@ -2168,9 +2168,11 @@ E4M3_FORMS = None                   # two names in place of attention_e4m3_form'
 E4M3_DENSE_SCRATCH = 512 << 20      # bytes of widened keys and values at a time; more only where one sequence needs more
 
 
-def e4m3_dense_scratch(nkv: int, d: int, max_seq_len: int) -> int:
-    """The most bytes that ``attention_e4m3`` takes for a while for prompt portions of sequences of up to so many tokens."""
-    if d not in (64, 128):
+def e4m3_dense_scratch(nkv: int, d: int, max_seq_len: int, dtype: torch.dtype = torch.bfloat16, nq: Optional[int] = None,
+                       scale: float = 1.0) -> int:
+    """The most bytes that ``attention_e4m3`` takes for a while for prompt portions of sequences of up to so many tokens; none where
+    ``attention_e4m3_form`` never says "dense"."""
+    if d not in (64, 128) or dtype is not torch.bfloat16 or (nq or nkv) // nkv > 128 or not scale > 0:
         return 0
     bn = 8192 // d
     return max(E4M3_DENSE_SCRATCH, 4 * (max_seq_len // bn + 2) * nkv * bn * d)

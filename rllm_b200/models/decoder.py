@@ -104,7 +104,7 @@ class DecoderModel:
         return max((b.mixer.step_scratch() for b in self.blocks), default=0)
 
     def step_scratch_8_bit(self, max_model_len: int) -> int:
-        return max((b.mixer.step_scratch_8_bit(max_model_len) for b in self.blocks), default=0)
+        return max((b.mixer.step_scratch_8_bit(max_model_len, self.dtype) for b in self.blocks), default=0)
 
     # -- cache ------------------------------------------------------------
     def check_8_bit_cache(self) -> None:

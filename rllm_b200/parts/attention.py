@@ -304,8 +304,8 @@ class PagedAttention(Mixer):
             return "attention with head norms, biases, value heads of their own size or other options keeps its pages in the run's type"
         return None
 
-    def step_scratch_8_bit(self, max_model_len: int) -> int:
-        return max(self.step_scratch(), ops.e4m3_dense_scratch(self.nkv, self.d, max_model_len))
+    def step_scratch_8_bit(self, max_model_len: int, dtype: torch.dtype) -> int:
+        return max(self.step_scratch(), ops.e4m3_dense_scratch(self.nkv, self.d, max_model_len, dtype, self.nq, self.scale))
 
     # -- compute ----------------------------------------------------------
     def fused_residual(self, num_rows: int, dtype: torch.dtype) -> bool:

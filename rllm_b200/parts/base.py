@@ -246,8 +246,8 @@ class Mixer(Part):
         scales)."""
         return "its mixer keeps its pages in the run's type"
 
-    def step_scratch_8_bit(self, max_model_len: int) -> int:
-        """``step_scratch`` where the pages are kept in 8 bits and no sequence passes ``max_model_len`` tokens."""
+    def step_scratch_8_bit(self, max_model_len: int, dtype: torch.dtype) -> int:
+        """``step_scratch`` where the pages are kept in 8 bits, no sequence passes ``max_model_len`` tokens and the run's type is ``dtype``."""
         return self.step_scratch()
 
     def step_scratch(self) -> int:
