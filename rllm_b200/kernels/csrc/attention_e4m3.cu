@@ -140,12 +140,15 @@ static int e4_check(const void* q, const void* out, const void* kcache, const vo
 //   V: it needs keys 2 tig, 2 tig + 1 and those plus 8, and d / 8 dims: bytes gid d / 8 .. of four rows; the bytes of two
 //      keys are interleaved (prmt) into pairs along the keys.
 //   P^T: the accumulators of S^T hold (key gid, rows 2 tig, 2 tig + 1); movmatrix turns them into (keys 2 tig, 2 tig + 1, row gid).
-// Factors: a key's power of two and its row's factor multiply the score; a value's power multiplies the weight, relative to
-// 2^E, E a running reference of the warp as the maximum is of a row: both move only when passed by 2^4, so that a tile costs
-// one vote, and P 2^(ev - E) 2^7 stays at or below 2^15, within a half (the 2^7 puts the halves' smallest step, 2^-24, at
-// 2^-31 of a weight of 1).  The denominator sums the weights themselves.
+// Factors: a key's power of two and its row's factor multiply the score s; a value's power rides in the weight, 2^(s + ev).  A row has
+// two references, m of its scores and t of its weights with their values' powers: the denominator sums 2^(s - m) in float32, and
+// the second product takes 2^(s + ev - t + 11) as halves, so that what a row keeps of its weights does not depend on how large the
+// values are that it, or another row, does not look at (with one reference of the values' powers for all rows, a row that looked
+// at values 2^20 below the others' kept 12 bits, and at 2^32 below zeros).  Both move only when passed by 2^4, so that a tile costs
+// one vote, and the halves stay at or below 2^15; their smallest step, 2^-24, lies at 2^-35 of the row's largest weight.  References
+// are whole numbers: what they are multiplied by when they move, or when parts meet, is exact.
 // Queries are put into halves after a division by a power of two of the row's own (bfloat16: exact down to 2^-27 of the
-// row's largest; float32: two halves, 22 bits, and P likewise, with which the path is as good as float32 products).
+// row's largest; float32: two halves, 22 bits, and P likewise).
 // What bounds it: over few keys the start (780 instructions a warp beside its keys: queries, merge) and the latency of one or two
 // tiles, 4.5 us for 511 keys of 8 heads of 64; over many the instructions, 286 for 16 keys of 128 dims (4 KB), a third of them
 // conversions to halves at half the ALU's rate: 64 sequences of 8,191 keys, 8 heads of 128, 221 us, 4.9 TB/s.
@@ -154,9 +157,14 @@ static int e4_check(const void* q, const void* out, const void* kcache, const vo
 // cluster, partial results are merged in shared memory, first the CTA's, then, each CTA a slice, the cluster's (distributed
 // shared memory): no workspace, no counters, and a captured graph needs nothing of its own.
 #define E4_WARPS 4
-#define E4_SLACK 4                   // log2 of how far a score may pass the row's reference, and a value's power the warp's
-#define E4_SHIFT 7                   // log2 of the weights' factor: 2 E4_SLACK + E4_SHIFT = 15
+#define E4_SLACK 4                   // log2 of how far a score, and a weight with its value's power, may pass the row's reference
+#define E4_SHIFT 11                  // log2 of the weights' factor: E4_SLACK + E4_SHIFT = 15
 #define E4_NONE -3.0e38f             // the reference of a row that has seen nothing: 2^(s - reference) is 0 for a masked s, and any score moves it
+// 2^x of a whole x <= 0, or 0 where it is below the normal numbers'
+__device__ __forceinline__ float e4_power(float x) {
+  const int e = (int)fmaxf(x, -127.f) + 127;
+  return __uint_as_float((unsigned)e << 23);
+}
 __device__ __forceinline__ void e4_mma(float* c, const unsigned* a, unsigned b0, unsigned b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
@@ -380,11 +388,10 @@ attention_e4m3_rows_kernel(const T* q, int q_stride, T* __restrict__ out, const 
     for (int c = 0; c < 2; ++c) rfc[nb][c] = __shfl_sync(0xffffffffu, up, (2 * tig + c) * 4);
   }
 
-  float o[NB][D / 16][4], m[NB][2], l[NB][2];
-  int E = -1000;                       // the warp's reference of the values' powers, as a scale byte
+  float o[NB][D / 16][4], m[NB][2], t[NB][2], l[NB][2];
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) {
-    m[nb][0] = m[nb][1] = E4_NONE;
+    m[nb][0] = m[nb][1] = t[nb][0] = t[nb][1] = E4_NONE;
     l[nb][0] = l[nb][1] = 0.f;
 #pragma unroll
     for (int j = 0; j < D / 16; ++j) o[nb][j][0] = o[nb][j][1] = o[nb][j][2] = o[nb][j][3] = 0.f;
@@ -463,53 +470,49 @@ attention_e4m3_rows_kernel(const T* q, int q_stride, T* __restrict__ out, const 
     }
     e4_copy_wait<1>();                 // the values are here; the next keys may be on their way
     __syncwarp();
-    int vb[4];
+    float ev[4];                       // log2 of a value's power, NaN where the value is (a row that was not read has some byte)
 #pragma unroll
-    for (int x = 0; x < 4; ++x) vb[x] = st[(x >> 1) * TB + 32 * D + 16 + gid + 8 * (x & 1)];
-    if (!whole) {                      // (a row that was not read has zeros, whatever its scale)
-#pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        const int j = j0 + gid + 8 * x;
-        if (j < kmin || j >= kend) vb[x] = 0;
-      }
+    for (int x = 0; x < 4; ++x) {
+      const int vb = st[(x >> 1) * TB + 32 * D + 16 + gid + 8 * (x & 1)];
+      ev[x] = vb == KV8_NAN_SCALE ? __uint_as_float(0x7FC00000u) : (float)(vb - 127);
     }
-    bool need = max(max(vb[0], vb[1]), max(vb[2], vb[3])) > E + E4_SLACK;
+    bool need = false;
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) need = need || sc[e >> 2][nb][e & 3] > m[nb][e & 1] + (float)E4_SLACK;
-    if (__any_sync(0xffffffffu, need)) {
-      int vmax = 0;
-#pragma unroll
-      for (int x = 0; x < 4; ++x) vmax = max(vmax, vb[x] == KV8_NAN_SCALE ? 0 : vb[x]);
-      vmax = __reduce_max_sync(0xffffffffu, vmax);
-      float fe = 1.0f;
-      if (vmax > E + E4_SLACK) {
-        fe = __uint_as_float((unsigned)max(127 + E - vmax, 0) << 23);
-        E = vmax;
+      for (int e = 0; e < 8; ++e) {
+        const float s = sc[e >> 2][nb][e & 3];
+        need = need || s > m[nb][e & 1] + (float)E4_SLACK || s + ev[e >> 1] > t[nb][e & 1] + (float)E4_SLACK;
       }
+    if (__any_sync(0xffffffffu, need)) {
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb) {
         float corr[2];
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           float mx = fmaxf(fmaxf(sc[0][nb][c], sc[0][nb][c + 2]), fmaxf(sc[1][nb][c], sc[1][nb][c + 2]));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-          const bool moves = mx > m[nb][c] + (float)E4_SLACK;
-          corr[c] = moves ? e4_ex2(m[nb][c] - mx) : 1.0f;
-          if (moves) m[nb][c] = mx;
-          l[nb][c] *= corr[c];
-          corr[c] *= fe;
+          float tx = fmaxf(fmaxf(sc[0][nb][c] + ev[0], sc[0][nb][c + 2] + ev[1]), fmaxf(sc[1][nb][c] + ev[2], sc[1][nb][c + 2] + ev[3]));
+#pragma unroll
+          for (int x = 4; x < 32; x <<= 1) {
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
+            tx = fmaxf(tx, __shfl_xor_sync(0xffffffffu, tx, x));
+          }
+          corr[c] = 1.0f;
+          if (mx > m[nb][c] + (float)E4_SLACK) {
+            mx = ceilf(mx);
+            l[nb][c] *= e4_power(m[nb][c] - mx);
+            m[nb][c] = mx;
+          }
+          if (tx > t[nb][c] + (float)E4_SLACK) {
+            tx = ceilf(tx);
+            corr[c] = e4_power(t[nb][c] - tx);
+            t[nb][c] = tx;
+          }
         }
 #pragma unroll
         for (int j = 0; j < D / 16; ++j) { o[nb][j][0] *= corr[0]; o[nb][j][1] *= corr[1]; o[nb][j][2] *= corr[0]; o[nb][j][3] *= corr[1]; }
       }
     }
-    float vf[4];                       // 2^(ev - E + E4_SHIFT); infinity for a NaN scale
-#pragma unroll
-    for (int x = 0; x < 4; ++x) vf[x] = __uint_as_float((unsigned)min(max(vb[x] == KV8_NAN_SCALE ? 255 : 127 + E4_SHIFT + vb[x] - E, 0), 255) << 23);
     unsigned pb[2][NB][2 * TERMS];
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
@@ -518,11 +521,10 @@ attention_e4m3_rows_kernel(const T* q, int q_stride, T* __restrict__ out, const 
         float w[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float p = e4_ex2(sc[u][nb][e] - m[nb][e & 1]);
-          l[nb][e & 1] += p;
-          w[e] = p * vf[2 * u + (e >> 1)];
+          l[nb][e & 1] += e4_ex2(sc[u][nb][e] - m[nb][e & 1]);
+          w[e] = e4_ex2(sc[u][nb][e] + (ev[2 * u + (e >> 1)] - (t[nb][e & 1] - (float)E4_SHIFT)));
         }
-        if (!clear) {                  // 0 times an infinite power is not 0
+        if (!clear) {                  // (a masked score plus a NaN is one)
 #pragma unroll
           for (int e = 0; e < 4; ++e)
             if (!(seen >> (nb * 8 + u * 4 + e) & 1u)) w[e] = 0.f;
@@ -578,9 +580,11 @@ attention_e4m3_rows_kernel(const T* q, int q_stride, T* __restrict__ out, const 
   constexpr int LD = D + 4;
   float* part = e4_smem;
   float* sM = part + E4_WARPS * R * LD;              // [warps][R]
-  float* sL = sM + E4_WARPS * R;
+  float* sT = sM + E4_WARPS * R;
+  float* sL = sT + E4_WARPS * R;
   float* cM = sL + E4_WARPS * R;                     // [R] the CTA's
-  float* cL = cM + R;
+  float* cT = cM + R;
+  float* cL = cT + R;
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
@@ -594,20 +598,20 @@ attention_e4m3_rows_kernel(const T* q, int q_stride, T* __restrict__ out, const 
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         sM[warp * R + nb * 8 + 2 * tig + c] = m[nb][c];
+        sT[warp * R + nb * 8 + 2 * tig + c] = t[nb][c];
         sL[warp * R + nb * 8 + 2 * tig + c] = l[nb][c];
       }
   }
   __syncthreads();
-  const float fe = E < 0 ? 0.f : kv8_power(E) * (1.0f / (1 << E4_SHIFT));
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       const int r = nb * 8 + 2 * tig + c;
-      float top = sM[r];
+      float top = sT[r];
 #pragma unroll
-      for (int w = 1; w < E4_WARPS; ++w) top = fmaxf(top, sM[w * R + r]);
-      const float f = e4_ex2(m[nb][c] - top) * fe;
+      for (int w = 1; w < E4_WARPS; ++w) top = fmaxf(top, sT[w * R + r]);
+      const float f = e4_power(t[nb][c] - top);
       float* dst = part + (warp * R + r) * LD + gid * (D / 8);
 #pragma unroll
       for (int j = 0; j < D / 16; j += 2)
@@ -615,25 +619,30 @@ attention_e4m3_rows_kernel(const T* q, int q_stride, T* __restrict__ out, const 
     }
   if (threadIdx.x < R) {
     const int r = threadIdx.x;
-    float top = sM[r], sum = 0.f;
+    float top = sM[r], high = sT[r], sum = 0.f;
 #pragma unroll
-    for (int w = 1; w < E4_WARPS; ++w) top = fmaxf(top, sM[w * R + r]);
+    for (int w = 1; w < E4_WARPS; ++w) { top = fmaxf(top, sM[w * R + r]); high = fmaxf(high, sT[w * R + r]); }
 #pragma unroll
-    for (int w = 0; w < E4_WARPS; ++w) sum += sL[w * R + r] * e4_ex2(sM[w * R + r] - top);
+    for (int w = 0; w < E4_WARPS; ++w) sum += sL[w * R + r] * e4_power(sM[w * R + r] - top);
     cM[r] = top;
+    cT[r] = high;
     cL[r] = sum;
   }
   __syncthreads();
-  auto store = [&](int r, int c, const float4& x, float sum) {
+  // high, top: the references of the weights and of the sum.  2^(high - top) as two factors, for it may lie below the normal numbers
+  auto store = [&](int r, int c, float4 x, float high, float top, float sum) {
     const int row = r0 + r;
     if (row < rows) {
       const float inv = sum == 0.f ? 0.f : 1.0f / sum;   // NaN stays NaN
+      const float by = fminf(fmaxf(high - top, -200.f), 200.f), half = floorf(by * 0.5f);
+      const float up = __uint_as_float((unsigned)(127 + (int)half - E4_SHIFT) << 23), more = __uint_as_float((unsigned)(127 + (int)(by - half)) << 23);
+      x.x *= up; x.y *= up; x.z *= up; x.w *= up;
       const int tok = row / g;
       T* dst = out + ((size_t)(qs + tok) * nq + kvh * g + row - tok * g) * D + c;
       if constexpr (sizeof(T) == 4) {
-        *(float4*)dst = make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv);
+        *(float4*)dst = make_float4(x.x * inv * more, x.y * inv * more, x.z * inv * more, x.w * inv * more);
       } else {
-        const __nv_bfloat162 lo = __floats2bfloat162_rn(x.x * inv, x.y * inv), hi = __floats2bfloat162_rn(x.z * inv, x.w * inv);
+        const __nv_bfloat162 lo = __floats2bfloat162_rn(x.x * inv * more, x.y * inv * more), hi = __floats2bfloat162_rn(x.z * inv * more, x.w * inv * more);
         *(uint2*)dst = make_uint2(*(const unsigned*)&lo, *(const unsigned*)&hi);
       }
     }
@@ -646,7 +655,7 @@ attention_e4m3_rows_kernel(const T* q, int q_stride, T* __restrict__ out, const 
       const float4 y = *(const float4*)(part + (w * R + r) * LD + c);
       x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
     }
-    if (C == 1) store(r, c, x, cL[r]);
+    if (C == 1) store(r, c, x, cT[r], cM[r], cL[r]);
     else *(float4*)(part + r * LD + c) = x;
   }
   if (C == 1) { kv8_end(known); return; }
@@ -655,16 +664,21 @@ attention_e4m3_rows_kernel(const T* q, int q_stride, T* __restrict__ out, const 
   cluster.sync();
   for (int i = (rank * 32 * E4_WARPS + threadIdx.x) * 4; i < R * D; i += C * 32 * E4_WARPS * 4) {
     const int r = i / D, at = r * LD + i - r * D;
-    float top = E4_NONE, sum = 0.f;
+    float top = E4_NONE, high = E4_NONE, sum = 0.f;
     float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int c = 0; c < C; ++c) top = fmaxf(top, cluster.map_shared_rank(cM, c)[r]);
     for (int c = 0; c < C; ++c) {
-      const float f = e4_ex2(cluster.map_shared_rank(cM, c)[r] - top);
+      const float* m_ = cluster.map_shared_rank(cM, c);              // the weights' lie R behind, the sums 2 R
+      top = fmaxf(top, m_[r]);
+      high = fmaxf(high, m_[R + r]);
+    }
+    for (int c = 0; c < C; ++c) {
+      const float* m_ = cluster.map_shared_rank(cM, c);
+      const float f = e4_power(m_[R + r] - high);
       const float4 y = *(const float4*)(cluster.map_shared_rank(part, c) + at);
       x.x = fmaf(y.x, f, x.x); x.y = fmaf(y.y, f, x.y); x.z = fmaf(y.z, f, x.z); x.w = fmaf(y.w, f, x.w);
-      sum += cluster.map_shared_rank(cL, c)[r] * f;
+      sum = fmaf(m_[2 * R + r], e4_power(m_[r] - top), sum);
     }
-    store(r, i - r * D, x, sum);
+    store(r, i - r * D, x, high, top, sum);
   }
   cluster.sync();                                    // nobody leaves while its shared memory is being read
   kv8_end(known);
@@ -677,7 +691,7 @@ static int e4_rows_launch(const void* q, int q_stride, void* out, const void* kc
                           int num_pages, int window, float scale, int known, int* err, cudaStream_t stream) {
   constexpr int R = 8 * NB;
   auto* kernel = attention_e4m3_rows_kernel<D, NB, T>;
-  const size_t stage = sizeof(float) * R * (D + 4), merge = sizeof(float) * (E4_WARPS * R * (D + 6) + 2 * R);
+  const size_t stage = sizeof(float) * R * (D + 4), merge = sizeof(float) * (E4_WARPS * R * (D + 7) + 3 * R);
   const size_t rings = stage + E4_WARPS * 2 * e4_tile_bytes<D>(), smem = rings > merge ? rings : merge;
   static SmemLimit limit;
   if (const int e = limit.allow(kernel, (int)smem)) return e;

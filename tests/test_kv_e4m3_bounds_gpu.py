@@ -1,0 +1,73 @@
+"""Attention over a cache kept in 8 bits, each sequence within the bound of the kernel that takes it and of what its own rows look at."""
+import pytest
+import torch
+
+from kv_e4m3_bounds import check
+from kv_e4m3_util import Step
+from rllm_b200.kernels import ops
+from test_kv_e4m3_gpu import SHAPES
+
+pytestmark = pytest.mark.gpu
+BF16, F32 = torch.bfloat16, torch.float32
+ROWS = [(F32, None), (BF16, "rows")]
+FORMS = ROWS + [(BF16, f) for f in ("columns", "dense")]
+
+
+def attend(st, form, monkeypatch, window=0, num_decode=None):
+    forced = form and (form, form)
+    monkeypatch.setattr(ops, "E4M3_FORMS", forced)
+    num_decode = st.num_decode if num_decode is None else num_decode
+    out = st.attend(ops, window, num_decode=num_decode)
+    assert int(st.err) == 0 and (out[sum(st.lens):] == 7).all()
+    check(st, out, window, num_decode=num_decode, forced=forced)
+    return out
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("nq,nkv,d,page,lens,starts,window", SHAPES)
+def test_steps_of_all_kinds(dtype, nq, nkv, d, page, lens, starts, window, monkeypatch):
+    attend(Step(lens, starts, nq, nkv, d, page, dtype, seed=nq + d, more_rows=2, stride_pad=16), None, monkeypatch, window)
+
+
+@pytest.mark.parametrize("dtype,form", FORMS)
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("lens,starts,window", [([1], [200], 0), ([1, 2, 7], [46, 600, 3000], 0), ([40], [60], 0), ([9, 30], [500, 90], 70)])
+@pytest.mark.parametrize("spread,qscale", [(1.0, 1.0), (3.0, 0.3)])
+def test_rows_of_like_and_of_very_different_sizes(dtype, form, d, lens, starts, window, spread, qscale, monkeypatch):
+    attend(Step(lens, starts, 8, 2, d, 16, dtype, seed=9, spread=spread, qscale=qscale), form, monkeypatch, window, 0)
+
+
+@pytest.mark.parametrize("dtype,form", FORMS)
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("gap", [8, 20, 25, 32, 45])
+def test_values_that_a_row_does_not_see_are_larger_by_far(dtype, form, d, gap, monkeypatch):
+    """Values of the portion's later tokens 2^gap times the others: the rows of the earlier ones keep all of their bits."""
+    for lens, starts in (([12], [20]), ([1, 7], [40, 300])):
+        st = Step(lens, starts, 8, 2, d, 16, dtype, seed=5, spread=0.3, qscale=0.5)
+        s = len(lens) - 1
+        for j in range(st.totals[s] - lens[s] // 2, st.totals[s]):
+            st.vs.view(torch.uint8)[int(st.table[s, j // 16]), :, j % 16] += gap
+        out = attend(st, form, monkeypatch, num_decode=0)
+        assert (out[:sum(lens) - lens[s] // 2] != 0).all()
+
+
+@pytest.mark.parametrize("dtype,form", FORMS)
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("gap", [8, 20, 25, 32, 45, 90])
+def test_values_that_have_the_weight_are_smaller_by_far(dtype, form, d, gap, monkeypatch):
+    """A few like keys that a row looks at, whose values lie 2^gap below those that weigh nothing, in one tile with them and tiles away."""
+    st = Step([1, 2], [46, 600], 8, 2, d, 16, dtype, seed=5, spread=0.3)
+    for s, keys in ((0, (1, 2, 40)), (1, (333, 5, 590))):
+        place = [(int(st.table[s, j // 16]), j % 16) for j in keys]
+        page, slot = place[0]
+        for other, at in place[1:]:                                # its neighbour, but for a number
+            for t in (st.k, st.ks):
+                t.view(torch.uint8)[other, :, at] = t.view(torch.uint8)[page, :, slot]
+            st.k.view(torch.uint8)[other, :, at, 3] = 0
+        k = (st.k[page, :, slot].float() * 2.0 ** (st.ks.view(torch.uint8)[page, :, slot].float() - 127)[:, None])
+        first, last = int(st.q_start[s]), int(st.q_start[s + 1])
+        st.q[first:last] = (k * 120 / k.square().sum(-1, keepdim=True) * d ** 0.5).repeat_interleave(4, 0).reshape(-1).to(dtype)
+        for other, at in place:
+            st.vs.view(torch.uint8)[other, :, at] -= gap
+    out = attend(st, form, monkeypatch, num_decode=0)
+    assert (out[:3] != 0).any(-1).all()
