@@ -592,9 +592,11 @@ attention_e4m3_columns_kernel(const bf16* q, int q_stride, bf16* __restrict__ ou
         add(cluster.map_shared_rank((const float*)ec_raw, c), at_ex2(m[R + r] - high));
       }
     }
-    const float inv = sum == 0.f ? 0.f : 1.0f / sum, by = at_ex2(high - top - EC_SHIFT);      // NaN stays NaN
+    // 2^(high - top) as two factors, for values near the small end of the range: as one it would be below the normal numbers, which ex2 makes 0
+    const float by = high - top - EC_SHIFT, half = floorf(0.5f * by);
+    const float inv = (sum == 0.f ? 0.f : 1.0f / sum) * at_ex2(half), more = at_ex2(by - half);      // NaN stays NaN
     const int tok = at / g;
-    const __nv_bfloat162 lo = __floats2bfloat162_rn(x.x * inv * by, x.y * inv * by), hi = __floats2bfloat162_rn(x.z * inv * by, x.w * inv * by);
+    const __nv_bfloat162 lo = __floats2bfloat162_rn(x.x * inv * more, x.y * inv * more), hi = __floats2bfloat162_rn(x.z * inv * more, x.w * inv * more);
     *(uint2*)(out + ((size_t)(qs + tok) * nq + kvh * g + at - tok * g) * D + col) = make_uint2(*(const unsigned*)&lo, *(const unsigned*)&hi);
   }
   if (C > 1) cluster.sync();                               // nobody leaves while its shared memory is being read

@@ -71,3 +71,14 @@ def test_values_that_have_the_weight_are_smaller_by_far(dtype, form, d, gap, mon
             st.vs.view(torch.uint8)[other, :, at] -= gap
     out = attend(st, form, monkeypatch, num_decode=0)
     assert (out[:3] != 0).any(-1).all()
+
+
+@pytest.mark.parametrize("dtype,form", FORMS)
+@pytest.mark.parametrize("power", [-118, -60, 60, 110])
+def test_values_near_the_ends_of_the_range(dtype, form, power, monkeypatch):
+    """All values about 2^power."""
+    for lens, starts in (([3], [100]), ([1, 20], [900, 30])):
+        st = Step(lens, starts, 8, 2, 64, 16, dtype, seed=5, spread=0.3)
+        scale = st.vs.view(torch.uint8)
+        scale.copy_((scale.int() + power).clamp(0, 247).to(torch.uint8))
+        attend(st, form, monkeypatch, num_decode=0)
