@@ -141,8 +141,9 @@ static int e4_check(const void* q, const void* out, const void* kcache, const vo
 //      keys are interleaved (prmt) into pairs along the keys.
 //   P^T: the accumulators of S^T hold (key gid, rows 2 tig, 2 tig + 1); movmatrix turns them into (keys 2 tig, 2 tig + 1, row gid).
 // Factors: a key's power of two and its row's factor multiply the score s; a value's power rides in the weight, 2^(s + ev).  A row has
-// two references, m of its scores and t of its weights with their values' powers: the denominator sums 2^(s - m) in float32, and
-// the second product takes 2^(s + ev - t + 11) as halves, so that what a row keeps of its weights does not depend on how large the
+// two references, m of its scores and t, relative to m, of its weights with their values' powers: the denominator sums 2^(s - m) in
+// float32, and the second product takes 2^((s - m) + (ev - t + 11)) as halves (in that order: s - m is exact where it matters, however
+// large scores are), so that what a row keeps of its weights does not depend on how large the
 // values are that it, or another row, does not look at (with one reference of the values' powers for all rows, a row that looked
 // at values 2^20 below the others' kept 12 bits, and at 2^32 below zeros).  Both move only when passed by 2^4, so that a tile costs
 // one vote, and the halves stay at or below 2^15; their smallest step, 2^-24, lies at 2^-35 of the row's largest weight.  References
@@ -160,11 +161,6 @@ static int e4_check(const void* q, const void* out, const void* kcache, const vo
 #define E4_SLACK 4                   // log2 of how far a score, and a weight with its value's power, may pass the row's reference
 #define E4_SHIFT 11                  // log2 of the weights' factor: E4_SLACK + E4_SHIFT = 15
 #define E4_NONE -3.0e38f             // the reference of a row that has seen nothing: 2^(s - reference) is 0 for a masked s, and any score moves it
-// 2^x of a whole x <= 0, or 0 where it is below the normal numbers'
-__device__ __forceinline__ float e4_power(float x) {
-  const int e = (int)fmaxf(x, -127.f) + 127;
-  return __uint_as_float((unsigned)e << 23);
-}
 __device__ __forceinline__ void e4_mma(float* c, const unsigned* a, unsigned b0, unsigned b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
@@ -481,33 +477,38 @@ attention_e4m3_rows_kernel(const T* q, int q_stride, T* __restrict__ out, const 
     for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const float s = sc[e >> 2][nb][e & 3];
-        need = need || s > m[nb][e & 1] + (float)E4_SLACK || s + ev[e >> 1] > t[nb][e & 1] + (float)E4_SLACK;
+        const float s = sc[e >> 2][nb][e & 3] - m[nb][e & 1];
+        need = need || s > (float)E4_SLACK || s + ev[e >> 1] > t[nb][e & 1] + (float)E4_SLACK;
       }
     if (__any_sync(0xffffffffu, need)) {
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb) {
-        float corr[2];
+        float corr[2], mx[2], tx[2];
+#pragma unroll
+        for (int c = 0; c < 2; ++c) mx[c] = fmaxf(fmaxf(sc[0][nb][c], sc[0][nb][c + 2]), fmaxf(sc[1][nb][c], sc[1][nb][c + 2]));
+#pragma unroll
+        for (int x = 4; x < 32; x <<= 1)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) mx[c] = fmaxf(mx[c], __shfl_xor_sync(0xffffffffu, mx[c], x));
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          float mx = fmaxf(fmaxf(sc[0][nb][c], sc[0][nb][c + 2]), fmaxf(sc[1][nb][c], sc[1][nb][c + 2]));
-          float tx = fmaxf(fmaxf(sc[0][nb][c] + ev[0], sc[0][nb][c + 2] + ev[1]), fmaxf(sc[1][nb][c] + ev[2], sc[1][nb][c + 2] + ev[3]));
+          mx[c] = mx[c] - m[nb][c] > (float)E4_SLACK ? ceilf(mx[c]) : m[nb][c];
+          const float down = m[nb][c] - mx[c];
+          l[nb][c] *= kv8_two_to(down);
+          t[nb][c] += down;                                // (the same place: O stays as it is)
+          m[nb][c] = mx[c];
+          tx[c] = fmaxf(fmaxf((sc[0][nb][c] - mx[c]) + ev[0], (sc[0][nb][c + 2] - mx[c]) + ev[1]),
+                        fmaxf((sc[1][nb][c] - mx[c]) + ev[2], (sc[1][nb][c + 2] - mx[c]) + ev[3]));
+        }
 #pragma unroll
-          for (int x = 4; x < 32; x <<= 1) {
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
-            tx = fmaxf(tx, __shfl_xor_sync(0xffffffffu, tx, x));
-          }
-          corr[c] = 1.0f;
-          if (mx > m[nb][c] + (float)E4_SLACK) {
-            mx = ceilf(mx);
-            l[nb][c] *= e4_power(m[nb][c] - mx);
-            m[nb][c] = mx;
-          }
-          if (tx > t[nb][c] + (float)E4_SLACK) {
-            tx = ceilf(tx);
-            corr[c] = e4_power(t[nb][c] - tx);
-            t[nb][c] = tx;
-          }
+        for (int x = 4; x < 32; x <<= 1)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) tx[c] = fmaxf(tx[c], __shfl_xor_sync(0xffffffffu, tx[c], x));
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          tx[c] = tx[c] > t[nb][c] + (float)E4_SLACK ? ceilf(tx[c]) : t[nb][c];
+          corr[c] = kv8_two_to(t[nb][c] - tx[c]);
+          t[nb][c] = tx[c];
         }
 #pragma unroll
         for (int j = 0; j < D / 16; ++j) { o[nb][j][0] *= corr[0]; o[nb][j][1] *= corr[1]; o[nb][j][2] *= corr[0]; o[nb][j][3] *= corr[1]; }
@@ -521,8 +522,9 @@ attention_e4m3_rows_kernel(const T* q, int q_stride, T* __restrict__ out, const 
         float w[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          l[nb][e & 1] += e4_ex2(sc[u][nb][e] - m[nb][e & 1]);
-          w[e] = e4_ex2(sc[u][nb][e] + (ev[2 * u + (e >> 1)] - (t[nb][e & 1] - (float)E4_SHIFT)));
+          const float s = sc[u][nb][e] - m[nb][e & 1];
+          l[nb][e & 1] += e4_ex2(s);
+          w[e] = e4_ex2(s + (ev[2 * u + (e >> 1)] - (t[nb][e & 1] - (float)E4_SHIFT)));
         }
         if (!clear) {                  // (a masked score plus a NaN is one)
 #pragma unroll
@@ -608,10 +610,10 @@ attention_e4m3_rows_kernel(const T* q, int q_stride, T* __restrict__ out, const 
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       const int r = nb * 8 + 2 * tig + c;
-      float top = sT[r];
+      float top = sM[r], high = sT[r];
 #pragma unroll
-      for (int w = 1; w < E4_WARPS; ++w) top = fmaxf(top, sT[w * R + r]);
-      const float f = e4_power(t[nb][c] - top);
+      for (int w = 1; w < E4_WARPS; ++w) kv8_join(top, high, sM[w * R + r], sT[w * R + r]);
+      const float f = kv8_two_to(t[nb][c] + (m[nb][c] - top) - high);
       float* dst = part + (warp * R + r) * LD + gid * (D / 8);
 #pragma unroll
       for (int j = 0; j < D / 16; j += 2)
@@ -621,20 +623,20 @@ attention_e4m3_rows_kernel(const T* q, int q_stride, T* __restrict__ out, const 
     const int r = threadIdx.x;
     float top = sM[r], high = sT[r], sum = 0.f;
 #pragma unroll
-    for (int w = 1; w < E4_WARPS; ++w) { top = fmaxf(top, sM[w * R + r]); high = fmaxf(high, sT[w * R + r]); }
+    for (int w = 1; w < E4_WARPS; ++w) kv8_join(top, high, sM[w * R + r], sT[w * R + r]);
 #pragma unroll
-    for (int w = 0; w < E4_WARPS; ++w) sum += sL[w * R + r] * e4_power(sM[w * R + r] - top);
+    for (int w = 0; w < E4_WARPS; ++w) sum += sL[w * R + r] * kv8_two_to(sM[w * R + r] - top);
     cM[r] = top;
     cT[r] = high;
     cL[r] = sum;
   }
   __syncthreads();
-  // high, top: the references of the weights and of the sum.  2^(high - top) as two factors, for it may lie below the normal numbers
-  auto store = [&](int r, int c, float4 x, float high, float top, float sum) {
+  // high: the weights' reference relative to the sum's.  2^high as two factors, for it may lie below the normal numbers
+  auto store = [&](int r, int c, float4 x, float high, float sum) {
     const int row = r0 + r;
     if (row < rows) {
       const float inv = sum == 0.f ? 0.f : 1.0f / sum;   // NaN stays NaN
-      const float by = fminf(fmaxf(high - top, -200.f), 200.f), half = floorf(by * 0.5f);
+      const float by = fminf(fmaxf(high, -200.f), 200.f), half = floorf(by * 0.5f);
       const float up = __uint_as_float((unsigned)(127 + (int)half - E4_SHIFT) << 23), more = __uint_as_float((unsigned)(127 + (int)(by - half)) << 23);
       x.x *= up; x.y *= up; x.z *= up; x.w *= up;
       const int tok = row / g;
@@ -655,7 +657,7 @@ attention_e4m3_rows_kernel(const T* q, int q_stride, T* __restrict__ out, const 
       const float4 y = *(const float4*)(part + (w * R + r) * LD + c);
       x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
     }
-    if (C == 1) store(r, c, x, cT[r], cM[r], cL[r]);
+    if (C == 1) store(r, c, x, cT[r], cL[r]);
     else *(float4*)(part + r * LD + c) = x;
   }
   if (C == 1) { kv8_end(known); return; }
@@ -664,21 +666,20 @@ attention_e4m3_rows_kernel(const T* q, int q_stride, T* __restrict__ out, const 
   cluster.sync();
   for (int i = (rank * 32 * E4_WARPS + threadIdx.x) * 4; i < R * D; i += C * 32 * E4_WARPS * 4) {
     const int r = i / D, at = r * LD + i - r * D;
-    float top = E4_NONE, high = E4_NONE, sum = 0.f;
+    float top = E4_NONE, high = -INFINITY, sum = 0.f;
     float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int c = 0; c < C; ++c) {
-      const float* m_ = cluster.map_shared_rank(cM, c);              // the weights' lie R behind, the sums 2 R
-      top = fmaxf(top, m_[r]);
-      high = fmaxf(high, m_[R + r]);
+      const float* m_ = cluster.map_shared_rank(cM, c);              // the weights' references lie R behind, the sums 2 R
+      kv8_join(top, high, m_[r], m_[R + r]);
     }
     for (int c = 0; c < C; ++c) {
       const float* m_ = cluster.map_shared_rank(cM, c);
-      const float f = e4_power(m_[R + r] - high);
+      const float f = kv8_two_to(m_[R + r] + (m_[r] - top) - high);
       const float4 y = *(const float4*)(cluster.map_shared_rank(part, c) + at);
       x.x = fmaf(y.x, f, x.x); x.y = fmaf(y.y, f, x.y); x.z = fmaf(y.z, f, x.z); x.w = fmaf(y.w, f, x.w);
-      sum = fmaf(m_[2 * R + r], e4_power(m_[r] - top), sum);
+      sum = fmaf(m_[2 * R + r], kv8_two_to(m_[r] - top), sum);
     }
-    store(r, i - r * D, x, high, top, sum);
+    store(r, i - r * D, x, high, sum);
   }
   cluster.sync();                                    // nobody leaves while its shared memory is being read
   kv8_end(known);

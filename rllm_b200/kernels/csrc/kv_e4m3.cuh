@@ -59,6 +59,17 @@ __device__ __forceinline__ float kv8_power(int byte) {
   const unsigned bits = byte == 0 ? 0x00400000u : (byte == KV8_NAN_SCALE ? 0x7FC00000u : (unsigned)byte << 23);
   return __uint_as_float(bits);
 }
+// 2^x of a whole x of up to 127; 0 where it is below the normal numbers'
+__device__ __forceinline__ float kv8_two_to(float x) {
+  return __uint_as_float((unsigned)((int)fminf(fmaxf(x, -127.f), 127.f) + 127) << 23);
+}
+// A row's two references, top of its scores and high, relative to top, of its weights with their values' powers, joined with those of another
+// part of its keys
+__device__ __forceinline__ void kv8_join(float& top, float& high, float m, float t) {
+  const float both = fmaxf(top, m);
+  high = fmaxf(high + (top - both), t + (m - both));
+  top = both;
+}
 // two numbers as e4m3, the first in the low byte
 __device__ __forceinline__ unsigned kv8_pack2(float a, float b) {
   return (unsigned)__nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);

@@ -82,3 +82,44 @@ def test_values_near_the_ends_of_the_range(dtype, form, power, monkeypatch):
         scale = st.vs.view(torch.uint8)
         scale.copy_((scale.int() + power).clamp(0, 247).to(torch.uint8))
         attend(st, form, monkeypatch, num_decode=0)
+
+
+@pytest.mark.parametrize("dtype,form", ROWS)
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("size", [200.0, 2.0 ** 14, 2.0 ** 20, 2.0 ** 26, 2.0 ** 32, 2.0 ** 62])
+@pytest.mark.parametrize("lens,starts", [([1], [700]), ([2, 20], [900, 700])])
+def test_keys_that_are_alike_weigh_the_same_however_large_scores_are(dtype, form, d, size, lens, starts, monkeypatch):
+    """Five like keys, tiles apart, whose scores of ``size`` leave all others behind: the result is their values' mean.  Like scores are
+    rounded alike, so what large ones lose does not count: a weight is off by its rounding, two exponentials and their arguments of up to
+    2^6 (2 (2^-22 + 2^6 2^-24)), and the sums by n 2^-24."""
+    st = Step(lens, starts, 8, 2, d, 16, dtype, seed=12, spread=0.1)
+    for s in range(len(lens)):
+        place = [(int(st.table[s, j // 16]), j % 16) for j in (3, 130, 333, 400, 690)]
+        page, slot = place[0]
+        for i, (other, at) in enumerate(place):
+            for t in (st.k, st.ks):
+                t.view(torch.uint8)[other, :, at] = t.view(torch.uint8)[page, :, slot]
+            st.vs.view(torch.uint8)[other, :, at] += (0, 3, 7, 1, 10)[i]
+        k = (st.k[page, :, slot].float() * 2.0 ** (st.ks.view(torch.uint8)[page, :, slot].float() - 127)[:, None])
+        first, last = int(st.q_start[s]), int(st.q_start[s + 1])
+        st.q[first:last] = (k * size / k.square().sum(-1, keepdim=True) * d ** 0.5).repeat_interleave(4, 0).reshape(-1).to(dtype)
+    forced = form and (form, form)
+    monkeypatch.setattr(ops, "E4M3_FORMS", forced)
+    out = st.attend(ops, num_decode=0)
+    assert int(st.err) == 0
+    at = 0
+    for s, n in enumerate(lens):
+        v, _ = st.rows_of(s, st.v, st.vs)
+        k, _ = st.rows_of(s, st.k, st.ks)
+        q = st.q[at:at + n].double().view(n, 2, 4, d)
+        scores = torch.einsum("nghd,gkd->nghk", q, k) * d ** -0.5
+        rest = scores.clone()
+        rest[..., [3, 130, 333, 400, 690]] = float("-inf")
+        assert (scores[..., 3] - rest.amax(-1) > 0.3 * size).all()
+        mean = v[:, [3, 130, 333, 400, 690]].mean(1)[None, :, None]
+        size_of = v[:, [3, 130, 333, 400, 690]].abs().mean(1)[None, :, None]
+        rel = {"dense": 2.0 ** -8 + 4e-5, None: 2.0 ** -22}.get(form, 2.0 ** -11) + 2 * (2.0 ** -22 + 64 * 2.0 ** -24) + st.totals[s] * 2.0 ** -24
+        bound = rel * size_of + torch.finfo(dtype).eps / 2 * mean.abs()
+        got = out[at:at + n].double().view(n, 2, 4, d)
+        assert ((got - mean).abs() <= bound).all(), float(((got - mean).abs() / bound).max())
+        at += n
