@@ -39,6 +39,8 @@
 #define EC_SHIFT 2.0f                // log2 of the weights' factor: a weight stays at or below 2^8
 #define EC_SCORES 34.0f              // a score may pass its reference by 2^40: it is only for the sum of the weights, which is float32
 #define EC_NONE -3.0e38f             // the reference of a row that has seen nothing
+// References are whole numbers, the weights' relative to the scores': s - m is exact where it matters, however large scores are, and so is
+// what a reference's move multiplies by.
 
 template <int D, int NB, bool MANY> struct EcShape {
   static constexpr int R = 8 * NB, QN = 16 * NB;                       // rows; columns of S
@@ -53,7 +55,7 @@ template <int D, int NB, bool MANY> struct EcShape {
   static constexpr int TILE = 128 * 128, P_BYTES = ON * 128, SLOT = 2 * TN;                  // SLOT: a tile's scales
   static constexpr int COLUMNS = 2 * QN * PAR + ON;
   static constexpr int TMEM = COLUMNS <= 64 ? 64 : COLUMNS <= 128 ? 128 : COLUMNS <= 256 ? 256 : 512;
-  static constexpr int SMEM = 2 * STAGES * TILE + QN * D + 2 * P_BYTES + 2 * STAGES * SLOT + 448 + R * (16 + 8 + 8 + 32 + 16);
+  static constexpr int SMEM = 2 * STAGES * TILE + QN * D + 2 * P_BYTES + 2 * STAGES * SLOT + 448 + R * (12 + 8 + 8 + 32 + 16);
   static_assert(CTAS * (SMEM + 1024) <= 228 * 1024 && SMEM <= 227 * 1024, "so many CTAs have room on an SM");
   static_assert(PAR * R * D * 4 <= 2 * STAGES * TILE, "the parts lie where keys and values were");
 };
@@ -164,9 +166,9 @@ attention_e4m3_columns_kernel(const bf16* q, int q_stride, bf16* __restrict__ ou
   unsigned long long *s_full = bars + 32, *p_full = bars + 34, *pv_full = bars + 36, *q_full = bars + 38;  // [2] each, q_full one
   unsigned* tmem_slot = (unsigned*)(bars + 39);
   unsigned* held = (unsigned*)(bars + 40);                 // [2 NS]: a bit for every 16 keys that were brought
-  // every eight rows' factors f, and, negative, their scores' references m, their weights' t, and m + EC_SCORES: [NB][4][8]
+  // every eight rows' factors f, and, negative, their scores' references m and, relative to m, their weights' t: [NB][3][8]
   float* info = (float*)((unsigned char*)bars + 448);
-  float2* moved = (float2*)(info + 4 * R);                     // [R]: what the row's sum and its output are multiplied by
+  float2* moved = (float2*)(info + 3 * R);                     // [R]: what the row's sum and its output are multiplied by
   int2* sight = (int2*)(moved + R);                        // [R]: the first key it sees, and the one behind its last
   float2* tops = (float2*)(sight + R);                     // [4][R]: the warps' largest score and weight; at the end their sums
   float* cM = (float*)(tops + 4 * R);                      // [3][R]: the CTA's references and sum
@@ -195,7 +197,7 @@ attention_e4m3_columns_kernel(const bf16* q, int q_stride, bf16* __restrict__ ou
     const int group = warp >> 2, quarter = warp & 3, line = tid & 127;
     typedef unsigned long long pair;                       // two rows' numbers, for instructions that take two
     pair l[4] = {0ull, 0ull, 0ull, 0ull};
-    auto notes = [&](int what, pair (&x)[4]) {             // 0: f, 1: -m, 2: -t, 3: -(m + EC_SCORES)
+    auto notes = [&](int what, pair (&x)[4]) {             // 0: f, 1: -m, 2: -t
       *(ulonglong2*)&x[0] = *(const ulonglong2*)(info + what * 8);
       *(ulonglong2*)&x[2] = *(const ulonglong2*)(info + what * 8 + 4);
     };
@@ -249,9 +251,9 @@ attention_e4m3_columns_kernel(const bf16* q, int q_stride, bf16* __restrict__ ou
           *(uint4*)(sQ + col * D + ((D == 128 ? c ^ (col & 7) : c ^ (col >> 1 & 3)) << 4)) = make_uint4(w[term][0], w[term][1], w[term][2], w[term][3]);
         }
         if (c == 0) {
-          float* note = info + (r >> 3) * 32 + (r & 7);
+          float* note = info + (r >> 3) * 24 + (r & 7);
           note[0] = __uint_as_float((unsigned)(127 - 7 + e) << 23) * scale_log2 + odd;
-          note[8] = note[16] = note[24] = -EC_NONE;
+          note[8] = note[16] = -EC_NONE;
           const int hi = pos0 + min(at, rows - 1) / g + 1;
           sight[r] = make_int2(window > 0 ? hi - window : 0, hi);
         }
@@ -262,7 +264,7 @@ attention_e4m3_columns_kernel(const bf16* q, int q_stride, bf16* __restrict__ ou
     if (lane == 0) mbar_arrive(q_full);
     asm volatile("bar.sync 5, %0;" ::"n"(128 * NB) : "memory");         // (the rows' notes, of all warps)
 
-    info += group * 32; moved += group * 8; sight += group * 8; tops += group * 32;
+    info += group * 24; moved += group * 8; sight += group * 8; tops += group * 32;
     const unsigned lane_sel = (unsigned)(quarter * 32) << 16;
     // this thread's half of O: even or odd keys' sums, and its rows' columns
     const unsigned my_o = tmem_o + lane_sel + (PAR == 2 ? (quarter >> 1) * X::PN : 0) + group * 32;
@@ -319,46 +321,59 @@ attention_e4m3_columns_kernel(const bf16* q, int q_stride, bf16* __restrict__ ou
       }
       float over = EC_NONE, over2 = EC_NONE;               // how far a score or a weight passes its reference
       {
-        pair t[4], lim[4];
+        pair m[4], t[4];
+        notes(1, m);
         notes(2, t);
-        notes(3, lim);
 #pragma unroll
         for (int u = 0; u < PAR; ++u)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             float a, b, c, d;
-            at_unpack2(at_add2(sc[u][i], lim[i]), a, b);
-            at_unpack2(at_add2(sc[u][i], at_add2(ev[u], t[i])), c, d);
+            const pair s = at_add2(sc[u][i], m[i]);
+            at_unpack2(s, a, b);
+            at_unpack2(at_add2(s, at_add2(ev[u], t[i])), c, d);
             over = at_max3(over, a, b);
             over2 = at_max3(over2, c, d);
           }
       }
-      if (ec_any(group, fmaxf(over, over2) > EC_SLACK)) {
-        float top[8], wt[8];
+      if (ec_any(group, fmaxf(over - EC_SCORES, over2) > EC_SLACK)) {
+        // the rows' largest of `what(keys of a line, pair of rows)` among the keys of all four warps
+        auto largest = [&](auto what, bool second) {
+          float top[8];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          at_unpack2(sc[0][i], top[2 * i], top[2 * i + 1]);
-          at_unpack2(at_add2(sc[0][i], ev[0]), wt[2 * i], wt[2 * i + 1]);
-          if (PAR == 2) {
-            float a, b, c, d;
-            at_unpack2(sc[PAR - 1][i], a, b);
-            at_unpack2(at_add2(sc[PAR - 1][i], ev[PAR - 1]), c, d);
-            top[2 * i] = fmaxf(top[2 * i], a); top[2 * i + 1] = fmaxf(top[2 * i + 1], b);
-            wt[2 * i] = fmaxf(wt[2 * i], c); wt[2 * i + 1] = fmaxf(wt[2 * i + 1], d);
+          for (int i = 0; i < 4; ++i) {
+            at_unpack2(what(0, i), top[2 * i], top[2 * i + 1]);
+            if (PAR == 2) {
+              float a, b;
+              at_unpack2(what(PAR - 1, i), a, b);
+              top[2 * i] = fmaxf(top[2 * i], a); top[2 * i + 1] = fmaxf(top[2 * i + 1], b);
+            }
           }
-        }
-        int at;
-        const float a = ec_fold<true>(top, lane, &at), b = ec_fold<true>(wt, lane, &at);
-        if (lane < 8) tops[quarter * 8 + at] = make_float2(a, b);
-        ec_sync(group);
-        if (line < 8) {
-          float2 t = tops[line];
+          int at;
+          const float x = ec_fold<true>(top, lane, &at);
+          if (lane < 8) (second ? tops[quarter * 8 + at].y : tops[quarter * 8 + at].x) = x;
+          ec_sync(group);
+          float t = EC_NONE;
+          if (line < 8)
 #pragma unroll
-          for (int w = 1; w < 4; ++w) { t.x = fmaxf(t.x, tops[w * 8 + line].x); t.y = fmaxf(t.y, tops[w * 8 + line].y); }
-          float2 by = make_float2(1.f, 1.f);
-          float* note = info + line;
-          if (t.x + note[24] > EC_SLACK) { by.x = at_ex2(-note[8] - t.x); note[8] = -t.x; note[24] = -(t.x + EC_SCORES); }
-          if (t.y + note[16] > EC_SLACK) { by.y = at_ex2(-note[16] - t.y); note[16] = -t.y; }
+            for (int w = 0; w < 4; ++w) t = fmaxf(t, second ? tops[w * 8 + line].y : tops[w * 8 + line].x);
+          return t;
+        };
+        float t = largest([&](int u, int i) { return sc[u][i]; }, false);
+        float2 by = make_float2(1.f, 1.f);
+        float* note = info + (line & 7);
+        if (line < 8 && t + note[8] - EC_SCORES > EC_SLACK) {
+          const float down = -note[8] - ceilf(t);
+          by.x = at_ex2(down);
+          note[8] = -ceilf(t);
+          note[16] -= down;                                // (the same place: the output stays as it is)
+        }
+        ec_sync(group);
+        pair m[4];
+        notes(1, m);
+        t = largest([&](int u, int i) { return at_add2(at_add2(sc[u][i], m[i]), ev[u]); }, true);
+        if (line < 8) {
+          if (t + note[16] > EC_SLACK) { by.y = at_ex2(-note[16] - ceilf(t)); note[16] = -ceilf(t); }
           moved[line] = by;
         }
         ec_sync(group);
@@ -390,8 +405,9 @@ attention_e4m3_columns_kernel(const bf16* q, int q_stride, bf16* __restrict__ ou
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           float a, b, c, d;
-          at_unpack2(at_add2(sc[u][i], m[i]), a, b);
-          at_unpack2(at_add2(sc[u][i], at_add2(up, t_[i])), c, d);
+          const pair s = at_add2(sc[u][i], m[i]);
+          at_unpack2(s, a, b);
+          at_unpack2(at_add2(s, at_add2(up, t_[i])), c, d);
           l[i] = at_add2(l[i], at_pack2(at_ex2(a), at_ex2(b)));
           __half2 h = __floats2half2_rn(at_ex2(c), at_ex2(d));
 #pragma unroll
@@ -566,7 +582,7 @@ attention_e4m3_columns_kernel(const bf16* q, int q_stride, bf16* __restrict__ ou
   for (int i = (rank * X::THREADS + tid) * 4; i < R * D; i += C * X::THREADS * 4) {
     const int r = i / D, col = i - r * D, at = r0 + r;
     if (at >= rows) break;
-    float top = EC_NONE, high = EC_NONE, sum = 0.f;
+    float top = EC_NONE, high = -INFINITY, sum = 0.f;      // the references of the sum and, relative to it, of the weights
     float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
     auto add = [&](const float* part, float by) {
 #pragma unroll
@@ -576,24 +592,22 @@ attention_e4m3_columns_kernel(const bf16* q, int q_stride, bf16* __restrict__ ou
       }
     };
     if (C == 1) {
-      top = cM[r];
       high = cM[R + r];
       sum = cM[2 * R + r];
       add((const float*)ec_raw, 1.f);
     } else {
       for (int c = 0; c < C; ++c) {
         const float* m = cluster.map_shared_rank(cM, c);
-        top = fmaxf(top, m[r]);
-        high = fmaxf(high, m[R + r]);
+        kv8_join(top, high, m[r], m[R + r]);
       }
       for (int c = 0; c < C; ++c) {
         const float* m = cluster.map_shared_rank(cM, c);
         sum = fmaf(m[2 * R + r], at_ex2(m[r] - top), sum);
-        add(cluster.map_shared_rank((const float*)ec_raw, c), at_ex2(m[R + r] - high));
+        add(cluster.map_shared_rank((const float*)ec_raw, c), at_ex2(m[R + r] + (m[r] - top) - high));
       }
     }
-    // 2^(high - top) as two factors, for values near the small end of the range: as one it would be below the normal numbers, which ex2 makes 0
-    const float by = high - top - EC_SHIFT, half = floorf(0.5f * by);
+    // 2^high as two factors, for values near the small end of the range: as one it would be below the normal numbers, which ex2 makes 0
+    const float by = high - EC_SHIFT, half = floorf(0.5f * by);
     const float inv = (sum == 0.f ? 0.f : 1.0f / sum) * at_ex2(half), more = at_ex2(by - half);      // NaN stays NaN
     const int tok = at / g;
     const __nv_bfloat162 lo = __floats2bfloat162_rn(x.x * inv * more, x.y * inv * more), hi = __floats2bfloat162_rn(x.z * inv * more, x.w * inv * more);
