@@ -416,7 +416,13 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
       }
       const float m_safe = (m_ref == -INFINITY) ? 0.f : m_ref;
       unsigned pk[HC / 2];
-      const unsigned long long scale2 = at_pack2(sl2, sl2), shift2 = at_pack2(-m_safe, -m_safe);
+      float times = sl2;
+      if (DENSE && __any_sync(0xffffffffu, fabsf(m_safe) > 65536.f)) {      // so large that an unrounded product passes its rounded maximum
+#pragma unroll
+        for (int j = 0; j < HC; ++j) sc[j] *= sl2;
+        times = 1.0f;
+      }
+      const unsigned long long scale2 = at_pack2(times, times), shift2 = at_pack2(-m_safe, -m_safe);
       unsigned long long sum01 = at_pack2(0.f, 0.f), sum23 = sum01;
 #pragma unroll
       for (int j = 0; j < HC; j += 4) {

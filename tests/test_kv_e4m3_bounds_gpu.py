@@ -84,7 +84,7 @@ def test_values_near_the_ends_of_the_range(dtype, form, power, monkeypatch):
         attend(st, form, monkeypatch, num_decode=0)
 
 
-@pytest.mark.parametrize("dtype,form", ROWS + [(BF16, "columns")])
+@pytest.mark.parametrize("dtype,form", FORMS)
 @pytest.mark.parametrize("d", [64, 128])
 @pytest.mark.parametrize("size", [200.0, 2.0 ** 14, 2.0 ** 20, 2.0 ** 26, 2.0 ** 32, 2.0 ** 62])
 @pytest.mark.parametrize("lens,starts", [([1], [700]), ([2, 20], [900, 700])])
