@@ -14,11 +14,14 @@
 //   warp 8      allocates TMEM and issues the products: S = Q K^T (128 x 64 x D), O += P V (128 x D x 64, P in TMEM, V as the
 //               MN-major operand, straight from its rows).
 // Halves, not bfloat16: e4m3 numbers become halves in one instruction a pair, and a weight keeps 11 bits.  Powers of two:
-//   K  a row's numbers are multiplied by 2^(ek - EK + 6), EK the largest ek of the tile, and the tile's scores by 2^(EK - 6): exact for
-//      powers down to 2^-21 of the tile's largest, to a step of 2^-30 of that below;
-//   V  by 2^(ev - EV' + 6), EV' the tile's largest, but at least 2^-30 of a running reference that moves when passed by 2^4, and the
-//      tile's weights by 2^(EV' - reference), which rides in the exponent's argument; 2^7 more, as in the mma.sync kernel;
+//   K  a row's numbers are multiplied by 2^(ek - EK + 6), EK the largest ek of the tile, and the tile's scores by 2^(EK - 6);
+//   V  by 2^(ev - EV + 6), EV the tile's largest, and a weight by 2^EV over a reference of the row's weights with their values' powers,
+//      beside that of its scores, as in the mma.sync kernel (both whole numbers, passed by 2^4 at most; 2^11 more, so that the halves'
+//      smallest step lies at 2^-35 of the row's largest weight): the factor rides in the exponent's argument, and the sum is divided by it;
 //   Q  a row by a power of two of its own, exact for bfloat16 down to 2^-27 of the row's largest.
+// A factor 2^(e - E + 6) is a half's normal number, and times an e4m3 number exact, down to e = E - 20.  A tile with rows further apart
+// than that ("wide": none in what a model makes) is taken key by key: what a factor lacks multiplies the key's scores, and stands in its
+// weights' exponents.  So are rows whose scores are so large that a sum of them and a value's power would be rounded to whole powers.
 // A token whose key or value is NaN has a NaN key and zeros for a value: rows that see it become NaN by the score, and the others'
 // products stay clean.
 #include "attention_tcgen05.cuh"
@@ -30,8 +33,11 @@
 #define E8_THREADS 320
 #define E8_AHEAD 8                   // tiles whose rows and factors are known at a time
 #define E8_SLACK 4.0f
-#define E8_SHIFT 7
-#define E8_LIFT 6                    // log2 of what keys and values are multiplied by beside: 448 2^6 is a half, and so is the factor 2^(6 - 30)
+#define E8_SHIFT 11                  // log2 of the weights' factor: E8_SLACK + E8_SHIFT = 15
+#define E8_LIFT 6                    // log2 of what keys and values are multiplied by beside: 448 2^6 is a half
+#define E8_APART 20                  // log2 of how far a tile's rows may lie apart for factors that are halves
+#define E8_NONE -3.0e38f             // the reference of a row that has seen nothing
+#define E8_LARGE 1048576.f           // whole numbers of this size and of a few hundred more have room in a float32
 
 // Q, the widened stages of K and of V (two each for heads of 64, one for 128: two CTAs fit one SM), two tiles of K and of V as
 // they come, barriers and the tiles' notes
@@ -42,13 +48,92 @@ template <int D> constexpr int e8_smem_bytes() { return E8_BM * D * 2 + 2 * e8_s
 struct E8Tile {
   int row[E8_BN];                    // a key's cache row; -1: not to be read, or of a page that is not held
   unsigned kf[E8_BN], vf[E8_BN];     // 2^(ek - EK) and 2^(ev - EV') as pairs of halves
-  int ek;                            // EK, a scale byte
-  int shift;                         // EV' - reference
-  int ref;                           // the reference, a scale byte
-  int drop;                          // the one before - it (0: it has not moved, or there was none)
+  int ek, ev;                        // EK and EV, scale bytes
+  int wide;                          // rows lie further apart than E8_APART
   unsigned missing[2];               // a bit a key whose page is not held
+  unsigned char kd[E8_BN], vd[E8_BN];      // of a wide one: EK - ek and EV - ev beyond E8_APART
 };
 static_assert(sizeof(E8Tile) <= 1024, "they lie behind the barriers");
+
+// A row's references: x of its scores; y of its weights with their values' powers, relative to x; z the sum of 2^(score - x).
+// They move to what is passed by more than 2^4; a weights' reference that moves changes the output so far, by what is returned.
+__device__ __forceinline__ void e8_move_scores(float4& ref, float top) {
+  if (top - ref.x > E8_SLACK) {
+    top = ceilf(top);
+    ref.z *= kv8_two_to(ref.x - top);                      // from nothing: 0, and nothing has been summed yet
+    ref.y += ref.x - top;                                  // (the same place: the output stays as it is)
+    ref.x = top;
+  }
+}
+__device__ __forceinline__ float e8_move_weights(float4& ref, float top) {
+  if (!(top > ref.y + E8_SLACK)) return 1.0f;
+  top = ceilf(top);
+  const float corr = kv8_two_to(ref.y - top);
+  ref.y = top;
+  return corr;
+}
+
+// A row's part of a tile key by key: the scores t_s of 64 keys, times f and what each key's factor lacks, become weights in their place
+// (a function of its own, for the registers and the instructions of the tiles that need none of it: in place they cost 15 %).
+// lacks: a wide tile's kd and vd, else null.  Returns the references, w: as e8_move_weights.
+__device__ __noinline__ float4 e8_key_by_key(unsigned t_s, const unsigned char* lacks, float f, float ev, unsigned lo_rel, unsigned span,
+                                             unsigned missing0, unsigned missing1, float4 ref) {
+  float sc[32];
+  auto lacks_key = [&](int j) { return lacks ? kv8_two_to(fmaxf(-(float)lacks[j], -126.f)) : 1.0f; };
+  auto value_power = [&](int j) { return lacks ? ev - (float)lacks[E8_BN + j] : ev; };
+  auto load = [&](int h) {
+    tmem_ld32(t_s + h * 32, (unsigned*)sc);
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int j = 0; j < 32; ++j) {
+      const bool seen = (unsigned)(h * 32 + j) - lo_rel < span && !((h ? missing1 : missing0) >> j & 1u);
+      sc[j] = seen ? sc[j] * f * lacks_key(h * 32 + j) : -INFINITY;
+    }
+  };
+  float top = -INFINITY;
+#pragma unroll 1
+  for (int h = 0; h < 2; ++h) {
+    load(h);
+#pragma unroll
+    for (int j = 0; j < 32; ++j) top = fmaxf(top, sc[j]);
+  }
+  e8_move_scores(ref, top);
+  top = -INFINITY;
+#pragma unroll 1
+  for (int h = 0; h < 2; ++h) {
+    load(h);
+#pragma unroll
+    for (int j = 0; j < 32; ++j) top = fmaxf(top, (sc[j] - ref.x) + value_power(h * 32 + j));
+  }
+  ref.w = e8_move_weights(ref, top);
+  const float base = ref.y - (float)E8_SHIFT;
+#pragma unroll 1
+  for (int h = 0; h < 2; ++h) {
+    load(h);
+    unsigned pk[16];
+#pragma unroll
+    for (int j = 0; j < 32; j += 2) {
+      float w[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float x = sc[j + e] - ref.x;
+        ref.z += at_ex2(x);
+        w[e] = at_ex2(x + (value_power(h * 32 + j + e) - base));
+      }
+      const __half2 y = __floats2half2_rn(w[0], w[1]);
+      pk[j / 2] = *(const unsigned*)&y;
+    }
+    tmem_st16(t_s + h * 16, pk);
+  }
+  return ref;
+}
+
+// 2^high without the factors of weights and values, as two: it may lie below the normal numbers
+__device__ __forceinline__ float e8_factors(float high, float* more) {
+  const float by = fminf(fmaxf(high, -200.f), 200.f), half = floorf(by * 0.5f);
+  *more = kv8_two_to(by - half);
+  return kv8_two_to(half - (float)(E8_SHIFT + E8_LIFT));
+}
 
 template <int D>
 __global__ void __launch_bounds__(E8_THREADS, 2)
@@ -149,8 +234,7 @@ attention_e4m3_tcgen05_kernel(const bf16* q, int q_stride, bf16* __restrict__ ou
   kv8_let_in(known);                                         // behind the allocation: see pdl_launch
   const unsigned tmem_s = __shfl_sync(0xffffffffu, *tmem_slot, 0), tmem_o = tmem_s + 2 * E8_BN;      // two tiles' scores: 128 + D <= 256 columns
 
-  float m_ref = -INFINITY, l = 0.f;
-  int ref = -1000;                                         // the reference of the values' powers, a scale byte
+  float4 ref = make_float4(E8_NONE, E8_NONE, 0.f, 1.f);    // see e8_move_scores
   bool ok = true;
   if (warp < 4) {
     const int r = threadIdx.x, tl = r / g;
@@ -166,14 +250,11 @@ attention_e4m3_tcgen05_kernel(const bf16* q, int q_stride, bf16* __restrict__ ou
       ok = __all_sync(0xffffffffu, mbar_wait(&s_full[it & 1], (it >> 1) & 1, err));
       if (!ok) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      struct { int ek, shift, ref, drop; unsigned missing[2]; } note;
-      {
-        const E8Tile& x = tiles[it % E8_AHEAD];
-        note = {x.ek, x.shift, x.ref, x.drop, {x.missing[0], x.missing[1]}};
-      }
+      struct { int ek, ev, wide; unsigned missing[2]; } note;
+      const E8Tile& tile = tiles[it % E8_AHEAD];
+      note = {tile.ek, tile.ev, tile.wide, {tile.missing[0], tile.missing[1]}};
       __syncwarp();
-      if (lane == 0) mbar_arrive(&t_free[it % E8_AHEAD]);
-      ref = note.ref;
+      if (!(warp_live && note.wide) && lane == 0) mbar_arrive(&t_free[it % E8_AHEAD]);       // (a wide one's is read to its end)
       if (!warp_live) {
         if (it > 0) {
           ok = __all_sync(0xffffffffu, mbar_wait(pv_full, (it - 1) & 1, err));
@@ -184,6 +265,7 @@ attention_e4m3_tcgen05_kernel(const bf16* q, int q_stride, bf16* __restrict__ ou
       }
       const float f = fmaxf(my_factor * kv8_power(note.ek), 1.2e-38f);     // (a masked score, -inf, times 0 would be NaN)
       const bool masked = !(j0 >= clear_lo && j0 + E8_BN <= clear_hi) || (note.missing[0] | note.missing[1]);
+      const unsigned lo_rel = (unsigned)(row_lo - j0), span = (unsigned)max(row_hi - row_lo, 0);
       // the scores come from TMEM twice, 32 at a time, for their maximum and for their exponentials: all 64 at once, and the
       // weights, would not leave registers for two CTAs an SM
       float sc[32];
@@ -191,13 +273,13 @@ attention_e4m3_tcgen05_kernel(const bf16* q, int q_stride, bf16* __restrict__ ou
         tmem_ld32(t_s + h * 32, (unsigned*)sc);
         asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
         if (masked) {
-          const unsigned lo_rel = (unsigned)(row_lo - j0 - h * 32), span = (unsigned)max(row_hi - row_lo, 0), miss = note.missing[h];
+          const unsigned lo = lo_rel - h * 32, miss = note.missing[h];
 #pragma unroll
           for (int j = 0; j < 32; ++j)
-            if (!((unsigned)j - lo_rel < span) || (miss >> j & 1u)) sc[j] = -INFINITY;
+            if (!((unsigned)j - lo < span) || (miss >> j & 1u)) sc[j] = -INFINITY;
         }
       };
-      float mx = -INFINITY;
+      float mx = -INFINITY;                                // the row's largest score
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         load(h);
@@ -210,50 +292,51 @@ attention_e4m3_tcgen05_kernel(const bf16* q, int q_stride, bf16* __restrict__ ou
         mx = at_max3(mx, mx0, mx1);
       }
       mx *= f;
-      const bool moves = mx > m_ref + E8_SLACK;
-      float corr = 1.0f;
-      if (moves) {
-        corr = at_ex2(m_ref - mx);                         // from -inf: 0, and nothing has been summed yet
-        m_ref = mx;
-        l *= corr;
-      }
-      const bool dropped = note.drop != 0;
-      if (dropped) corr *= note.drop < -126 ? 0.f : __uint_as_float((unsigned)(127 + note.drop) << 23);
-      // weights times 2^(EV' - reference + 7), in the place of the scores, and the sum without that factor
-      const float up = (float)(note.shift + E8_SHIFT), m_safe = ((m_ref == -INFINITY) ? 0.f : m_ref) - up;
-      const unsigned long long scale2 = at_pack2(f, f), shift2 = at_pack2(-m_safe, -m_safe);
-      unsigned long long sum01 = at_pack2(0.f, 0.f), sum23 = sum01;
-      unsigned pk[2][16];
+      float corr;                                          // what the output so far is multiplied by
+      const float ev = (float)(note.ev - 127), reach = fmaxf(mx, ref.x);
+      if (note.wide || __any_sync(0xffffffffu, fabsf(reach) > E8_LARGE && reach != E8_NONE)) {
+        ref = e8_key_by_key(t_s, note.wide ? tiles[it % E8_AHEAD].kd : nullptr, f, ev, lo_rel, span, note.missing[0], note.missing[1], ref);
+        corr = ref.w;
+        __syncwarp();
+        if (note.wide && lane == 0) mbar_arrive(&t_free[it % E8_AHEAD]);
+      } else {
+        e8_move_scores(ref, mx);
+        corr = e8_move_weights(ref, (mx - ref.x) + ev);
+        // weights times 2^(EV - reference + 11), in the place of the scores, and the sum without that factor.  Where it is so small that no
+        // weight is above the halves' smallest, 2^-60 of the sum's, the sum keeps its bits (-1000: of a row that has seen nothing)
+        const float by = fmaxf(fminf(ref.y - ev - (float)E8_SHIFT, 60.f), -1000.f), base = ref.x + by;
+        const unsigned long long scale2 = at_pack2(f, f), shift2 = at_pack2(-base, -base);
+        unsigned long long sum01 = at_pack2(0.f, 0.f), sum23 = sum01;
+        unsigned pk[2][16];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        load(h);
+        for (int h = 0; h < 2; ++h) {
+          load(h);
 #pragma unroll
-        for (int j = 0; j < 32; j += 4) {
-          float x0, x1, x2, x3;
-          at_unpack2(at_fma2(at_pack2(sc[j], sc[j + 1]), scale2, shift2), x0, x1);
-          at_unpack2(at_fma2(at_pack2(sc[j + 2], sc[j + 3]), scale2, shift2), x2, x3);
-          const float p0 = at_ex2(x0), p1 = at_ex2(x1), p2 = at_ex2(x2), p3 = at_ex2(x3);
-          sum01 = at_add2(sum01, at_pack2(p0, p1));
-          sum23 = at_add2(sum23, at_pack2(p2, p3));
-          const __half2 h0 = __floats2half2_rn(p0, p1), h1 = __floats2half2_rn(p2, p3);
-          pk[h][j / 2] = *(const unsigned*)&h0;
-          pk[h][j / 2 + 1] = *(const unsigned*)&h1;
+          for (int j = 0; j < 32; j += 4) {
+            float x0, x1, x2, x3;
+            at_unpack2(at_fma2(at_pack2(sc[j], sc[j + 1]), scale2, shift2), x0, x1);
+            at_unpack2(at_fma2(at_pack2(sc[j + 2], sc[j + 3]), scale2, shift2), x2, x3);
+            const float p0 = at_ex2(x0), p1 = at_ex2(x1), p2 = at_ex2(x2), p3 = at_ex2(x3);
+            sum01 = at_add2(sum01, at_pack2(p0, p1));
+            sum23 = at_add2(sum23, at_pack2(p2, p3));
+            const __half2 h0 = __floats2half2_rn(p0, p1), h1 = __floats2half2_rn(p2, p3);
+            pk[h][j / 2] = *(const unsigned*)&h0;
+            pk[h][j / 2 + 1] = *(const unsigned*)&h1;
+          }
+          if (h == 0) tmem_st16(t_s, pk[0]);               // (columns 0 .. 15: scores that have been read; the other half's lie behind)
         }
-        if (h == 0) tmem_st16(t_s, pk[0]);                 // (columns 0 .. 15: scores that have been read; the other half's lie behind)
-      }
-      tmem_st16(t_s + 16, pk[1]);
-      {
+        tmem_st16(t_s + 16, pk[1]);
         float a, b, c, d;
         at_unpack2(sum01, a, b);
         at_unpack2(sum23, c, d);
-        l = fmaf((a + b) + (c + d), at_ex2(-up), l);
+        ref.z = fmaf((a + b) + (c + d), kv8_two_to(by), ref.z);
       }
       // the product of the tile before has to be through: it wrote the output that is rescaled here
       if (it > 0) {
         ok = __all_sync(0xffffffffu, mbar_wait(pv_full, (it - 1) & 1, err));
         if (!ok) break;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        if (__any_sync(0xffffffffu, moves || dropped)) {
+        if (__any_sync(0xffffffffu, corr != 1.0f)) {
 #pragma unroll
           for (int c0 = 0; c0 < D; c0 += 32) {
             unsigned* v = (unsigned*)sc;
@@ -274,10 +357,9 @@ attention_e4m3_tcgen05_kernel(const bf16* q, int q_stride, bf16* __restrict__ ou
     if (ntiles == 0) ok = false;
     if (ok) ok = __all_sync(0xffffffffu, mbar_wait(pv_full, (ntiles - 1) & 1, err));
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    // the result, without the values' powers' reference
-    const float fe = ref < 0 ? 0.f : kv8_power(ref) * (1.0f / (1 << (E8_SHIFT + E8_LIFT)));
     if (splits == 1) {
-      const float inv = (l == 0.f ? 0.f : 1.0f / l) * fe;  // NaN stays NaN
+      float more;
+      const float inv = (ref.z == 0.f ? 0.f : 1.0f / ref.z) * e8_factors(ref.y, &more);      // NaN stays NaN
       bf16* orow = out + ((size_t)(qs + t0 + tl) * nq + kvh * g + (r - tl * g)) * D;
       if (warp_live) {
 #pragma unroll
@@ -295,7 +377,7 @@ attention_e4m3_tcgen05_kernel(const bf16* q, int q_stride, bf16* __restrict__ ou
             for (int c = 0; c < 32; c += 8) {
               float y[8];
 #pragma unroll
-              for (int e = 0; e < 8; ++e) y[e] = __uint_as_float(v[c + e]) * inv;
+              for (int e = 0; e < 8; ++e) y[e] = __uint_as_float(v[c + e]) * inv * more;
               store8(orow + c0 + c, y);
             }
           }
@@ -316,12 +398,12 @@ attention_e4m3_tcgen05_kernel(const bf16* q, int q_stride, bf16* __restrict__ ou
         }
 #pragma unroll
         for (int c = 0; c < 32; c += 4)
-          *(float4*)(mine + c0 + c) = make_float4(__uint_as_float(v[c]) * fe, __uint_as_float(v[c + 1]) * fe, __uint_as_float(v[c + 2]) * fe,
-                                                  __uint_as_float(v[c + 3]) * fe);
+          *(float4*)(mine + c0 + c) = make_float4(__uint_as_float(v[c]), __uint_as_float(v[c + 1]), __uint_as_float(v[c + 2]), __uint_as_float(v[c + 3]));
       }
       float* ml = (float*)sQ + E8_BM * (D + 4);
-      ml[r] = m_ref;
-      ml[E8_BM + r] = l;
+      ml[r] = ref.x;
+      ml[E8_BM + r] = ref.y;
+      ml[2 * E8_BM + r] = ref.z;
     }
   } else if (warp < 8) {
     // ---- widening ----
@@ -456,7 +538,7 @@ attention_e4m3_tcgen05_kernel(const bf16* q, int q_stride, bf16* __restrict__ ou
       }
     };
     auto factor = [&](int b, int top) {                    // 2^(b - top + E8_LIFT) twice, as halves
-      const __half2 p = __float2half2_rn(b - top < -30 ? 0.f : __uint_as_float((unsigned)(127 + E8_LIFT + b - top) << 23));
+      const __half2 p = __float2half2_rn(__uint_as_float((unsigned)(127 + E8_LIFT + max(b - top, -E8_APART)) << 23));
       return *(const unsigned*)&p;
     };
     rows_of(0);
@@ -464,28 +546,30 @@ attention_e4m3_tcgen05_kernel(const bf16* q, int q_stride, bf16* __restrict__ ou
       int r[2] = {row[0], row[1]}, k[2] = {kb[0], kb[1]}, v[2] = {vb[0], vb[1]};
       const unsigned ms[2] = {miss[0], miss[1]}, rd[2] = {readable[0], readable[1]};
       int kt = 0, vt = 0;
+      bool live[2];                                        // neither hidden from all nor NaN
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        if (!(rd[h] >> lane & 1u)) k[h] = v[h] = 0;
-        if (k[h] == KV8_NAN_SCALE || v[h] == KV8_NAN_SCALE) { k[h] = KV8_NAN_SCALE; v[h] = 0; }
-        else { kt = max(kt, k[h]); vt = max(vt, v[h]); }
+        const bool odd = k[h] == KV8_NAN_SCALE || v[h] == KV8_NAN_SCALE, read = rd[h] >> lane & 1u;
+        live[h] = read && !odd;
+        if (live[h]) { kt = max(kt, k[h]); vt = max(vt, v[h]); }
+        else { k[h] = read ? KV8_NAN_SCALE : 0; v[h] = 0; }
       }
       kt = __reduce_max_sync(0xffffffffu, kt);
       vt = __reduce_max_sync(0xffffffffu, vt);
+      const int kd[2] = {live[0] ? max(kt - k[0] - E8_APART, 0) : 0, live[1] ? max(kt - k[1] - E8_APART, 0) : 0};
+      const int vd[2] = {live[0] ? max(vt - v[0] - E8_APART, 0) : 0, live[1] ? max(vt - v[1] - E8_APART, 0) : 0};
+      const bool wide = __any_sync(0xffffffffu, (kd[0] | kd[1] | vd[0] | vd[1]) != 0);
       rows_of(it + 1);
-      int drop = 0;
-      if (ref < 0) ref = vt;
-      else if ((float)vt > (float)ref + E8_SLACK) { drop = ref - vt; ref = vt; }
-      const int eff = max(vt, ref - 30);
       if (!__all_sync(0xffffffffu, mbar_wait(&t_free[it % E8_AHEAD], ((it / E8_AHEAD) & 1) ^ 1, err))) break;
       E8Tile& x = tiles[it % E8_AHEAD];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         x.row[h * 32 + lane] = r[h];
         x.kf[h * 32 + lane] = k[h] == KV8_NAN_SCALE ? 0x7E007E00u : factor(k[h], kt);
-        x.vf[h * 32 + lane] = factor(v[h], eff);
+        x.vf[h * 32 + lane] = factor(v[h], vt);
+        if (wide) { x.kd[h * 32 + lane] = (unsigned char)kd[h]; x.vd[h * 32 + lane] = (unsigned char)vd[h]; }
       }
-      if (lane == 0) { x.ek = kt; x.shift = eff - ref; x.ref = ref; x.drop = drop; x.missing[0] = ms[0]; x.missing[1] = ms[1]; }
+      if (lane == 0) { x.ek = kt; x.ev = vt; x.wide = wide; x.missing[0] = ms[0]; x.missing[1] = ms[1]; }
       __syncwarp();
       if (lane == 0) mbar_arrive(&t_full[it % E8_AHEAD]);
     }
@@ -547,18 +631,21 @@ attention_e4m3_tcgen05_kernel(const bf16* q, int q_stride, bf16* __restrict__ ou
   const int first = live_rows * rank / splits, last = live_rows * (rank + 1) / splits;     // this CTA's rows
   for (int i = threadIdx.x; i < (last - first) * (D / 4); i += E8_THREADS) {
     const int row = first + i / (D / 4), c = (i % (D / 4)) * 4, tok = row / g;
-    float top = -INFINITY, sum = 0.f;
+    float top = E8_NONE, high = -INFINITY, sum = 0.f, more;
     float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int k = 0; k < splits; ++k) top = fmaxf(top, cluster.map_shared_rank(ml, k)[row]);
     for (int k = 0; k < splits; ++k) {
       const float* other = cluster.map_shared_rank(ml, k);
-      const float f = other[row] == -INFINITY ? 1.0f : at_ex2(other[row] - top);       // (with nothing seen, zeros or NaN)
+      kv8_join(top, high, other[row], other[E8_BM + row]);
+    }
+    for (int k = 0; k < splits; ++k) {                       // (a CTA that has seen nothing has zeros or NaN)
+      const float* other = cluster.map_shared_rank(ml, k);
+      const float f = kv8_two_to(other[E8_BM + row] + (other[row] - top) - high);
       const float4 y = *(const float4*)(cluster.map_shared_rank(part, k) + row * (D + 4) + c);
       x.x = fmaf(y.x, f, x.x); x.y = fmaf(y.y, f, x.y); x.z = fmaf(y.z, f, x.z); x.w = fmaf(y.w, f, x.w);
-      sum = fmaf(other[E8_BM + row], f, sum);
+      sum = fmaf(other[2 * E8_BM + row], kv8_two_to(other[row] - top), sum);
     }
-    const float inv = sum == 0.f ? 0.f : 1.0f / sum;
-    const __nv_bfloat162 lo = __floats2bfloat162_rn(x.x * inv, x.y * inv), hi = __floats2bfloat162_rn(x.z * inv, x.w * inv);
+    const float inv = (sum == 0.f ? 0.f : 1.0f / sum) * e8_factors(high, &more);
+    const __nv_bfloat162 lo = __floats2bfloat162_rn(x.x * inv * more, x.y * inv * more), hi = __floats2bfloat162_rn(x.z * inv * more, x.w * inv * more);
     *(uint2*)(out + ((size_t)(qs + t0 + tok) * nq + kvh * g + row - tok * g) * D + c) = make_uint2(*(const unsigned*)&lo, *(const unsigned*)&hi);
   }
   cluster.sync();                                          // nobody leaves while its shared memory is being read

@@ -9,8 +9,7 @@ from test_kv_e4m3_gpu import SHAPES
 
 pytestmark = pytest.mark.gpu
 BF16, F32 = torch.bfloat16, torch.float32
-ROWS = [(F32, None), (BF16, "rows")]
-FORMS = ROWS + [(BF16, f) for f in ("columns", "dense")]
+FORMS = [(F32, None)] + [(BF16, f) for f in ("rows", "columns", "tcgen05", "dense")]
 
 
 def attend(st, form, monkeypatch, window=0, num_decode=None):
@@ -82,6 +81,25 @@ def test_values_near_the_ends_of_the_range(dtype, form, power, monkeypatch):
         scale = st.vs.view(torch.uint8)
         scale.copy_((scale.int() + power).clamp(0, 247).to(torch.uint8))
         attend(st, form, monkeypatch, num_decode=0)
+
+
+@pytest.mark.parametrize("dtype,form", FORMS)
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("gap", [18, 20, 21, 30, 60])
+@pytest.mark.parametrize("lens,starts", [([12], [20]), ([1, 70], [40, 300])])
+def test_keys_that_a_row_does_not_see_are_larger_by_far(dtype, form, d, gap, lens, starts, monkeypatch):
+    """Keys of the portion's later tokens 2^gap times the others; some values too, and a row of zeros among each."""
+    st = Step(lens, starts, 8, 2, d, 16, dtype, seed=5, spread=0.3, qscale=0.5)
+    s = len(lens) - 1
+    for j in range(st.totals[s] - lens[s] // 2, st.totals[s]):
+        page, slot = int(st.table[s, j // 16]), j % 16
+        st.ks.view(torch.uint8)[page, :, slot] += gap
+        if j % 3 == 0:
+            st.vs.view(torch.uint8)[page, :, slot] += gap + 1
+    for t in (st.k, st.v, st.ks, st.vs):
+        t.view(torch.uint8)[int(st.table[s, 0]), :, 5] = 0
+    out = attend(st, form, monkeypatch, num_decode=0)
+    assert (out[:sum(lens) - lens[s] // 2] != 0).all()
 
 
 @pytest.mark.parametrize("dtype,form", FORMS)
