@@ -2,6 +2,8 @@
 
     python -m rllm_b200.kernels.microbench attention_decode --batch 8 --context 4096
     python -m rllm_b200.kernels.microbench attention_prefill --tokens 2048 [--impl tcgen05]
+    python -m rllm_b200.kernels.microbench attention_e4m3 --batch 8 --context 4095 --each 4 [--form rows]
+    python -m rllm_b200.kernels.microbench attention_e4m3 --contexts 32768,500*63      (attention_decode too)
     python -m rllm_b200.kernels.microbench gemm_small_m --rows 8 [--variant residual|rstd]
     python -m rllm_b200.kernels.microbench gemm_tcgen05 --rows 2048
     python -m rllm_b200.kernels.microbench latent_attention --tokens 2048 --heads 16 --kv-rank 512 --rot-dim 64
@@ -98,18 +100,32 @@ def _seen(p: int, window: int, keep: int, chunk: int) -> int:
     return p + 1 - lo + (min(keep, lo) if window else 0)
 
 
+def _contexts(args, page: int):
+    """Keys of every sequence (``--contexts``, else ``--batch`` times ``--context``), pages, and a table of pages in any order."""
+    lens = [int(n) for part in args.contexts.split(",") for n in [part.split("*")[0]] * int((part + "*1").split("*")[1])] \
+        if args.contexts else [args.context] * args.batch
+    need = [-(-n // page) for n in lens]
+    pages = sum(need) + 8
+    order = torch.randperm(pages - 8, device=DEV).int()
+    table = torch.full((len(lens), max(need)), -1, dtype=torch.int32, device=DEV)
+    at = 0
+    for row, n in zip(table, need):
+        row[:n] = order[at:at + n]
+        at += n
+    return lens, pages, table
+
+
 def attention_decode(args) -> None:
     nq, nkv, d, page = args.heads, args.kv_heads, args.head_dim, args.page
-    B, ctx = args.batch, args.context
-    pages = B * (ctx // page) + 8
+    lens, pages, table = _contexts(args, page)
+    B, ctx = len(lens), max(lens)
     nc = max(2, min(8, int(300e6 // (pages * nkv * page * d * 4)) + 1))
     caches = [(torch.randn(pages, nkv, page, d, device=DEV).bfloat16(),
                torch.randn(pages, nkv, page, d, device=DEV).bfloat16()) for _ in range(nc)]
-    table = torch.randperm(pages - 8, device=DEV).int().view(B, ctx // page).contiguous()
     err = torch.zeros(1, dtype=torch.int32, device=DEV)
     q = torch.randn(B, nq * d, device=DEV).bfloat16()
     out = torch.empty_like(q)
-    seq_lens = torch.full((B,), ctx, dtype=torch.int32, device=DEV)
+    seq_lens = torch.tensor(lens, dtype=torch.int32, device=DEV)
     ws = torch.empty(ops.attention_decode_workspace(B, nq, d, ctx), device=DEV)
     scale = 1 / math.sqrt(d)
 
@@ -120,9 +136,36 @@ def attention_decode(args) -> None:
         ops.attention_decode_bf16(q, nq * d, out, k, v, table, seq_lens, B, ctx, nq, nkv, d, args.window, scale, err, ws,
                                   **kw)
     us = time_graph_us(run, args.iters)
-    nbytes = B * _seen(ctx - 1, args.window, args.keep_first, args.chunk) * nkv * d * 2 * 2
-    print(f"attention_decode batch {B} context {ctx} window {args.window}{word}: {us:.1f} us, "
+    nbytes = sum(_seen(n - 1, args.window, args.keep_first, args.chunk) for n in lens) * nkv * d * 2 * 2
+    print(f"attention_decode batch {B} context {args.contexts or ctx} window {args.window}{word}: {us:.1f} us, "
           f"{nbytes / us / 1e3:.0f} GB/s of visible K and V")
+
+
+def attention_e4m3(args) -> None:
+    """Attention of ``--each`` tokens a sequence, the last of its keys, over a cache kept in 8 bits."""
+    nq, nkv, d, page, dtype = args.heads, args.kv_heads, args.head_dim, args.page, getattr(torch, args.dtype)
+    lens, pages, table = _contexts(args, page)
+    S, each = len(lens), args.each
+    ops.E4M3_FORMS = args.form and (args.form, args.form)
+    nc = max(2, min(8, int(300e6 // (pages * nkv * page * d * 2)) + 1))
+    byte = lambda lo, hi, *shape: torch.randint(lo, hi, shape, dtype=torch.uint8, device=DEV)  # noqa: E731
+    caches = [[byte(0, 120, pages, nkv, page, d).view(ops.E4M3) for _ in range(2)] +
+              [byte(118, 122, pages, nkv, page).view(ops.E8M0) for _ in range(2)] for _ in range(nc)]
+    err = torch.zeros(1, dtype=torch.int32, device=DEV)
+    q = torch.randn(S * each, nq * d, device=DEV).to(dtype)
+    out = torch.empty_like(q)
+    q_start = torch.arange(S + 1, dtype=torch.int32, device=DEV) * each
+    seq_lens = torch.tensor(lens, dtype=torch.int32, device=DEV)
+
+    def run(i):
+        ops.attention_e4m3(q, out, *caches[i % nc], table, q_start, seq_lens, S if each == 1 else 0, each, max(lens), nq, nkv, args.window,
+                           1 / math.sqrt(d), err, lengths_ready=True)
+    us = time_graph_us(run, args.iters)
+    first = [n - each for n in lens]
+    nbytes = sum(_seen(n - 1, args.window + each - 1 if args.window else 0, 0, 0) for n in lens) * nkv * (d + 1) * 2
+    flops = 4 * nq * d * sum(_seen(p, args.window, 0, 0) for n, a in zip(lens, first) for p in range(a, n))
+    print(f"attention_e4m3 {args.form or 'by the rule'} batch {S} context {args.contexts or max(lens)} each {each} window {args.window} head {d} "
+          f"{args.dtype}: {us:.1f} us, {nbytes / us / 1e3:.0f} GB/s of visible K and V, {flops / us / 1e6:.1f} TFLOP/s")
 
 
 def attention_prefill(args) -> None:
@@ -491,12 +534,17 @@ def streams(args) -> None:
 
 def main(argv=None) -> int:
     p = argparse.ArgumentParser(prog="python -m rllm_b200.kernels.microbench", description=__doc__.split("\n\n")[0])
-    p.add_argument("kernel", choices=["attention_decode", "attention_prefill", "gemm_small_m", "gemm_tcgen05",
+    p.add_argument("kernel", choices=["attention_decode", "attention_e4m3", "attention_prefill", "gemm_small_m", "gemm_tcgen05",
                                       "latent_attention", "routed_experts", "lightning_scan", "selective_scan",
                                       "streams", "mlstm_scan", "channel_delta", "channel_delta_step", "ssd_scan",
                                       "linear_state", "shared_key_attention", "talking_prep"])
     p.add_argument("--batch", type=int, default=8)
     p.add_argument("--context", type=int, default=4096)
+    p.add_argument("--contexts", default=None, help="attention_decode, attention_e4m3: keys of every sequence, n or n*times, by commas")
+    p.add_argument("--each", type=int, default=1, help="attention_e4m3: tokens that a sequence brings")
+    p.add_argument("--form", choices=["rows", "columns", "tcgen05", "dense", "simt"], default=None,
+                   help="attention_e4m3: this kernel in place of the rule's")
+    p.add_argument("--dtype", choices=["bfloat16", "float32"], default="bfloat16", help="attention_e4m3: the queries' type")
     p.add_argument("--tokens", type=int, default=2048)
     p.add_argument("--rows", type=int, default=8)
     p.add_argument("--iters", type=int, default=20)
@@ -533,7 +581,7 @@ def main(argv=None) -> int:
     if not torch.cuda.is_available():
         print("microbench needs a CUDA device", file=sys.stderr)
         return 1
-    {"attention_decode": attention_decode, "attention_prefill": attention_prefill,
+    {"attention_decode": attention_decode, "attention_e4m3": attention_e4m3, "attention_prefill": attention_prefill,
      "gemm_small_m": gemm_small_m, "gemm_tcgen05": gemm_tcgen05, "latent_attention": latent_attention,
      "routed_experts": routed_experts, "lightning_scan": lightning_scan, "selective_scan": selective_scan,
      "streams": streams, "mlstm_scan": mlstm_scan, "channel_delta": channel_delta,
