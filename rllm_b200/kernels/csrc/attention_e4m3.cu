@@ -150,9 +150,9 @@ static int e4_check(const void* q, const void* out, const void* kcache, const vo
 // are whole numbers: what they are multiplied by when they move, or when parts meet, is exact.
 // Queries are put into halves after a division by a power of two of the row's own (bfloat16: exact down to 2^-27 of the
 // row's largest; float32: two halves, 22 bits, and P likewise).
-// What bounds it: over few keys the start (780 instructions a warp beside its keys: queries, merge) and the latency of one or two
-// tiles, 4.5 us for 511 keys of 8 heads of 64; over many the instructions, 286 for 16 keys of 128 dims (4 KB), a third of them
-// conversions to halves at half the ALU's rate: 64 sequences of 8,191 keys, 8 heads of 128, 221 us, 4.9 TB/s.
+// What bounds it: over few keys the start (queries, the first references, merge) and the latency of one or two tiles, 5.9 us for 511
+// keys of 8 heads of 64; over many the instructions, about 300 for 16 keys of 128 dims (4 KB), a third of them conversions to
+// halves at half the ALU's rate: 64 sequences of 8,191 keys, 8 heads of 128, 224 us, 4.8 TB/s.
 //
 // A cluster of C CTAs of 4 warps shares one (sequence, kv head, tile of rows): key tiles go round over the warps of the
 // cluster, partial results are merged in shared memory, first the CTA's, then, each CTA a slice, the cluster's (distributed

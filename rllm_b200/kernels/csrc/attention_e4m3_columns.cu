@@ -25,10 +25,12 @@
 // two are left where they are (the tensor core has time).
 // A cluster shares the keys of a (sequence, kv head, tile of rows); parts are merged in shared memory as in attention_e4m3.cu.
 //
-// What bounds it: memory for heads of 128 (64 sequences of 8,191 keys, 8 kv heads of four rows: 157 us, 6.9 TB/s; the mma.sync kernel
-// 221).  For heads of 64 a key has half the bytes and the same work for a thread (two exponentials and nine conversions for every two
-// rows, seven of them at half and a quarter of the ALU's rate): 96 us, 5.7 TB/s (118), and 20 us for 24 rows of 8 sequences of 4,095 (29).
-// Over few keys the way to the first tile's result, 6 us, is longer than the mma.sync kernel's.
+// What bounds it: memory for heads of 128 (64 sequences of 8,191 keys, 8 kv heads of four rows: 159 us, 6.8 TB/s of reads over two caches
+// of 1.1 GB in turn; a single cold launch 6.0; the mma.sync kernel 224).  For heads of 64 a key has half the bytes and the same work for a thread (two exponentials and nine conversions for every two
+// rows, seven of them at half and a quarter of the ALU's rate): 96 us, 5.7 TB/s (120), and 18 us for 24 rows of 8 sequences of 4,095 (30).
+// Over few keys the way to the first tile's result, 6 us, is longer than the mma.sync kernel's.  Every sequence has clusters of one size,
+// which goes by the number of sequences: one long sequence among many short ones is walked by few CTAs (63 of 500 keys and one of 32,768,
+// heads of 128: 187 us, where chunks of a sequence's own length, as over the run's own type, take 89).
 #include "attention_tcgen05.cuh"
 #include "kv_e4m3.cuh"
 #include <cooperative_groups.h>

@@ -2059,8 +2059,7 @@ def softcap_rows(x: torch.Tensor, cap: float) -> torch.Tensor:
 # ---------------------------------------------------------------------------
 # a cache kept in 8 bits: pages of float8_e4m3fn [pages, nkv, page_size, d] and a power of two a row, float8_e8m0fnu
 # [pages, nkv, page_size], for keys and for values (csrc/kv_e4m3.cuh says what a row becomes)
-# Each operator's common call is checked and launched by the extension module in one go; what it turns down is checked here,
-# for the reason or for another way.
+# Each operator's call is checked and launched by the extension module in one go; what it turns down is looked at here for the reason.
 # ---------------------------------------------------------------------------
 E4M3, E8M0 = torch.float8_e4m3fn, torch.float8_e8m0fnu
 
@@ -2143,8 +2142,8 @@ def kv_read_e4m3(positions: torch.Tensor, token_seq: torch.Tensor, block_table: 
                  vcache: torch.Tensor, kscale: torch.Tensor, vscale: torch.Tensor, out_k: torch.Tensor, out_v: torch.Tensor,
                  err: torch.Tensor) -> None:
     """Keys and values of given tokens out of a cache kept in 8 bits: out_k, out_v [T, nkv d] (bfloat16 or float32) = the
-    rows of sequence ``token_seq[t]``'s token at ``positions[t]``.  Exact in float32, and in bfloat16 down to its smallest
-    numbers; NaN where a row's scale is.  A token whose page is not held sets bit 4 of ``err`` and reads as zeros."""
+    rows of sequence ``token_seq[t]``'s token at ``positions[t]``.  Exact in float32 (but that numbers of 248 2^120 and more, which
+    are kept as 2^128, are infinite), and in bfloat16 down to its smallest numbers; NaN where a row's scale is.  A token whose page is not held sets bit 4 of ``err`` and reads as zeros."""
     if _launch().e4m3_read(_entries.rllm_kv_e4m3_read, out_k, out_v, positions, token_seq, err, kcache, vcache, kscale, vscale, block_table):
         return
     dt = dtype_code(out_k.dtype)
@@ -2185,15 +2184,17 @@ def attention_e4m3_form(dtype: torch.dtype, nq: int, nkv: int, d: int, page_size
     group), "rows" (mma.sync, 8 to 32 rows), "tcgen05" (128 rows, keys and values widened inside), "dense" (tcgen05 over keys and
     values widened once for all tiles of rows), "simt".
 
-    Measured (microseconds in a row; 8 kv heads with four heads each):
-      rows / columns, heads of 64: one token each, one sequence of 511 keys 4.6 / 6.0, 2,047 6.1 / 6.6, 8,191 11.7 / 9.5; 8 of 1,023
-        8.9 / 7.8, 8,191 23.4 / 16.4; 64 of 255 8.3 / 11.5, 511 12.7 / 13.6, 1,023 21.6 / 18.5, 8,191 118 / 96; 8 of 4,095, 16 rows
-        25 / 16.9, 24 rows 29 / 19.6; heads of 128: one sequence of 511 5.9 / 5.7, 8 of 1,023 10.9 / 8.6, 64 of 255 11.6 / 12.5,
-        8,191 221 / 157; 8 of 4,095, 16 rows 34 / 19.3, 24 rows 43 / 22.8;
-      columns / tcgen05, more rows: heads of 128, one of 4,095, 64 rows 16.8 / 20.0, 128 rows 17.8 / 22.5 (heads of 64, rows / tcgen05:
-        15.0 / 17.1 and 16.5 / 18.4); 8 of 4,095, 64 rows 40 / 38, 128 rows 78 / 45;
-      tcgen05 / dense, heads of 64: 4 of 16,000, 4 tiles of 128 rows 182 / 240, 6 tiles 340 / 287, 16 tiles 682 / 518; heads of
-        128: 216 / 353, 406 / 381, 798 / 666."""
+    Measured (``microbench attention_e4m3 --form ...``, microseconds in a row, over several caches in turn; 8 kv heads with four heads each):
+      rows / columns, heads of 64: one token each, one sequence of 511 keys 5.9 / 5.8, 2,047 6.3 / 6.8, 8,191 12.0 / 9.2; 8 of 1,023
+        7.0 / 7.4, 8,191 24.7 / 17.2; 64 of 255 9.3 / 12.9, 511 14.1 / 15.3, 1,023 22.8 / 20.6, 8,191 120 / 96; 8 of 4,095, 16 rows
+        27.6 / 15.4, 24 rows 29.6 / 18.4; heads of 128: one sequence of 511 7.1 / 6.5, 2,047 7.7 / 6.6, 8 of 1,023 10.2 / 8.8, 64 of 255
+        12.5 / 13.9, 8,191 224 / 159; 8 of 4,095, 16 rows 34.5 / 18.4, 24 rows 43.7 / 22.0;
+      columns / tcgen05, more rows: heads of 128, one of 4,095, 64 rows 14.9 / 19.1, 128 rows 16.3 / 21.9 (heads of 64, rows / tcgen05:
+        16.0 / 16.6 and 17.6 / 18.0); 8 of 4,095, 64 rows 37.2 / 36.8, 128 rows 73 / 43;
+      tcgen05 / dense, heads of 64: 4 of 16,000, 4 tiles of 128 rows 189 / 218, 6 tiles 360 / 260, 16 tiles 690 / 466; heads of
+        128: 207 / 361, 392 / 381, 752 / 661.
+    Heads of other sizes than 64, 128 and 256, and pages of other sizes than multiples of 16 where no other takes the call, go to "simt", a
+    warp a (token, head): 8 sequences of 2,048 keys, heads of 32 725, of 96 1,470 (heads of 64 9.2)."""
     return _launch().e4m3_form(dtype is torch.bfloat16, nq, nkv, d, page_size, scale, max_q_len, num_seqs, max_keys)
 
 

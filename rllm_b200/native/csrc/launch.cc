@@ -512,7 +512,7 @@ PyObject* e4m3_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
          *pks = THPVariable_Unpack(args[8]).data_ptr(), *pvs = THPVariable_Unpack(args[9]).data_ptr(), *pt = table.data_ptr();
     const cudaStream_t stream = stream_now();
     // Where no fewer sequences bring several tokens than one, and all of them few, they go together: one launch behind another costs
-    // more than the rows that single tokens leave empty (32/8 heads of 64, behind 4,000: 4 of one token and 4 of 5 24.4 -> 18.0 us; 16
+    // more than the rows that single tokens leave empty (32/8 heads of 64, behind 4,000: 4 of one token and 4 of 5 25.6 -> 18.7 us; 16
     // and 16 of 8 behind 2,000, more tiles of 32 rows than SMs, would be 30 -> 35).
     const long long few = max_q * (nq / nkv);
     const bool together_all = args[19] == Py_None && decode > 0 && S - decode >= decode && (few <= 16 || (few <= 32 && S * nkv <= 148));
