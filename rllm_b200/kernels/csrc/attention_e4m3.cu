@@ -229,7 +229,9 @@ attention_e4m3_rows_kernel(const T* q, int q_stride, T* __restrict__ out, const 
   // i % 16 (its first cache row / 16; -1: not held or behind the end): 16 pairs are looked up at a time, for a lookup a tile
   // would stand, as a second trip to memory, between a tile and its loads.
   const int page_tiles = page_size >> 4, page_shift = (page_tiles & (page_tiles - 1)) == 0 ? __ffs(page_tiles) - 1 : -1;
-  const int t_hi = (kend + 15) >> 4, stride = 2 * C * E4_WARPS, t0 = (kmin >> 4) + 2 * (rank * E4_WARPS + warp);
+  // A pair of tiles is a warp's by its place in the sequence, not in the tile of rows: see e4_rows_launch.
+  const int t_lo = kmin >> 4, t_hi = (kend + 15) >> 4, stride = 2 * C * E4_WARPS;
+  const int t0 = 2 * ((t_lo >> 1) + ((rank * E4_WARPS + warp - (t_lo >> 1)) & (C * E4_WARPS - 1)));
   const int pairs = t_hi > t0 ? (t_hi - t0 + stride - 1) / stride : 0;
   int places0 = -1, places1 = -1;      // of the even and the odd 16s: pairs on their way may lie 16 beyond the one at hand
   bool missing = false;                // a page of the warp's is not held (from where it is looked up on)
@@ -237,7 +239,7 @@ attention_e4m3_rows_kernel(const T* q, int q_stride, T* __restrict__ out, const 
     const int t = t0 + (i + (lane >> 1)) * stride + (lane & 1);
     int place = -1;
     bool bad = false;
-    if (t < t_hi) {
+    if (t >= t_lo && t < t_hi) {
       const int at = page_shift >= 0 ? t >> page_shift : t / page_tiles, page = bt[at];
       bad = page < 0 || page >= num_pages;
       if (!bad) place = (page * nkv + kvh) * page_tiles + (t - at * page_tiles);
@@ -701,8 +703,11 @@ static int e4_rows_launch(const void* q, int q_stride, void* out, const void* kc
   // CTAs a unit: to fill the GPU's places, of 128 keys at least (a CTA costs 2 us beside its keys); where there are enough of
   // them and keys are many, several rounds of CTAs, so that the last round is short beside the rest (64 sequences of 4,000 to
   // 12,000 keys, 32/8 heads of 128: 270 us with one CTA, 252 with two, 238 with four, 242 with eight)
-  int C = 1;
-  while (C < 8 && ((units * C * 2 <= 592 && C * 2 * 128 <= max_keys) || (units * C * 2 <= 2368 && C * 2 * 1024 <= max_keys))) C *= 2;
+  // float32: the same number whatever the call.  A row's keys then go to the same warps, and their results are added up in the same
+  // order, whoever else is in the step and however the prompt was cut: its result does not depend on them (nothing else of another
+  // row's enters: references are the row's own, and what they are multiplied by when they move is exact)
+  int C = sizeof(T) == 4 ? 4 : 1;
+  while (sizeof(T) == 2 && C < 8 && ((units * C * 2 <= 592 && C * 2 * 128 <= max_keys) || (units * C * 2 <= 2368 && C * 2 * 1024 <= max_keys))) C *= 2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)C, (unsigned)(tiles * nkv), (unsigned)num_seqs);
   cfg.blockDim = dim3(32 * E4_WARPS);

@@ -141,3 +141,37 @@ def test_keys_that_are_alike_weigh_the_same_however_large_scores_are(dtype, form
         got = out[at:at + n].double().view(n, 2, 4, d)
         assert ((got - mean).abs() <= bound).all(), float(((got - mean).abs() / bound).max())
         at += n
+
+
+@pytest.mark.parametrize("nq,nkv,d,page,window,total", [(8, 2, 64, 16, 0, 700), (8, 2, 64, 16, 100, 700), (32, 8, 128, 16, 0, 190), (8, 1, 256, 32, 33, 300),
+                                                        (24, 8, 128, 48, 500, 2100), (3, 3, 48, 4, 0, 90), (4, 4, 64, 8, 20, 130)])
+def test_a_float32_result_does_not_depend_on_the_step(nq, nkv, d, page, window, total):
+    """The last 40 tokens of a sequence in one portion, cut in any way, one by one, and beside others: the same bits."""
+    st = Step([40], [total - 40], nq, nkv, d, page, F32, seed=3, spread=1.5)
+    whole = st.attend(ops, window)
+    check(st, whole, window)
+    q, table, pages = st.q, st.table, st.pages
+
+    def step(parts, num_decode=None):
+        """Sequences over the same pages: (first, last) of the tokens of each."""
+        st.lens = [b - a for a, b in parts]
+        st.totals = [total - 40 + b for _, b in parts]
+        st.q = torch.cat([q[a:b] for a, b in parts])
+        st.q_start = torch.tensor([sum(st.lens[:i]) for i in range(len(parts) + 1)], dtype=torch.int32, device="cuda")
+        st.seq_lens = torch.tensor(st.totals, dtype=torch.int32, device="cuda")
+        st.table = table.expand(len(parts), -1).contiguous()
+        st.num_decode = next((i for i, n in enumerate(st.lens) if n != 1), len(parts))
+        out = st.attend(ops, window)
+        assert int(st.err) == 0
+        at = 0
+        for (a, b), n in zip(parts, st.lens):
+            assert torch.equal(out[at:at + n], whole[a:b]), (a, b)
+            at += n
+
+    for cut in ([0, 1, 2, 5, 21, 40], [0, 39, 40], [0, 8, 16, 24, 32, 40]):
+        for a, b in zip(cut, cut[1:]):
+            step([(a, b)])
+    step([(i, i + 1) for i in range(40)])
+    step([(0, 1)])
+    step([(3, 4)] * 70 + [(39, 40), (0, 40), (5, 9)])
+    step([(7, 8), (1, 4), (36, 40)])
